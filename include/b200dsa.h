@@ -638,6 +638,83 @@ int b200dsa_indexer_k_quant_and_cache(const void* k_bf16, const int64_t* slot_ma
                                       void* cache, int64_t num_pages, int32_t page_size, int32_t use_ue8m0,
                                       int32_t* status, void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Quantised latent cache: one row of 656 bytes for a token, slot s (= page * page_size + offset) at byte 656 * s:
+ * 512 e4m3 codes, four fp32 scales (one for 128 codes; value = code * scale), 64 bf16 position dims.  43 % fewer
+ * bytes than the bf16 row.  The reference keeps its latents in bf16 (OpenDSA/opendsa/ops/sparse_mla.py:39-43); its
+ * 8-bit counterpart in the reference is the index-key cache (b200dsa_indexer_k_quant_and_cache).
+ *
+ * b200dsa_latent_quant_and_cache: row t of kv (576 values, rows in_stride elements apart, bf16 or fp32 when in_f32)
+ *   is normalised over its 512 latent dims (n = c * rsqrt(mean(c^2) + eps) * gain; gain [512] bf16 or fp32, NULL = no
+ *   norm), its 64 position dims are rotated (cos / sin fp32 [n_tokens, 64], NULL = no rotation; half form
+ *   r_i c_i - r_{i+32} s_i, r_{i+32} c_{i+32} + r_i s_{i+32}, or with interleaved != 0 the pairs (2i, 2i+1) by c_i, s_i),
+ *   and the row is written to slot slot_mapping[t].  scale = max(amax, 1e-4) / 448, rounded up to a power of two when
+ *   use_ue8m0 != 0 (then code * scale is exact in bf16).  One pass, fp32 arithmetic, one rounding per stored number.
+ *   A negative slot is a padding token; a slot >= n_slots is skipped (status 2).  Slots of one call must be distinct:
+ *   which token a slot named twice ends up with is not defined.
+ * b200dsa_latent_cache_rows: out[i] = the bf16 row of slots[i] (code * scale rounded once); negative = zeros.
+ * b200dsa_latent_cache_gather: rows of requests in order: row i of request r (cu_rows[r] <= i < cu_rows[r+1]) is
+ *   position i - cu_rows[r] through block_table[r] (table_cols pages).  Rows from cu_rows[n_requests] on are left as
+ *   they are; a page outside the table or the cache gives a row of zeros and status 2.
+ * b200dsa_draft_tree_masks: masks[r, j] = bit i set for every node i on the path from node j to its root, j included;
+ *   parents int32 [n_trees, n_nodes], -1 = root, a parent before its children (else the path ends there, status 2);
+ *   at most 64 nodes.
+ * ------------------------------------------------------------------------------------- */
+int b200dsa_latent_quant_and_cache(const void* kv, int32_t in_f32, int64_t in_stride, int64_t n_tokens,
+                                   const void* gain, int32_t gain_f32, float eps, const float* cos, const float* sin,
+                                   int32_t interleaved, const int64_t* slot_mapping, void* cache, int64_t n_slots,
+                                   int32_t use_ue8m0, int32_t* status, void* stream);
+int b200dsa_latent_cache_rows(const void* cache, int64_t n_slots, const int64_t* slots, int64_t n_rows, void* out_bf16,
+                              int32_t* status, void* stream);
+int b200dsa_latent_cache_gather(const void* cache, int64_t n_slots, int32_t page_size, const int32_t* block_table,
+                                int64_t table_stride, int32_t table_cols, const int32_t* cu_rows, int32_t n_requests,
+                                int64_t n_rows, void* out_bf16, int32_t* status, void* stream);
+int b200dsa_draft_tree_masks(const int32_t* parents, int32_t n_trees, int32_t n_nodes, int64_t* masks, int32_t* status,
+                             void* stream);
+
+/* Sparse MLA attention over the quantised latent cache: b200dsa_sparse_mla_decode with the rows of an item's request
+ * read through its page table, and with drafted tokens as a tree.
+ *   keys of item i = its selected positions idx_j (0 <= idx_j <= q_pos[i] + q_pos_bias; < tree_base[request] when
+ *   tree_mask is given) and, with tree_mask, the positions tree_base[request] + b for every bit b of tree_mask[i]
+ *   (the drafted tokens stand in the cache behind the tree_base[request] committed ones).
+ *   cache / block_table / page_size as above (block_table [n_requests, table_stride], table_cols entries used);
+ *   row_request int32 [n_items], NULL = item i is request i;  indices int32 [n_items, idx_stride], -1 = none;
+ *   n_idx_item, q_pos optional;  ctx [n_items, n_heads, 512] bf16 or fp32;  lse fp32 [n_items, n_heads].
+ *   An item without keys gives ctx = 0 and lse = -inf.  A key without a page or outside the cache, and an item whose
+ *   request does not exist, are left out and reported (status 2).
+ * splits (1..32): every item's keys are cut into that many runs, merged by a second kernel; the caller lends
+ * splits * n_items * n_heads * 513 floats, which two calls in flight must not share.
+ * b200dsa_sparse_mla_decode_cached_splits is the number that fills the current device (1 = no workspace). */
+int b200dsa_sparse_mla_decode_cached_splits(int32_t n_items, int32_t n_heads, int32_t n_idx, int32_t tree);
+int b200dsa_sparse_mla_decode_cached(const void* q_bf16, const void* cache, int64_t n_slots, int32_t page_size,
+                                     const int32_t* block_table, int64_t table_stride, int32_t table_cols,
+                                     int32_t n_requests, const int32_t* row_request, const int32_t* indices,
+                                     int64_t idx_stride, int32_t n_idx, const int32_t* n_idx_item, const int32_t* q_pos,
+                                     int32_t q_pos_bias, const int64_t* tree_mask, const int32_t* tree_base,
+                                     int32_t n_items, int32_t n_heads, float sm_scale, void* ctx, int32_t ctx_bf16,
+                                     float* lse, int32_t splits, void* workspace, int64_t workspace_bytes,
+                                     int32_t* status, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * 8-bit products with block scales (the projections of DeepSeek-style checkpoints):
+ *   y[m, n] = sum_g sa[m, g] sw[n / 128, g] sum_{k in block g of 128} a[m, k] w[n, k]
+ * b200dsa_fp8_quantise_rows: x [m, k] bf16 / fp32 (rows in_stride elements apart) to e4m3 codes [m, k] and one scale
+ *   for 128 values of a row at scale[g * scale_ld + row]; scale = max(amax, 1e-10) / 448, or the power of two above.
+ * b200dsa_fp8_quantise_blocks: w [n, k] to codes and one scale for a 128 x 128 block, scale [ceil(n/128), ceil(k/128)].
+ * b200dsa_fp8_block_matmul: a [m, k], w [n, k] e4m3, strides in elements, scales at sa_m / sa_g and sw_r / sw_g; out
+ *   [m, n] bf16 or fp32 (rows out_stride elements apart).  fp32 accumulation; block products in the tensor pipe.
+ * k is a multiple of 16; operand rows start on 16-byte boundaries; m and n are arbitrary; the last blocks may be
+ * partial.  The reference's projections are torch Linears (OpenDSA/opendsa/modeling/indexer.py:60-63).
+ * ------------------------------------------------------------------------------------- */
+int b200dsa_fp8_quantise_rows(const void* x, int32_t in_f32, int64_t in_stride, int64_t m, int32_t k, int32_t use_ue8m0,
+                              void* q_e4m3, float* scale, int64_t scale_ld, void* stream);
+int b200dsa_fp8_quantise_blocks(const void* w, int32_t in_f32, int64_t in_stride, int32_t n, int32_t k,
+                                int32_t use_ue8m0, void* q_e4m3, float* scale, void* stream);
+int b200dsa_fp8_block_matmul(const void* a_e4m3, int64_t a_stride, const float* a_scale, int64_t sa_m, int64_t sa_g,
+                             const void* w_e4m3, int64_t w_stride, const float* w_scale, int64_t sw_r, int64_t sw_g,
+                             int32_t m, int32_t n, int32_t k, void* out, int32_t out_f32, int64_t out_stride,
+                             int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,431 @@
+"""Quantised latent cache: written, read back, and attended (also by trees of drafted tokens), against 64-bit
+definitions.  Bounds are derived: a stored or returned number is off by half a step of its type, a product of bf16
+probabilities by 2^-8 of the mass it sums, fp32 sums by their length times 2^-24."""
+import pytest
+import torch
+
+from oracle import latent_oracle as L
+
+pytestmark = pytest.mark.gpu
+
+E4M3, BF16, F32 = 2.0 ** -4, 2.0 ** -8, 2.0 ** -24
+DEV = "cuda"
+
+
+def _status():
+    from transarch_b200 import _lib
+    return _lib.read_status(torch.device(DEV))
+
+
+def random_cache(slots, g, pow2=True):
+    sc = torch.exp2(torch.randint(-9, -6, (slots, 4), generator=g).float())
+    if not pow2:
+        sc = sc * (1 + torch.rand(slots, 4, generator=g))
+    codes = (torch.randn(slots, 512, generator=g) * 110).clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
+    pe = (0.5 * torch.randn(slots, 64, generator=g)).bfloat16().view(torch.uint8)
+    return torch.cat([codes, sc.view(torch.uint8), pe], 1)
+
+
+def check_written(cache, slots, n, r):
+    """Rows of the cache against the 64-bit latent n and position dims r."""
+    v = L.cache_rows(cache, slots)
+    sc = L.cache_scales(cache, slots).double().repeat_interleave(128, 1)
+    assert bool(((v[:, :512] - n).abs() <= E4M3 * n.abs() * (1 + 1e-5) + sc * 2.0 ** -10 + 1e-6 * n.abs()).all())
+    # fp32 products of the rotation: two roundings of terms no larger than the pair's norm
+    size = torch.sqrt((r * r).sum(1, keepdim=True))
+    assert bool(((v[:, 512:] - r).abs() <= BF16 * r.abs() + 4 * F32 * size + 2.0 ** -133).all())
+    return sc
+
+
+@pytest.mark.parametrize("n,width,f32,norm,rope,offset", [
+    (1, 576, False, True, "pairs", 0), (5, 576, True, True, "half", 0), (64, 2112, False, True, "pairs", 1536),
+    (33, 700, False, False, "half", 13), (130, 600, True, True, None, 24), (7, 577, True, False, "pairs", 1)])
+def test_write(n, width, f32, norm, rope, offset):
+    """All forms, rows aligned and not, padding tokens; rows of other slots stay as they were."""
+    from transarch_b200 import kernels as K
+    g = torch.Generator().manual_seed(n + width)
+    page, pages = 16, n // 16 + 3
+    before = random_cache(pages * page, g)
+    raw = torch.randn(n, width, generator=g) * torch.exp(2 * torch.randn(n, 1, generator=g))
+    raw = raw if f32 else raw.bfloat16()
+    kv = raw[:, offset:offset + 576]
+    slots = torch.randperm(pages * page, generator=g)[:n]
+    if n > 4:
+        slots[2] = -1
+    gain = torch.randn(512, generator=g).to(torch.float32 if f32 else torch.bfloat16) if norm else None
+    pos = torch.randint(0, 160000, (n, 1), generator=g).double()
+    a = pos * 10000.0 ** (-torch.arange(32).double() / 32)
+    a = torch.cat([a, a], 1)
+    cos, sin = (a.cos().float(), a.sin().float()) if rope else (None, None)
+    cache = before.clone().to(DEV).view(pages, page * 656)
+    on = lambda t: None if t is None else t.to(DEV)
+    K.latent_quant_and_cache(raw.to(DEV)[:, offset:offset + 576], cache, slots.to(DEV), page, norm_weight=on(gain),
+                             eps=1e-5, cos=on(cos), sin=on(sin), interleaved=rope == "pairs")
+    assert _status() == 0
+    after = cache.cpu().view(-1, 656)
+    live = slots[slots >= 0]
+    other = torch.ones(pages * page, dtype=torch.bool)
+    other[live] = False
+    assert torch.equal(after[other], before[other])
+    nn, rr = L.norm_rotate(kv, gain, 1e-5, cos, sin, rope == "pairs")
+    keep = slots >= 0
+    sc = check_written(after, live, nn[keep], rr[keep])[:, ::128]
+    # power-of-two scales, the smallest that holds the group's largest value (fp32 arithmetic: 2^-20 either way)
+    top = nn[keep].view(-1, 4, 128).abs().amax(2).clamp_min(1e-4) / 448
+    assert torch.equal(torch.exp2(torch.log2(sc).round()), sc)
+    assert bool((sc >= top * (1 - 2.0 ** -20)).all()) and bool((sc < 2 * top * (1 + 2.0 ** -20)).all())
+
+
+def test_write_plain_scales_and_specials():
+    """scale_fmt None; a row of zeros, tiny and huge rows, NaN and infinity, a slot behind the cache."""
+    from transarch_b200 import kernels as K
+    g = torch.Generator().manual_seed(3)
+    kv = torch.randn(8, 576, generator=g)
+    kv[1] = 0
+    kv[2] *= 1e-30
+    kv[3] *= 1e30
+    kv[4, 7] = float("nan")
+    kv[5, 200] = float("inf")
+    slots = torch.tensor([9, 0, 3, 8, 5, 15, 16, 1])
+    cache = random_cache(16, g).to(DEV)
+    before = cache.cpu().clone()
+    K.latent_quant_and_cache(kv.to(DEV), cache, slots.to(DEV), 16, scale_fmt=None)
+    assert _status() == 2                                      # slot 16 does not exist
+    after = cache.cpu()
+    fine = [0, 1, 2, 3, 7]
+    check_written(after, slots[fine], kv[fine, :512].double(), kv[fine, 512:].double())
+    sc = L.cache_scales(after, slots[[0, 7]]).double()
+    top = kv[[0, 7], :512].double().view(2, 4, 128).abs().amax(2) / 448
+    assert bool(((sc - top).abs() <= F32 * top * 2).all())
+    v = L.cache_rows(after, slots[[4, 5]])
+    assert bool(torch.isnan(v[0, 7])) and bool(torch.isfinite(v[0, 128:512]).all())
+    assert bool(torch.isnan(v[1, 200])) and bool(torch.isfinite(v[1, :128]).all())
+    untouched = [s for s in range(16) if s not in slots.tolist()]
+    assert torch.equal(after[untouched], before[untouched])
+
+
+@pytest.mark.parametrize("n", [1, 3, 70])
+@pytest.mark.parametrize("pow2", [True, False])
+def test_rows_read_back(n, pow2):
+    from transarch_b200 import kernels as K
+    g = torch.Generator().manual_seed(n)
+    cache = random_cache(96, g, pow2)
+    slots = torch.randint(0, 96, (n,), generator=g)            # the same slot may be read twice
+    slots[0] = -1
+    out = K.latent_cache_rows(cache.to(DEV), slots.to(DEV), 32).cpu()
+    ref = L.cache_rows(cache, slots.clamp_min(0)).float().bfloat16()
+    ref[slots < 0] = 0
+    assert _status() == 0 and torch.equal(out, ref)
+    bad = slots.clone()
+    bad[-1] = 96
+    out = K.latent_cache_rows(cache.to(DEV), bad.to(DEV), 32).cpu()
+    assert _status() == 2 and bool((out[-1] == 0).all()) and torch.equal(out[:-1], ref[:-1])
+
+
+def test_gather_requests():
+    """Ragged requests, an empty one, a page outside the cache, rows behind the last request left alone."""
+    from transarch_b200 import kernels as K
+    g = torch.Generator().manual_seed(8)
+    page, lens = 16, [33, 0, 1, 16, 50] + [3] * 40
+    each = 4
+    pages = len(lens) * each
+    cache = random_cache(pages * page, g)
+    table = torch.randperm(pages, generator=g).view(len(lens), each).to(torch.int32)
+    cu = torch.zeros(len(lens) + 1, dtype=torch.int32)
+    cu[1:] = torch.tensor(lens).cumsum(0)
+    total = int(cu[-1])
+    refs = []
+    for r, n in enumerate(lens):
+        p = torch.arange(n)
+        refs.append(L.cache_rows(cache, table[r, p // page].long() * page + p % page).float().bfloat16())
+    ref = torch.cat(refs)
+    out = torch.full((total + 5, 576), 7.0, dtype=torch.bfloat16, device=DEV)
+    K.latent_cache_gather(cache.to(DEV), page, table.to(DEV), cu.to(DEV), total + 5, out=out)
+    assert _status() == 0
+    assert torch.equal(out[:total].cpu(), ref) and bool((out[total:] == 7).all())
+    # a wider table's slice as the block table; a page that does not exist
+    wide = torch.cat([table, torch.full((len(lens), 3), -5, dtype=torch.int32)], 1).to(DEV)
+    wide[4, 1] = pages
+    out = K.latent_cache_gather(cache.to(DEV), page, wide[:, :each], cu.to(DEV), total).cpu()
+    assert _status() == 2
+    hole = slice(int(cu[4]) + 16, int(cu[4]) + 32)
+    ref[hole] = 0
+    assert torch.equal(out, ref)
+
+
+def _tree(n, g):
+    parents = torch.full((n,), -1, dtype=torch.int32)
+    for j in range(1, n):
+        parents[j] = int(torch.randint(-1, j, (1,), generator=g))
+    return parents
+
+
+@pytest.mark.parametrize("trees,nodes", [(1, 1), (3, 7), (5, 64)])
+def test_tree_masks(trees, nodes):
+    from transarch_b200 import kernels as K
+    g = torch.Generator().manual_seed(nodes)
+    parents = torch.stack([_tree(nodes, g) for _ in range(trees)])
+    ref = torch.zeros(trees, nodes, dtype=torch.int64)
+    for r in range(trees):
+        for j in range(nodes):
+            at = j
+            while at >= 0:
+                ref[r, j] |= (1 << at) if at < 63 else -(1 << 63)
+                at = int(parents[r, at])
+    assert torch.equal(K.draft_tree_masks(parents.to(DEV)).cpu(), ref) and _status() == 0
+    if nodes > 2:
+        parents[0, 1] = 2                                      # a child before its parent: reported, the path ends
+        m = K.draft_tree_masks(parents.to(DEV)).cpu()
+        assert _status() == 2 and int(m[0, 1]) == 2
+
+
+def attend_case(seed, requests, per, H, k, ctx, page, drafts=0, holes=True, pow2=True):
+    g = torch.Generator().manual_seed(seed)
+    each = (ctx + drafts + page - 1) // page
+    pages = requests * each + 1
+    c = {"cache": random_cache(pages * page, g, pow2), "page": page, "scale": 192 ** -0.5,
+         "table": (torch.randperm(pages - 1, generator=g) + 1)[:requests * each].view(requests, each).to(torch.int32),
+         "q": torch.randn(requests * per, H, 576, generator=g).bfloat16(),
+         "req": torch.arange(requests, dtype=torch.int32).repeat_interleave(per),
+         "lens": torch.randint(1, ctx + 1, (requests,), generator=g).to(torch.int32)}
+    idx = torch.full((requests * per, k), -1, dtype=torch.int32)
+    for i in range(requests * per):
+        pick = torch.randperm(ctx, generator=g)[:k].to(torch.int32)
+        idx[i, :pick.numel()] = pick
+    if holes:
+        idx[:, 3::7] = -1
+    c["idx"] = idx
+    c["qpos"] = c["lens"][c["req"].long()] - 1 - torch.arange(per, dtype=torch.int32).repeat(requests) * (drafts == 0)
+    c["mask"] = None
+    if drafts:
+        masks = torch.zeros(requests * per, dtype=torch.int64)
+        for r in range(requests):
+            parents = _tree(drafts, g)
+            for j in range(per):
+                at = j % drafts
+                while at >= 0:
+                    masks[r * per + j] |= (1 << at) if at < 63 else -(1 << 63)
+                    at = int(parents[at])
+        c["mask"] = masks
+    return c
+
+
+def run_attend(c, **kw):
+    from transarch_b200 import kernels as K
+    d = {k: (v.to(DEV) if isinstance(v, torch.Tensor) else v) for k, v in c.items()}
+    return K.sparse_mla_decode_cached(d["q"], d["cache"], d["page"], d["idx"], d["scale"], block_table=d["table"],
+                                      row_request=d["req"], q_pos=d["qpos"], tree_mask=d["mask"],
+                                      tree_base=d["lens"] if d["mask"] is not None else None, **kw)
+
+
+def check_attend(c, ctx, lse, items=None, limit=None, pow2=True):
+    n, H, _ = c["q"].shape
+    widen = 0.0 if pow2 else BF16                             # a plain scale rounds the widened row once
+    for i in items if items is not None else range(n):
+        r = int(c["req"][i])
+        idx = c["idx"][i] if limit is None else c["idx"][i, :max(0, int(limit[i]))]
+        base = int(c["lens"][r]) if c["mask"] is not None else None
+        slots = L.item_keys(idx, c["table"][r], c["page"], int(c["qpos"][i]), base,
+                            None if c["mask"] is None else int(c["mask"][i]))
+        ref, ref_lse, mass, qk = L.attend(c["q"][i], L.cache_rows(c["cache"], slots), c["scale"])
+        k = max(1, slots.numel())
+        d = (576 * F32 + widen) * qk.view(-1, 1) + 1e-6       # error of a score; exp of it is relative
+        step = BF16 if ctx.dtype == torch.bfloat16 else F32
+        bound = (BF16 + widen + 2 * d + k * F32) * mass + step * ref.abs() + 1e-30
+        got = ctx[i].double().cpu()
+        assert bool(((got - ref).abs() <= bound).all()), (i, float(((got - ref).abs() / bound).max()))
+        got_lse = lse[i].double().cpu()
+        if slots.numel() == 0:
+            assert bool((got == 0).all()) and bool((got_lse == float("-inf")).all())
+        else:
+            lim = d.view(-1) + k * F32 + 8 * F32 * ref_lse.abs() + 2e-7
+            assert bool(((got_lse - ref_lse).abs() <= lim).all()), (i, float(((got_lse - ref_lse).abs() / lim).max()))
+
+
+@pytest.mark.parametrize("requests,per,H,k,ctx,page", [
+    (1, 1, 128, 1, 5, 16), (1, 1, 128, 2048, 4000, 64), (3, 1, 64, 64, 200, 16), (2, 3, 16, 100, 300, 32),
+    (5, 1, 1, 33, 50, 16), (40, 2, 128, 65, 130, 64), (2, 1, 65, 700, 900, 128), (160, 1, 128, 200, 400, 16)])
+def test_attend(requests, per, H, k, ctx, page):
+    c = attend_case(requests + k, requests, per, H, k, ctx, page)
+    out, lse = run_attend(c)
+    assert _status() == 0 and out.dtype == torch.bfloat16
+    check_attend(c, out, lse, items=range(0, requests * per, max(1, requests * per // 8)))
+
+
+@pytest.mark.parametrize("requests,nodes,H,k", [(1, 1, 128, 64), (2, 24, 16, 300), (3, 64, 128, 40), (2, 5, 64, 0)])
+def test_attend_tree(requests, nodes, H, k):
+    c = attend_case(nodes + k, requests, nodes, H, k, 400, 32, drafts=nodes)
+    out, lse = run_attend(c)
+    assert _status() == 0
+    check_attend(c, out, lse, items=range(0, requests * nodes, max(1, requests * nodes // 10)))
+
+
+@pytest.mark.parametrize("splits", [1, 2, 5, 32])
+def test_attend_splits_and_fp32(splits):
+    """Every number of splits gives the same attention; runs without a single key among them; fp32 result."""
+    from transarch_b200 import kernels as K
+    c = attend_case(11, 2, 2, 128, 1000, 1500, 64)
+    c["idx"][1, 64:640] = -1                                  # whole tiles without a key
+    c["idx"][2] = -1                                          # an item without keys
+    ws = (splits, torch.empty(splits * 4 * 128 * 513, device=DEV))
+    out32 = torch.empty(4, 128, 512, device=DEV)
+    out, lse = run_attend(c, ctx=out32, workspace=ws)
+    assert _status() == 0 and out.dtype == torch.float32
+    check_attend(c, out, lse)
+    out16, lse16 = run_attend(c, workspace=ws)
+    assert torch.equal(out16, out.bfloat16()) and torch.equal(lse16, lse)
+
+
+def test_attend_lengths_per_item():
+    """n_idx_item: only the first entries of a list count, none at all for a negative length."""
+    c = attend_case(12, 4, 1, 32, 300, 400, 16)
+    limit = torch.tensor([0, 1, 150, 999], dtype=torch.int32)
+    out, lse = run_attend(c, n_idx_item=limit.to(DEV))
+    assert _status() == 0
+    check_attend(c, out, lse, limit=limit)
+    limit[0] = -3
+    out2, lse2 = run_attend(c, n_idx_item=limit.to(DEV))
+    assert torch.equal(out2, out) and torch.equal(lse2, lse)
+
+
+def test_attend_plain_scales():
+    """Scales that are no powers of two: the widened row is rounded to bf16 once."""
+    c = attend_case(13, 2, 1, 128, 500, 900, 64, pow2=False)
+    out, lse = run_attend(c)
+    assert _status() == 0
+    check_attend(c, out, lse, pow2=False)
+
+
+def test_attend_growing_maximum():
+    """Keys whose scores keep growing: the accumulator is rescaled again and again."""
+    c = attend_case(14, 1, 1, 128, 512, 512, 64, holes=False)
+    c["lens"][:] = 512
+    c["qpos"][:] = 511
+    sc = torch.exp2(torch.linspace(-10, -4, 512).floor()).view(-1, 1).repeat(1, 4)
+    slots = L.item_keys(torch.arange(512), c["table"][0], 64, 511)
+    rows = c["cache"].clone()
+    rows[slots, 512:528] = sc.contiguous().view(torch.uint8)
+    c["cache"], c["scale"] = rows, 0.3
+    c["idx"] = torch.arange(512, dtype=torch.int32).view(1, -1)
+    out, lse = run_attend(c)
+    assert _status() == 0
+    check_attend(c, out, lse)
+    one = (1, None)                                           # and without splitting, where one CTA sees them all
+    out, lse = run_attend(c, workspace=one)
+    check_attend(c, out, lse)
+
+
+def test_attend_masked_places_may_hold_anything():
+    """NaN and infinities in rows that no item selects, and behind the mask, do not reach the result."""
+    c = attend_case(15, 2, 2, 64, 200, 300, 16, drafts=2)
+    used = set()
+    for i in range(4):
+        r = int(c["req"][i])
+        used |= set(L.item_keys(c["idx"][i], c["table"][r], 16, int(c["qpos"][i]), int(c["lens"][r]), int(c["mask"][i])).tolist())
+    rest = [s for s in range(c["cache"].shape[0]) if s not in used]
+    c["cache"][rest, :512] = 0x7f
+    c["cache"][rest, 512:528] = torch.full((1, 4), float("inf")).view(torch.uint8)
+    c["cache"][rest, 528:] = torch.full((1, 64), float("nan"), dtype=torch.bfloat16).view(torch.uint8)
+    out, lse = run_attend(c)
+    assert _status() == 0 and bool(torch.isfinite(out).all())
+    check_attend(c, out, lse)
+
+
+def test_attend_bad_pages_and_requests():
+    """A page outside the cache, a position outside the table and a request that does not exist: left out, reported."""
+    c = attend_case(16, 3, 1, 32, 100, 200, 16, holes=False)
+    c["lens"][:] = 200
+    c["qpos"][:] = 2 ** 30
+    pages = c["cache"].shape[0] // 16
+    bad = dict(c, table=c["table"].clone(), idx=c["idx"].clone(), req=c["req"].clone())
+    bad["table"][0, 2] = pages
+    bad["table"][0, 4] = -1
+    bad["idx"][1, 5] = 4000                                    # beyond the table
+    bad["req"][2] = 3
+    out, lse = run_attend(bad)
+    assert _status() == 2
+    good = dict(c, idx=c["idx"].clone())
+    lost = (good["idx"][0] // 16 == 2) | (good["idx"][0] // 16 == 4)
+    good["idx"][0][lost] = -1
+    good["idx"][1, 5] = -1
+    good["idx"][2] = -1
+    check_attend(good, out, lse)
+
+
+def test_cache_written_attended_and_read_in_one_stream():
+    """As a decode step uses it: new tokens written, then attended and read back, captured in a graph and replayed on
+    new inputs; another stream gives the same; two captured graphs do not share a workspace."""
+    from transarch_b200 import kernels as K
+    g = torch.Generator().manual_seed(21)
+    B, H, page, ctx = 4, 128, 64, 700
+    each = (ctx + page) // page
+    cache = random_cache(B * each * page, g).to(DEV)
+    table = torch.arange(B * each, dtype=torch.int32).view(B, each).to(DEV)
+    lens = torch.tensor([700, 1, 333, 64], dtype=torch.int32)
+    slots = torch.tensor([(int(table[b, (int(lens[b]) - 1) // page]) * page + (int(lens[b]) - 1) % page) for b in range(B)])
+    idx = torch.arange(704, dtype=torch.int32).repeat(B, 1).to(DEV)
+    kv = torch.randn(B, 576, generator=g).bfloat16()
+    q = torch.randn(B, H, 576, generator=g).bfloat16()
+    s_kv, s_q, s_slots, s_lens = kv.to(DEV), q.to(DEV), slots.to(DEV), lens.to(DEV)
+
+    def step():
+        K.latent_quant_and_cache(s_kv, cache, s_slots, page)
+        out, lse = K.sparse_mla_decode_cached(s_q, cache, page, idx, 0.1, block_table=table, q_pos=s_lens, q_pos_bias=-1)
+        return out, lse, K.latent_cache_rows(cache, s_slots, page)
+
+    def verify(out, lse, rows):
+        host = cache.cpu()
+        c = {"q": q, "idx": idx.cpu(), "req": torch.arange(B), "lens": lens, "qpos": lens - 1, "mask": None,
+             "table": table.cpu(), "page": page, "cache": host, "scale": 0.1}
+        check_attend(c, out, lse)
+        check_written(host, slots, kv[:, :512].double(), kv[:, 512:].double())
+        assert torch.equal(rows.cpu(), L.cache_rows(host, slots).float().bfloat16())
+
+    verify(*step())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    torch.cuda.current_stream().wait_stream(side)
+    verify(*got)
+    graphs = []
+    for _ in range(2):
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step()
+        graphs.append((graph, outs))
+    for turn in range(2):
+        kv.copy_(torch.randn(B, 576, generator=g).bfloat16())
+        q.copy_(torch.randn(B, H, 576, generator=g).bfloat16())
+        s_kv.copy_(kv)
+        s_q.copy_(q)
+        for graph, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, outs in graphs:
+            verify(*outs)
+    assert _status() == 0
+
+
+def test_long_cache_offsets():
+    """Slots whose byte offset passes 32 bits (a cache of 6.6 million tokens, 4.3 GB)."""
+    from transarch_b200 import kernels as K
+    slots_n = 6_600_000 // 64 * 64
+    cache = torch.zeros(slots_n, 656, dtype=torch.uint8, device=DEV)
+    g = torch.Generator().manual_seed(5)
+    kv = torch.randn(70, 576, generator=g).bfloat16()
+    slots = slots_n - 1 - torch.arange(70) * 3
+    K.latent_quant_and_cache(kv.to(DEV), cache, slots.to(DEV), 64)
+    part = cache[slots_n - 512:].cpu()
+    local = slots - (slots_n - 512)
+    check_written(part, local, kv[:, :512].double(), kv[:, 512:].double())
+    rows = K.latent_cache_rows(cache, slots.to(DEV), 64).cpu()
+    assert torch.equal(rows, L.cache_rows(part, local).float().bfloat16())
+    table = torch.tensor([[slots_n // 64 - 4 + i for i in range(4)]], dtype=torch.int32)
+    pos = (slots - (slots_n - 256)).to(torch.int32)
+    q = torch.randn(1, 128, 576, generator=g).bfloat16()
+    out, lse = K.sparse_mla_decode_cached(q.to(DEV), cache, 64, pos.view(1, -1).to(DEV), 0.05, block_table=table.to(DEV))
+    ref, ref_lse, mass, qk = L.attend(q[0], L.cache_rows(part, local), 0.05)
+    assert bool(((out[0].double().cpu() - ref).abs() <= (2 * BF16 + 1e-3) * mass + BF16 * ref.abs()).all())
+    assert _status() == 0

@@ -79,6 +79,18 @@ SIGNATURES = {
     "b200dsa_router_qnorm_topk": [_vp, _vp, _i32, _i32, _vp, _vp, _vp],
     "b200dsa_router_block_score_topk": [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp],
     "b200dsa_router_linear_topk_softmax": [_vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp],
+    "b200dsa_latent_quant_and_cache": [_vp, _i32, _i64, _i64, _vp, _i32, _f32, _vp, _vp, _i32, _vp, _vp, _i64, _i32, _vp,
+                                       _vp],
+    "b200dsa_latent_cache_rows": [_vp, _i64, _vp, _i64, _vp, _vp, _vp],
+    "b200dsa_latent_cache_gather": [_vp, _i64, _i32, _vp, _i64, _i32, _vp, _i32, _i64, _vp, _vp, _vp],
+    "b200dsa_draft_tree_masks": [_vp, _i32, _i32, _vp, _vp, _vp],
+    "b200dsa_sparse_mla_decode_cached_splits": [_i32, _i32, _i32, _i32],
+    "b200dsa_sparse_mla_decode_cached": [_vp, _vp, _i64, _i32, _vp, _i64, _i32, _i32, _vp, _vp, _i64, _i32, _vp, _vp, _i32,
+                                         _vp, _vp, _i32, _i32, _f32, _vp, _i32, _vp, _i32, _vp, _i64, _vp, _vp],
+    "b200dsa_fp8_quantise_rows": [_vp, _i32, _i64, _i64, _i32, _i32, _vp, _vp, _i64, _vp],
+    "b200dsa_fp8_quantise_blocks": [_vp, _i32, _i64, _i32, _i32, _i32, _vp, _vp, _vp],
+    "b200dsa_fp8_block_matmul": [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _i32, _i32, _i32, _vp, _i32, _i64,
+                                 _vp, _vp],
     "b200dsa_indexer_k_quant_and_cache": [_vp, _vp, _i64, _vp, _i64, _i32, _i32, _vp, _vp],
 }
 

@@ -1,0 +1,621 @@
+// Sparse MLA attention over the quantised, paged latent cache (rows of 656 bytes, latent_cache.cuh), with the drafted
+// tokens of a speculative step as a tree.
+//
+//   keys of an item:  the selected positions idx_j with  0 <= idx_j <= q_pos + q_pos_bias  (and idx_j < tree_base)
+//                     and, for a drafted token, the positions tree_base + i for every bit i of its ancestor mask
+//   s[h, j] = sm_scale * <q[h, 0:576], row_j>,  p = softmax_j(s),  ctx[h, :] = sum_j p[h, j] row_j[0:512],  lse[h]
+//
+// The tensor work is that of the bf16 kernel (sparse_mla_decode.cu: 64 heads a CTA as UMMA M, 64 keys a tile, O and two
+// score buffers and Q in TMEM, the row bytes read K-major by the scores and MN-major by the values).  What differs is
+// the way of a row into shared memory: 656 bytes come from HBM into registers, are widened to bf16 (exactly, when the
+// scales are powers of two) and stored in the 128-byte-swizzled layout of the MMA operands.  Eight warps do that, eight
+// rows of a tile each, lane l the codes 16l..16l+15 of a row; the loads of tile t+1 are issued row by row as the
+// registers of tile t are stored, so a tile's worth of tensor work covers their latency.  (Staging the codes in shared
+// memory by cp.async would add 2 x 42 KB of shared-memory traffic a tile to the 208 KB that the MMAs and the widened
+// rows take, and that port is already the second busiest unit.)
+//
+// A tree is one more tile: its 64 keys are the drafted positions in order, its validity bits are the mask itself.
+//
+// Work split: CTA = (item, 64-head half, split).  Small batches cut an item's tiles into `splits` runs whose partial
+// contexts (normalised, fp32) and log-sum-exps are merged by mla_merge_kernel; large ones have splits = 1 and no merge.
+//
+// Roles (416 threads): warps 0-7 rows, warps 8-11 softmax, warp 12 MMAs.  All waits are bounded.
+#include "latent_cache.cuh"
+#include "sparse_mla.cuh"
+
+namespace b200dsa {
+
+void set_last_error(const char* msg);
+
+constexpr int kMlcThreads = 416;
+constexpr int kMlcRowWarps = 8;
+constexpr int kMlcMaxSplits = 32;
+
+struct MlaCachedParams {
+  const __nv_bfloat16* q;        // [n_items, n_heads, 576]
+  const uint8_t* cache;
+  int64_t n_slots;
+  const int32_t* table;          // [n_requests, table_stride] pages
+  int64_t table_stride;
+  int table_cols, page_size, n_requests;
+  const int32_t* row_request;    // nullable [n_items]
+  const int32_t* indices;        // [n_items, idx_stride]
+  int64_t idx_stride;
+  int n_idx;
+  const int32_t* n_idx_item;     // nullable [n_items]
+  const int32_t* q_pos;          // nullable [n_items]
+  int q_pos_bias;
+  const int64_t* tree_mask;      // nullable [n_items]
+  const int32_t* tree_base;      // [n_requests] with tree_mask
+  int n_items, n_heads, halves, splits;
+  float scale_log2;
+  void* ctx;
+  int ctx_bf16;
+  float* lse;
+  float* part;                   // splits > 1: [splits, n_items, n_heads, 512] then [splits, n_items, n_heads]
+  int32_t* status;
+};
+
+__global__ void __launch_bounds__(kMlcThreads, 1)
+sparse_mla_cached_kernel(const MlaCachedParams p) {
+  pdl_launch_dependents();
+  pdl_wait_prior();
+  extern __shared__ uint8_t smem_dyn[];
+  __shared__ uint32_t s_tmem_base;
+  __shared__ int s_abort;
+  __shared__ uint32_t s_mask[kMlaStages][2];  // validity bit per key of the stage
+
+  const int split = blockIdx.x % p.splits;
+  const int hh = (blockIdx.x / p.splits) % p.halves;
+  const int item = blockIdx.x / (p.splits * p.halves);
+
+  const uint32_t smem_base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
+  uint8_t* smem_al = smem_dyn + (smem_base - smem_u32(smem_dyn));
+  const uint32_t kv_addr = smem_base;
+  const uint32_t p_addr = kv_addr + kMlaStages * kMlaStageBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem_al + kMlaStages * kMlaStageBytes + kMlaPBytes);
+  uint64_t* q_full = bars;                       // [1] Q sits in TMEM
+  uint64_t* s_full = bars + 1;                   // [2] score MMA retired
+  uint64_t* s_empty = bars + 3;                  // [2] 128 softmax threads have read the scores
+  uint64_t* p_full = bars + 5;                   // [1] 128 softmax threads: P written
+  uint64_t* pv_done = bars + 6;                  // [1] value MMA retired (P buffer free, O stable)
+  uint64_t* kv_full = bars + 7;                  // [stages] eight row warps
+  uint64_t* kv_empty = bars + 7 + kMlaStages;    // [stages] value MMA retired
+  uint64_t* q_land = bars + 7 + 2 * kMlaStages;  // [1] bytes of the Q rows
+
+  const int tid = threadIdx.x;
+  const int warp = tid >> 5;
+  const int lane = tid & 31;
+  const int n_idx = p.n_idx_item ? max(0, min(p.n_idx, p.n_idx_item[item])) : p.n_idx;
+  const int sel_tiles = (n_idx + kMlaTile - 1) / kMlaTile;
+  const int all_tiles = sel_tiles + (p.tree_mask ? 1 : 0);
+  // this CTA's run of tiles; below, t counts from its first one
+  const int tile0 = static_cast<int>(static_cast<int64_t>(all_tiles) * split / p.splits);
+  const int n_tiles = static_cast<int>(static_cast<int64_t>(all_tiles) * (split + 1) / p.splits) - tile0;
+  volatile int* abort_flag = &s_abort;
+
+  if (tid == 0) {
+    s_abort = 0;
+    mbar_init(q_full, 128);
+    for (int s = 0; s < kMlaStages; ++s) {
+      mbar_init(&kv_full[s], kMlcRowWarps);
+      mbar_init(&kv_empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&s_empty[s], 128);
+    }
+    mbar_init(p_full, 128);
+    mbar_init(pv_done, 1);
+    mbar_init(q_land, 1);
+    mbar_fence_init();
+  }
+  if (warp == 12) {
+    tmem_alloc(&s_tmem_base, kMlaTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = s_tmem_base;
+
+  if (warp < kMlcRowWarps) {
+    // ------------------------------------------------------------------ rows
+    const int32_t* idx_row = p.indices + static_cast<int64_t>(item) * p.idx_stride;
+    int req = p.row_request ? __ldg(p.row_request + item) : item;
+    bool known = req >= 0 && req < p.n_requests;
+    if (!known) {
+      if (tid == 0) atomicMax(p.status, kDevBadIndex);
+      req = 0;
+    }
+    const int32_t* table = p.table + static_cast<int64_t>(req) * p.table_stride;
+    const unsigned long long mask = p.tree_mask ? static_cast<unsigned long long>(__ldg(p.tree_mask + item)) : 0ull;
+    const int base = p.tree_mask ? __ldg(p.tree_base + req) : 0x7fffffff;
+    int64_t last = static_cast<int64_t>(base) - 1;    // the last position that may be attended by selection
+    if (p.q_pos) last = min(last, static_cast<int64_t>(__ldg(p.q_pos + item)) + p.q_pos_bias);
+    const int r0 = warp * 8;
+    // position of this lane's row of tile t (lanes 0..7), -1 = none
+    auto position = [&](int t) -> int {
+      if (lane >= 8 || t >= n_tiles || !known) return -1;
+      const int tt = tile0 + t;
+      if (tt < sel_tiles) {
+        const int j = tt * kMlaTile + r0 + lane;
+        const int v = j < n_idx ? __ldg(idx_row + j) : -1;
+        return v >= 0 && v <= last ? v : -1;
+      }
+      const int64_t v = static_cast<int64_t>(base) + r0 + lane;
+      return ((mask >> (r0 + lane)) & 1) && base >= 0 && v <= 0x7fffffff ? static_cast<int>(v) : -1;
+    };
+    // its slot in the cache, -1 = none (a page that does not exist is reported and left out)
+    auto slot_of = [&](int pos) -> int {
+      if (pos < 0) return -1;
+      const int col = pos / p.page_size;
+      const int page = col < p.table_cols ? __ldg(table + col) : -1;
+      const int64_t slot = static_cast<int64_t>(page) * p.page_size + (pos - col * p.page_size);
+      if (page < 0 || slot >= p.n_slots) {
+        atomicMax(p.status, kDevBadIndex);
+        return -1;
+      }
+      return static_cast<int>(slot);
+    };
+    uint4 code[8];
+    float scale[8];
+    uint4 pe[2];
+    const uint4 zero4 = make_uint4(0, 0, 0, 0);
+    auto load_row = [&](int slot, int i) {          // codes and scale of row i of the warp
+      const int s = __shfl_sync(0xffffffffu, slot, i);
+      const uint8_t* src = p.cache + static_cast<int64_t>(s < 0 ? 0 : s) * kLatentRowBytes;
+      code[i] = s < 0 ? zero4 : __ldg(reinterpret_cast<const uint4*>(src) + lane);
+      scale[i] = s < 0 ? 0.f : __ldg(reinterpret_cast<const float*>(src + 512) + (lane >> 3));
+    };
+    auto load_pe = [&](int slot, int j) {           // position dims: lane = chunk lane % 8 of row lane / 8 + 4 j
+      const int s = __shfl_sync(0xffffffffu, slot, (lane >> 3) + 4 * j);
+      const uint8_t* src = p.cache + static_cast<int64_t>(s < 0 ? 0 : s) * kLatentRowBytes + 528;
+      pe[j] = s < 0 ? zero4 : __ldg(reinterpret_cast<const uint4*>(src) + (lane & 7));
+    };
+    int slot = slot_of(position(0));
+    int pos_next = position(1);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) load_row(slot, i);
+    load_pe(slot, 0);
+    load_pe(slot, 1);
+    // Lane l stores 16-byte chunks 2 (l % 4) and 2 (l % 4) + 1 of the 128-byte chunk l / 4 of a row.  Lanes 4..7 of
+    // every eight store them in the other order, so that the eight lanes of a store phase hit eight different banks
+    // groups.
+    const int flip = (lane >> 2) & 1;
+    for (int t = 0; t < n_tiles; ++t) {
+      const int s = t % kMlaStages;
+      const unsigned vmask = __ballot_sync(0xffffffffu, lane < 8 && slot >= 0);
+      const int slot_next = slot_of(pos_next);
+      pos_next = position(t + 2);
+      bool ok = mbar_wait(&kv_empty[s], ((t / kMlaStages) & 1) ^ 1, abort_flag);
+      // the tail of the ring holds the Q rows until the softmax threads have moved them to TMEM
+      if (t < kMlaStages && (t + 1) * kMlaStageBytes > kMlaQStageOff) ok = ok && mbar_wait(q_full, 0, abort_flag);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      const uint32_t stage_addr = kv_addr + s * kMlaStageBytes;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        uint32_t w[8];
+        dequant_e4m3x4(code[i].x, scale[i], w[0], w[1]);
+        dequant_e4m3x4(code[i].y, scale[i], w[2], w[3]);
+        dequant_e4m3x4(code[i].z, scale[i], w[4], w[5]);
+        dequant_e4m3x4(code[i].w, scale[i], w[6], w[7]);
+        load_row(slot_next, i);
+        const uint32_t dst = stage_addr + (lane >> 2) * kMlaChunkBytesK + (r0 + i) * 128;
+        const uint32_t c0 = (((lane & 3) * 2 + flip) ^ i) << 4, c1 = (((lane & 3) * 2 + (flip ^ 1)) ^ i) << 4;
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + c0), "r"(flip ? w[4] : w[0]),
+                     "r"(flip ? w[5] : w[1]), "r"(flip ? w[6] : w[2]), "r"(flip ? w[7] : w[3]) : "memory");
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + c1), "r"(flip ? w[0] : w[4]),
+                     "r"(flip ? w[1] : w[5]), "r"(flip ? w[2] : w[6]), "r"(flip ? w[3] : w[7]) : "memory");
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int i = (lane >> 3) + 4 * j;
+        const uint32_t dst = stage_addr + 8 * kMlaChunkBytesK + (r0 + i) * 128 + (((lane & 7) ^ i) << 4);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(pe[j].x), "r"(pe[j].y), "r"(pe[j].z),
+                     "r"(pe[j].w) : "memory");
+        load_pe(slot_next, j);
+      }
+      if (lane == 0) reinterpret_cast<volatile uint8_t*>(&s_mask[s][0])[warp] = static_cast<uint8_t>(vmask);
+      __threadfence_block();
+      fence_proxy_async();               // the rows were written through the generic proxy; the MMAs read them
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&kv_full[s]);
+      slot = slot_next;
+    }
+  } else if (warp < 12) {
+    // ------------------------------------------------------------------ softmax
+    // lanes 16..31: score row `row`; lanes 0..15: the same row of O (partner lane = lane ^ 16)
+    const int wq = warp & 3;
+    const int row = wq * 16 + (lane & 15);          // head row inside this CTA's 64
+    const bool is_s = lane >= 16;
+    const uint32_t lane_addr = static_cast<uint32_t>(wq * 32) << 16;  // sub-partition base lane
+    float m_ref = -INFINITY, l = 0.f;
+    bool aborted = false;
+    {
+      // Q -> TMEM once: one bulk copy per head row into the tail of the key ring, which the row warps do not
+      // touch before q_full (rows padded by 16 bytes against bank conflicts; the last one spills into the P
+      // tile, unused so far), then lane 16+i stores head row 16*wq+i into the upper half-lanes (two bf16 per
+      // cell, 288 cells per row).  The lower half-lanes of these columns belong to O, not written yet.
+      const int qhead = hh * kMlaHeadsTile + row;
+      const bool have = is_s && qhead < p.n_heads;
+      const int rows_have = min(kMlaHeadsTile, p.n_heads - hh * kMlaHeadsTile);
+      if (warp == 8) {
+        if (lane == 0) mbar_arrive_expect_tx(q_land, static_cast<uint32_t>(rows_have) * (kMlaD * 2));
+        __syncwarp();
+        const __nv_bfloat16* q0 = p.q + (static_cast<int64_t>(item) * p.n_heads + hh * kMlaHeadsTile) * kMlaD;
+        for (int r = lane; r < rows_have; r += 32)
+          bulk_load_1d(smem_al + kMlaQStageOff + r * kMlaQRowBytes, q0 + static_cast<int64_t>(r) * kMlaD, kMlaD * 2, q_land);
+      }
+      const bool okq = mbar_wait(q_land, 0, abort_flag);
+      aborted = !__all_sync(0xffffffffu, okq);
+      if (aborted) {                    // the copies in flight land before the shared memory is given up
+        const long long t0 = clock64();
+        while (!mbar_test(q_land, 0) && clock64() - t0 < kWaitLimitCycles) {
+        }
+      }
+      const uint32_t qrow = smem_base + kMlaQStageOff + row * kMlaQRowBytes;
+#pragma unroll 1
+      for (int c = 0; c < kMlaD / 64 && !aborted; ++c) {
+        uint32_t qv[32];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (have) {
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(qv[4 * j]), "=r"(qv[4 * j + 1]), "=r"(qv[4 * j + 2]), "=r"(qv[4 * j + 3])
+                         : "r"(qrow + c * 128 + j * 16));
+          } else {
+            qv[4 * j] = qv[4 * j + 1] = qv[4 * j + 2] = qv[4 * j + 3] = 0u;
+          }
+        }
+        tmem_st_32x32(tmem_base + lane_addr + 128 + c * 32, qv);
+      }
+      tc_wait_st();
+      tc_fence_before();
+      mbar_arrive(q_full);
+    }
+    for (int t = 0; t < n_tiles && !aborted; ++t) {
+      const int sb = t & 1;
+      bool ok = mbar_wait(&s_full[sb], (t >> 1) & 1, abort_flag);
+      if (!__all_sync(0xffffffffu, ok)) { aborted = true; break; }
+      tc_fence_after();
+      const int ks = t % kMlaStages;
+      constexpr int kNV = kMlaTile / 32;   // 32-column groups per tile
+      uint32_t v[kNV][32];
+#pragma unroll
+      for (int h = 0; h < kNV; ++h)
+        tmem_ld_32x32(tmem_base + lane_addr + sb * kMlaTile + 32 * h, v[h]);   // lanes 16-31: score rows
+      tc_wait_ld();
+      float mt = -INFINITY;   // tile maximum of the raw scores, scaled once below (the scale is positive)
+#pragma unroll
+      for (int h = 0; h < kNV; ++h) {
+        const uint32_t mk = s_mask[ks][h];
+        if (mk == 0xffffffffu) {   // common case: all 32 keys of the group are valid
+#pragma unroll
+          for (int j = 0; j < 32; ++j) mt = fmaxf(mt, __uint_as_float(v[h][j]));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float a = ((mk >> j) & 1u) ? __uint_as_float(v[h][j]) : -INFINITY;
+            v[h][j] = __float_as_uint(a);
+            mt = fmaxf(mt, a);
+          }
+        }
+      }
+      mt *= p.scale_log2;
+      if (!is_s) mt = -INFINITY;
+      bool waited_pv = false;
+      // lazy rescale: only when the running maximum grows by more than 2^8
+      const bool grow = is_s && (mt > m_ref + 8.0f);
+      if (__any_sync(0xffffffffu, grow) && t > 0) {
+        ok = mbar_wait(pv_done, (t - 1) & 1, abort_flag);
+        if (!__all_sync(0xffffffffu, ok)) { aborted = true; break; }
+        waited_pv = true;
+        if (t + 1 < n_tiles) {
+          // the write-back below also touches the upper half-lanes of columns 0..127, where the
+          // next tile's scores may still be landing: let that MMA finish first
+          ok = mbar_wait(&s_full[(t + 1) & 1], ((t + 1) >> 1) & 1, abort_flag);
+          if (!__all_sync(0xffffffffu, ok)) { aborted = true; break; }
+        }
+        tc_fence_after();
+        float f = grow ? ((m_ref == -INFINITY) ? 0.f : exp2f(m_ref - mt)) : 1.0f;
+        if (is_s) l *= f;
+        f = __shfl_xor_sync(0xffffffffu, f, 16);   // O-row lanes take the factor of their partner
+#pragma unroll 1
+        for (int c = 0; c < kMlaDv / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld_32x32(tmem_base + lane_addr + kMlaTmemO + c * 32, o);
+          tc_wait_ld();
+          if (!is_s) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+          }
+          // upper lanes write back what they read (score buffers and unused cells)
+          tmem_st_32x32(tmem_base + lane_addr + kMlaTmemO + c * 32, o);
+        }
+        tc_wait_st();
+        tc_fence_before();
+      }
+      // Only now may the score issuer overwrite this buffer (two tiles ahead): the write-back of a
+      // rescale above also touches the score cells.
+      tc_fence_before();
+      mbar_arrive(&s_empty[sb]);
+      if (grow) m_ref = mt;
+      uint32_t pk[kMlaTile / 2];
+      float lsum = 0.f;
+      // p = 2^(s*scale - m_ref) as one FMA and one ex2; masked scores are -inf and give exactly 0
+      const float neg_m = (m_ref == -INFINITY) ? 0.f : -m_ref;
+#pragma unroll
+      for (int h = 0; h < kNV; ++h) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+          const float p0 = fast_exp2(fmaf(__uint_as_float(v[h][j]), p.scale_log2, neg_m));
+          const float p1 = fast_exp2(fmaf(__uint_as_float(v[h][j + 1]), p.scale_log2, neg_m));
+          lsum += p0 + p1;
+          __nv_bfloat162 h01 = __floats2bfloat162_rn(p0, p1);
+          pk[16 * h + (j >> 1)] = *reinterpret_cast<uint32_t*>(&h01);
+        }
+      }
+      if (is_s) l += lsum;
+      if (t > 0 && !waited_pv) {
+        ok = mbar_wait(pv_done, (t - 1) & 1, abort_flag);
+        if (!__all_sync(0xffffffffu, ok)) { aborted = true; break; }
+      }
+      if (is_s) {
+        // P row (tile bf16) as core-matrix rows of 16 bytes: (row/8)*(tile/8*128) + c*128 + (row%8)*16
+        const uint32_t prow = p_addr + (row >> 3) * (kMlaTile / 8 * 128) + (row & 7) * 16;
+#pragma unroll
+        for (int c = 0; c < kMlaTile / 8; ++c) {
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(prow + c * 128), "r"(pk[4 * c]),
+                       "r"(pk[4 * c + 1]), "r"(pk[4 * c + 2]), "r"(pk[4 * c + 3])
+                       : "memory");
+        }
+      }
+      fence_proxy_async();
+      mbar_arrive(p_full);
+    }
+    // ---- output: lanes 0..15 own the O rows; l and m_ref come from the partner lane
+    const float l_o = __shfl_xor_sync(0xffffffffu, l, 16);
+    const float m_o = __shfl_xor_sync(0xffffffffu, m_ref, 16);
+    const int head = hh * kMlaHeadsTile + row;
+    const int64_t out_row = static_cast<int64_t>(item) * p.n_heads + head;
+    const int64_t part_row = static_cast<int64_t>(split) * p.n_items * p.n_heads + out_row;
+    const bool write = !is_s && head < p.n_heads && !aborted;
+    // a split writes its normalised fp32 part and its log-sum-exp
+    const bool to_bf16 = p.splits == 1 && p.ctx_bf16;
+    float* ctx_row = p.splits == 1 ? static_cast<float*>(p.ctx) + out_row * kMlaDv : p.part + part_row * kMlaDv;
+    __nv_bfloat16* ctx_row_h = static_cast<__nv_bfloat16*>(p.ctx) + out_row * kMlaDv;
+    float* lse_out = p.splits == 1 ? p.lse + out_row
+                                   : p.part + static_cast<int64_t>(p.splits) * p.n_items * p.n_heads * kMlaDv + part_row;
+    bool ok = !aborted;
+    if (ok && n_tiles > 0) ok = __all_sync(0xffffffffu, mbar_wait(pv_done, (n_tiles - 1) & 1, abort_flag));
+    if (ok) {
+      tc_fence_after();
+      const bool any = n_tiles > 0 && l_o != 0.f;       // a NaN sum stays NaN in the result
+      const float inv = any ? 1.0f / l_o : 0.f;
+#pragma unroll 1
+      for (int c = 0; c < kMlaDv / 32; ++c) {
+        uint32_t o[32];
+        if (n_tiles > 0) {
+          tmem_ld_32x32(tmem_base + lane_addr + kMlaTmemO + c * 32, o);
+          tc_wait_ld();
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) o[j] = any ? __float_as_uint(__uint_as_float(o[j]) * inv) : 0u;
+        if (write && to_bf16) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 8) {
+            uint4 v;
+            v.x = pack_bf16x2(__uint_as_float(o[j]), __uint_as_float(o[j + 1]));
+            v.y = pack_bf16x2(__uint_as_float(o[j + 2]), __uint_as_float(o[j + 3]));
+            v.z = pack_bf16x2(__uint_as_float(o[j + 4]), __uint_as_float(o[j + 5]));
+            v.w = pack_bf16x2(__uint_as_float(o[j + 6]), __uint_as_float(o[j + 7]));
+            *reinterpret_cast<uint4*>(ctx_row_h + c * 32 + j) = v;
+          }
+        } else if (write) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 4)
+            *reinterpret_cast<uint4*>(ctx_row + c * 32 + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+        }
+      }
+      tc_fence_before();
+      if (write) *lse_out = any ? (m_o + log2f(l_o)) * 0.6931471805599453f : -INFINITY;
+    }
+  } else {
+    // ------------------------------------------------------------------ MMA issuer (warp 12)
+    // One warp issues everything, in the order S(0), S(1), PV(0), S(2), PV(1), ...: the tensor pipe runs
+    // its instructions in issue order, so S(t+1) keeps it busy while the softmax of tile t runs, and the
+    // ring stage that PV(t-1) frees is not needed before S(t+2), a whole tile of tensor work later, which
+    // is the time the gather of tile t+2 has to land.  (Issuing the scores as early as their buffers allow
+    // puts S(t+2) directly behind PV(t-1) and exposes the whole gather latency on every tile.)
+    constexpr uint32_t idesc_s = make_idesc(kFmtBF16, kFmtBF16, kMlaHeadsTile, kMlaTile);
+    constexpr uint32_t idesc_pv = make_idesc(kFmtBF16, kFmtBF16, kMlaHeadsTile, 256, 0, 1);
+    auto issue_scores = [&](int t) -> bool {
+      const int s = t % kMlaStages, sb = t & 1;
+      const bool w = mbar_wait(&kv_full[s], (t / kMlaStages) & 1, abort_flag) &&
+                     mbar_wait(&s_empty[sb], ((t >> 1) & 1) ^ 1, abort_flag);
+      if (!__all_sync(0xffffffffu, w)) return false;
+      fence_proxy_async();  // gathered rows were written through the generic proxy
+      tc_fence_after();
+      if (elect_one()) {
+        const uint32_t d = tmem_base + kMlaTmemS + sb * kMlaTile;
+        // descriptors differ only in the 16-byte-granular start address: one add per operand
+        const uint64_t b0 = make_desc_k_sw128(kv_addr + s * kMlaStageBytes);
+#pragma unroll
+        for (int c = 0; c < kMlaChunks; ++c) {
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {
+            mma_f16_ts(d, tmem_base + kMlaTmemQ + c * 32 + kk * 8, b0 + ((c * kMlaChunkBytesK + kk * 32) >> 4),
+                       idesc_s, (c | kk) != 0);
+          }
+        }
+        tc_commit(&s_full[sb]);
+      }
+      __syncwarp();
+      return true;
+    };
+    bool ok = mbar_wait(q_full, 0, abort_flag);
+    ok = __all_sync(0xffffffffu, ok);
+    if (ok && n_tiles > 0) ok = issue_scores(0);
+    for (int t = 0; ok && t < n_tiles; ++t) {
+      if (t + 1 < n_tiles && !issue_scores(t + 1)) break;
+      const int s = t % kMlaStages;
+      const bool w = mbar_wait(p_full, t & 1, abort_flag);
+      if (!__all_sync(0xffffffffu, w)) break;
+      fence_proxy_async();
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t pa0 = make_desc_k_noswz(p_addr, 128, kMlaTile / 8 * 128);
+        const uint64_t vb0 = make_desc_mn_sw128(kv_addr + s * kMlaStageBytes, kMlaChunkBytesK, 1024);
+#pragma unroll
+        for (int j = 0; j < kMlaTile / 16; ++j) {  // 16 keys per MMA
+#pragma unroll
+          for (int nh = 0; nh < 2; ++nh) {        // value dims [256*nh, 256*nh+256)
+            mma_f16_ss(tmem_base + kMlaTmemO + nh * 256, pa0 + ((j * 256) >> 4),
+                       vb0 + (((4 * nh) * kMlaChunkBytesK + j * 2048) >> 4), idesc_pv, (t | j) != 0);
+          }
+        }
+        tc_commit(&kv_empty[s]);
+        tc_commit(pv_done);
+      }
+      __syncwarp();
+    }
+  }
+
+  // ---------------------------------------------------------------------- common tail
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 12) tmem_dealloc(tmem_base, kMlaTmemCols);
+  if (tid == 0 && s_abort) atomicMax(p.status, kDevWaitTimeout);
+}
+
+// Merge of the splits of a (item, head) row: weights exp(lse_s - max), parts without a key left out.  One CTA a row,
+// four dims a thread.
+__global__ void __launch_bounds__(128) mla_merge_kernel(const float* __restrict__ part, int n_rows, int splits,
+                                                        void* __restrict__ ctx, int ctx_bf16, float* __restrict__ lse) {
+  pdl_launch_dependents();
+  pdl_wait_prior();
+  const int row = blockIdx.x;
+  const float* part_lse = part + static_cast<int64_t>(splits) * n_rows * kMlaDv;
+  float top = -INFINITY;
+  for (int s = 0; s < splits; ++s) top = fmaxf(top, __ldg(part_lse + static_cast<int64_t>(s) * n_rows + row));
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float den = 0.f;
+#pragma unroll 8
+  for (int s = 0; s < splits; ++s) {
+    const float l = __ldg(part_lse + static_cast<int64_t>(s) * n_rows + row);
+    const float4 v = __ldg(reinterpret_cast<const float4*>(part + (static_cast<int64_t>(s) * n_rows + row) * kMlaDv) + threadIdx.x);
+    if (l != -INFINITY) {
+      const float w = expf(l - top);
+      den += w;
+      acc.x = fmaf(w, v.x, acc.x); acc.y = fmaf(w, v.y, acc.y);
+      acc.z = fmaf(w, v.z, acc.z); acc.w = fmaf(w, v.w, acc.w);
+    }
+  }
+  const float inv = den != 0.f ? 1.0f / den : 0.f;   // a NaN denominator stays one
+  acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
+  const int64_t at = static_cast<int64_t>(row) * kMlaDv + threadIdx.x * 4;
+  if (ctx_bf16) {
+    uint2 o;
+    o.x = pack_bf16x2(acc.x, acc.y);
+    o.y = pack_bf16x2(acc.z, acc.w);
+    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(ctx) + at) = o;
+  } else {
+    *reinterpret_cast<float4*>(static_cast<float*>(ctx) + at) = acc;
+  }
+  if (threadIdx.x == 0) lse[row] = den != 0.f ? top + logf(den) : -INFINITY;
+}
+
+static int mlc_rc(cudaError_t e) {
+  if (e == cudaSuccess) return B200DSA_OK;
+  set_last_error(cudaGetErrorString(e));
+  return B200DSA_ECUDA;
+}
+
+}  // namespace b200dsa
+
+using namespace b200dsa;
+
+extern "C" int b200dsa_sparse_mla_decode_cached_splits(int32_t n_items, int32_t n_heads, int32_t n_idx, int32_t tree) {
+  if (n_items < 1 || n_heads < 1 || n_idx < 0) return 1;
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int64_t ctas = static_cast<int64_t>(n_items) * (n_heads > kMlaHeadsTile ? 2 : 1);
+  const int tiles = (n_idx + kMlaTile - 1) / kMlaTile + (tree ? 1 : 0);
+  int64_t splits = sms / ctas;
+  if (splits > tiles / 2) splits = tiles / 2;          // a run of one tile costs as much in prologue and merge as it saves
+  if (splits > kMlcMaxSplits) splits = kMlcMaxSplits;
+  return splits < 1 ? 1 : static_cast<int>(splits);
+}
+
+extern "C" int b200dsa_sparse_mla_decode_cached(const void* q_bf16, const void* cache, int64_t n_slots, int32_t page_size,
+                                                const int32_t* block_table, int64_t table_stride, int32_t table_cols,
+                                                int32_t n_requests, const int32_t* row_request, const int32_t* indices,
+                                                int64_t idx_stride, int32_t n_idx, const int32_t* n_idx_item,
+                                                const int32_t* q_pos, int32_t q_pos_bias, const int64_t* tree_mask,
+                                                const int32_t* tree_base, int32_t n_items, int32_t n_heads,
+                                                float sm_scale, void* ctx, int32_t ctx_bf16, float* lse, int32_t splits,
+                                                void* workspace, int64_t workspace_bytes, int32_t* status,
+                                                void* stream) {
+  if (n_items == 0) return B200DSA_OK;
+  if (!q_bf16 || !cache || !block_table || (!indices && n_idx > 0) || !ctx || !lse || !status || n_items < 0 ||
+      n_heads < 1 || n_heads > kMlaMaxHeads || n_idx < 0 || idx_stride < n_idx || n_slots < 1 ||
+      n_slots > 0x7fffffffll || page_size < 1 || table_cols < 1 || table_stride < table_cols || n_requests < 1 ||
+      (!row_request && n_requests < n_items) || !(sm_scale > 0.f) || (tree_mask && !tree_base) || splits < 1 || splits > kMlcMaxSplits ||
+      static_cast<int64_t>(n_items) * 2 * splits > 0x7fffffffll) {
+    set_last_error("b200dsa_sparse_mla_decode_cached: bad argument (1 <= n_heads <= 128, 1 <= splits <= 32, "
+                   "idx_stride >= n_idx, sm_scale > 0, a request for every item)");
+    return B200DSA_EINVAL;
+  }
+  const int64_t rows = static_cast<int64_t>(n_items) * n_heads;
+  if (splits > 1 && (!workspace || workspace_bytes < rows * splits * (kMlaDv + 1) * 4)) {
+    set_last_error("b200dsa_sparse_mla_decode_cached: the workspace is smaller than splits * n_items * n_heads * 513 floats");
+    return B200DSA_EINVAL;
+  }
+  if ((reinterpret_cast<uintptr_t>(q_bf16) & 15) || (reinterpret_cast<uintptr_t>(cache) & 15) ||
+      (reinterpret_cast<uintptr_t>(ctx) & 15) || (splits > 1 && (reinterpret_cast<uintptr_t>(workspace) & 15))) {
+    set_last_error("b200dsa_sparse_mla_decode_cached: q, cache, ctx and workspace must be 16-byte aligned");
+    return B200DSA_EALIGN;
+  }
+  cudaError_t e = cudaFuncSetAttribute(sparse_mla_cached_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMlaSmemBytes);
+  if (e != cudaSuccess) return mlc_rc(e);
+  MlaCachedParams p{};
+  p.q = static_cast<const __nv_bfloat16*>(q_bf16);
+  p.cache = static_cast<const uint8_t*>(cache);
+  p.n_slots = n_slots;
+  p.table = block_table;
+  p.table_stride = table_stride;
+  p.table_cols = table_cols;
+  p.page_size = page_size;
+  p.n_requests = n_requests;
+  p.row_request = row_request;
+  p.indices = indices;
+  p.idx_stride = idx_stride;
+  p.n_idx = n_idx;
+  p.n_idx_item = n_idx_item;
+  p.q_pos = q_pos;
+  p.q_pos_bias = q_pos_bias;
+  p.tree_mask = tree_mask;
+  p.tree_base = tree_base;
+  p.n_items = n_items;
+  p.n_heads = n_heads;
+  p.halves = n_heads > kMlaHeadsTile ? 2 : 1;
+  p.splits = splits;
+  p.scale_log2 = sm_scale * 1.4426950408889634f;
+  p.ctx = ctx;
+  p.ctx_bf16 = ctx_bf16 != 0;
+  p.lse = lse;
+  p.part = static_cast<float*>(workspace);
+  p.status = status;
+  e = launch_chained(sparse_mla_cached_kernel, dim3(n_items * p.halves * splits), dim3(kMlcThreads), kMlaSmemBytes,
+                     static_cast<cudaStream_t>(stream), p);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e == cudaSuccess && splits > 1) {
+    e = launch_chained(mla_merge_kernel, dim3(static_cast<unsigned>(rows)), dim3(128), 0,
+                       static_cast<cudaStream_t>(stream), static_cast<const float*>(p.part), static_cast<int>(rows),
+                       static_cast<int>(splits), ctx, static_cast<int>(ctx_bf16 != 0), lse);
+    if (e == cudaSuccess) e = cudaGetLastError();
+  }
+  return mlc_rc(e);
+}
