@@ -652,6 +652,8 @@ int b200dsa_indexer_k_quant_and_cache(const void* k_bf16, const int64_t* slot_ma
  *   use_ue8m0 != 0 (then code * scale is exact in bf16).  One pass, fp32 arithmetic, one rounding per stored number.
  *   A negative slot is a padding token; a slot >= n_slots is skipped (status 2).  Slots of one call must be distinct:
  *   which token a slot named twice ends up with is not defined.
+ *   A group with a value that is not finite gets scale NaN: it reads as NaN throughout (the codes 0x7f and 0xff, e4m3's
+ *   own NaN, mean nothing in the cache).
  * b200dsa_latent_cache_rows: out[i] = the bf16 row of slots[i] (code * scale rounded once); negative = zeros.
  * b200dsa_latent_cache_gather: rows of requests in order: row i of request r (cu_rows[r] <= i < cu_rows[r+1]) is
  *   position i - cu_rows[r] through block_table[r] (table_cols pages).  Rows from cu_rows[n_requests] on are left as
@@ -714,6 +716,13 @@ int b200dsa_fp8_block_matmul(const void* a_e4m3, int64_t a_stride, const float* 
                              const void* w_e4m3, int64_t w_stride, const float* w_scale, int64_t sw_r, int64_t sw_g,
                              int32_t m, int32_t n, int32_t k, void* out, int32_t out_f32, int64_t out_stride,
                              int32_t* status, void* stream);
+/* b200dsa_fp8_quantise_rows and b200dsa_fp8_block_matmul on its result in one call (the product's kernel becomes
+ * resident while the quantiser drains).  workspace: m * (k + 4 * ceil(k / 128)) bytes, 16-byte aligned, not shared by
+ * two calls in flight. */
+int b200dsa_fp8_block_linear(const void* x, int32_t in_f32, int64_t in_stride, int32_t use_ue8m0, const void* w_e4m3,
+                             int64_t w_stride, const float* w_scale, int64_t sw_r, int64_t sw_g, int32_t m, int32_t n,
+                             int32_t k, void* out, int32_t out_f32, int64_t out_stride, void* workspace,
+                             int64_t workspace_bytes, int32_t* status, void* stream);
 
 #ifdef __cplusplus
 }

@@ -91,6 +91,8 @@ SIGNATURES = {
     "b200dsa_fp8_quantise_blocks": [_vp, _i32, _i64, _i32, _i32, _i32, _vp, _vp, _vp],
     "b200dsa_fp8_block_matmul": [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _i32, _i32, _i32, _vp, _i32, _i64,
                                  _vp, _vp],
+    "b200dsa_fp8_block_linear": [_vp, _i32, _i64, _i32, _vp, _i64, _vp, _i64, _i64, _i32, _i32, _i32, _vp, _i32, _i64, _vp,
+                                 _i64, _vp, _vp],
     "b200dsa_indexer_k_quant_and_cache": [_vp, _vp, _i64, _vp, _i64, _i32, _i32, _vp, _vp],
 }
 
@@ -132,7 +134,8 @@ def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 
 def stream_ptr() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """Current stream of the current device (the raw handle: building a Stream object costs 3 us a call)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def check(rc: int, what: str) -> None:
@@ -156,6 +159,17 @@ def status_word(device: torch.device) -> torch.Tensor:
     if key not in _status_words:
         _status_words[key] = torch.zeros(1, dtype=torch.int32, device=device)
     return _status_words[key]
+
+
+_status_ptrs = {}
+
+
+def status_ptr(index: int) -> int:
+    """Address of the status word of CUDA device `index`."""
+    p = _status_ptrs.get(index)
+    if p is None:
+        p = _status_ptrs[index] = status_word(torch.device("cuda", index)).data_ptr()
+    return p
 
 
 def read_status(device: torch.device) -> int:

@@ -6,6 +6,8 @@
 #include <cuda.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/b200dsa.h"
 
 namespace b200dsa {
@@ -255,6 +257,25 @@ inline cudaError_t launch_chained(void (*kernel)(KArgs...), dim3 grid, dim3 bloc
   cfg.numAttrs = pdl_enabled() ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
+
+// The current device and its SM count (cached: the query costs more than a launch's share of a short call).
+struct DeviceInfo {
+  int index, sms;
+};
+cudaError_t current_device_info(DeviceInfo* out);   // runtime.cu
+
+// Runs a set-up call (a kernel's shared-memory opt-in) once for every device.  Two threads may both run it.
+struct OncePerDevice {
+  std::atomic<uint64_t> done{0};
+  template <typename F>
+  cudaError_t run(int device, F f) {
+    const uint64_t bit = 1ull << (device & 63);
+    if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+    const cudaError_t e = f();
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return e;
+  }
+};
 
 // In-place inclusive prefix sum of counts[1..n] (counts[0] stays 0), run by ONE full warp: every lane adds up a
 // run of consecutive entries, a shuffle scan joins the runs.  The run length is odd so that the lanes walk

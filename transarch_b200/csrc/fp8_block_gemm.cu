@@ -103,7 +103,6 @@ fp8_block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
                       const GemmParams p) {
   using S = GemmShape<NT>;
   pdl_launch_dependents();
-  pdl_wait_prior();
   extern __shared__ uint8_t smem_dyn[];
   __shared__ uint32_t s_tmem_base;
   __shared__ int s_abort;
@@ -143,6 +142,7 @@ fp8_block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = s_tmem_base;
+  pdl_wait_prior();      // nothing above touches global memory: as a dependent launch it overlaps the previous kernel
 
   // tiles: neighbouring CTAs share a token tile's neighbours in N, i.e. the same activations
   const int n_work = p.m_tiles * p.n_tiles;
@@ -330,11 +330,15 @@ fp8_block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
 }
 
 template <int NT>
-static cudaError_t gemm_launch(const CUtensorMap& mw, const CUtensorMap& ma, const GemmParams& p, int sms,
-                               cudaStream_t stream) {
+static cudaError_t gemm_launch(const CUtensorMap& mw, const CUtensorMap& ma, const GemmParams& p, const DeviceInfo& dev,
+                               bool dependent, cudaStream_t stream) {
   using S = GemmShape<NT>;
-  cudaError_t e = cudaFuncSetAttribute(fp8_block_gemm_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+  static OncePerDevice once;
+  cudaError_t e = once.run(dev.index, [] {
+    return cudaFuncSetAttribute(fp8_block_gemm_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+  });
   if (e != cudaSuccess) return e;
+  const int sms = dev.sms;
   const int tiles = p.m_tiles * p.n_tiles;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(p.splits > 1 ? tiles * p.splits : (tiles < sms ? tiles : sms));
@@ -350,7 +354,7 @@ static cudaError_t gemm_launch(const CUtensorMap& mw, const CUtensorMap& ma, con
     attr[na].val.clusterDim.z = 1;
     ++na;
   }
-  if (pdl_enabled()) {
+  if (dependent || pdl_enabled()) {
     attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[na].val.programmaticStreamSerializationAllowed = 1;
     ++na;
@@ -508,13 +512,6 @@ static void gemm_plan(int m, int n, int blocks, int sms, int* nt_out, int* split
   *splits_out = best_s;
 }
 
-static int sm_count(int* sms) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
-  return gemm_rc(e);
-}
-
 }  // namespace b200dsa
 
 using namespace b200dsa;
@@ -566,11 +563,9 @@ extern "C" int b200dsa_fp8_quantise_blocks(const void* w, int32_t in_f32, int64_
   return gemm_rc(e == cudaSuccess ? cudaGetLastError() : e);
 }
 
-extern "C" int b200dsa_fp8_block_matmul(const void* a_e4m3, int64_t a_stride, const float* a_scale, int64_t sa_m,
-                                        int64_t sa_g, const void* w_e4m3, int64_t w_stride, const float* w_scale,
-                                        int64_t sw_r, int64_t sw_g, int32_t m, int32_t n, int32_t k, void* out,
-                                        int32_t out_f32, int64_t out_stride, int32_t* status, void* stream) {
-  if (m == 0 || n == 0) return B200DSA_OK;
+static int check_matmul(const void* a_e4m3, int64_t a_stride, const float* a_scale, const void* w_e4m3, int64_t w_stride,
+                        const float* w_scale, int32_t m, int32_t n, int32_t k, const void* out, int32_t out_f32,
+                        int64_t out_stride, const int32_t* status) {
   if (!a_e4m3 || !a_scale || !w_e4m3 || !w_scale || !out || !status || m < 0 || n < 0 || k < 16 || (k & 15) ||
       a_stride < k || w_stride < k || out_stride < n) {
     set_last_error("b200dsa_fp8_block_matmul: bad argument (K a multiple of 16, strides at least the row lengths)");
@@ -581,12 +576,23 @@ extern "C" int b200dsa_fp8_block_matmul(const void* a_e4m3, int64_t a_stride, co
     set_last_error("b200dsa_fp8_block_matmul: operands and their row strides must be multiples of 16 bytes");
     return B200DSA_EALIGN;
   }
+  return B200DSA_OK;
+}
+
+// dependent: the launch may start while the previous kernel of the stream drains (its results are waited for inside)
+static int block_matmul(const void* a_e4m3, int64_t a_stride, const float* a_scale, int64_t sa_m, int64_t sa_g,
+                        const void* w_e4m3, int64_t w_stride, const float* w_scale, int64_t sw_r, int64_t sw_g, int32_t m,
+                        int32_t n, int32_t k, void* out, int32_t out_f32, int64_t out_stride, int32_t* status,
+                        bool dependent, void* stream) {
+  if (m == 0 || n == 0) return B200DSA_OK;
+  if (int rc = check_matmul(a_e4m3, a_stride, a_scale, w_e4m3, w_stride, w_scale, m, n, k, out, out_f32, out_stride, status)) return rc;
   PFN_encodeTiled enc = get_encode_tiled();
   if (!enc) return B200DSA_ECUDA;
-  int sms = 0, nt = 0, splits = 1;
-  if (int rc = sm_count(&sms)) return rc;
+  DeviceInfo dev;
+  if (cudaError_t e = current_device_info(&dev)) return gemm_rc(e);
+  int nt = 0, splits = 1;
   const int blocks = (k + 127) / 128;
-  gemm_plan(m, n, blocks, sms, &nt, &splits);
+  gemm_plan(m, n, blocks, dev.sms, &nt, &splits);
   CUtensorMap mw, ma;
   cuuint32_t es[2] = {1, 1};
   cuuint64_t dw[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(n)}, sw[1] = {static_cast<cuuint64_t>(w_stride)};
@@ -620,10 +626,41 @@ extern "C" int b200dsa_fp8_block_matmul(const void* a_e4m3, int64_t a_stride, co
   p.status = status;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (nt) {
-    case 16: return gemm_rc(gemm_launch<16>(mw, ma, p, sms, st));
-    case 32: return gemm_rc(gemm_launch<32>(mw, ma, p, sms, st));
-    case 64: return gemm_rc(gemm_launch<64>(mw, ma, p, sms, st));
-    case 128: return gemm_rc(gemm_launch<128>(mw, ma, p, sms, st));
-    default: return gemm_rc(gemm_launch<256>(mw, ma, p, sms, st));
+    case 16: return gemm_rc(gemm_launch<16>(mw, ma, p, dev, dependent, st));
+    case 32: return gemm_rc(gemm_launch<32>(mw, ma, p, dev, dependent, st));
+    case 64: return gemm_rc(gemm_launch<64>(mw, ma, p, dev, dependent, st));
+    case 128: return gemm_rc(gemm_launch<128>(mw, ma, p, dev, dependent, st));
+    default: return gemm_rc(gemm_launch<256>(mw, ma, p, dev, dependent, st));
   }
+}
+
+extern "C" int b200dsa_fp8_block_matmul(const void* a_e4m3, int64_t a_stride, const float* a_scale, int64_t sa_m,
+                                        int64_t sa_g, const void* w_e4m3, int64_t w_stride, const float* w_scale,
+                                        int64_t sw_r, int64_t sw_g, int32_t m, int32_t n, int32_t k, void* out,
+                                        int32_t out_f32, int64_t out_stride, int32_t* status, void* stream) {
+  return block_matmul(a_e4m3, a_stride, a_scale, sa_m, sa_g, w_e4m3, w_stride, w_scale, sw_r, sw_g, m, n, k, out, out_f32,
+                      out_stride, status, false, stream);
+}
+
+extern "C" int b200dsa_fp8_block_linear(const void* x, int32_t in_f32, int64_t in_stride, int32_t use_ue8m0,
+                                        const void* w_e4m3, int64_t w_stride, const float* w_scale, int64_t sw_r,
+                                        int64_t sw_g, int32_t m, int32_t n, int32_t k, void* out, int32_t out_f32,
+                                        int64_t out_stride, void* workspace, int64_t workspace_bytes, int32_t* status,
+                                        void* stream) {
+  if (m == 0 || n == 0) return B200DSA_OK;
+  const int64_t codes = static_cast<int64_t>(m) * k, groups = (static_cast<int64_t>(k) + 127) / 128;
+  if (m < 0 || k < 16 || (k & 15) || !workspace || workspace_bytes < codes + 4 * groups * m) {
+    set_last_error("b200dsa_fp8_block_linear: bad argument (K a multiple of 16, workspace of m * (k + 4 * ceil(k / 128)) bytes)");
+    return B200DSA_EINVAL;
+  }
+  if (reinterpret_cast<uintptr_t>(workspace) & 15) {
+    set_last_error("b200dsa_fp8_block_linear: the workspace must be 16-byte aligned");
+    return B200DSA_EALIGN;
+  }
+  float* scale = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + codes);
+  // the product's arguments are checked before anything is launched
+  if (int rc = check_matmul(workspace, k, scale, w_e4m3, w_stride, w_scale, m, n, k, out, out_f32, out_stride, status)) return rc;
+  if (int rc = b200dsa_fp8_quantise_rows(x, in_f32, in_stride, m, k, use_ue8m0, workspace, scale, m, stream)) return rc;
+  return block_matmul(workspace, k, scale, 1, m, w_e4m3, w_stride, w_scale, sw_r, sw_g, m, n, k, out, out_f32, out_stride,
+                      status, true, stream);
 }

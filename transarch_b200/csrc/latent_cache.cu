@@ -8,6 +8,7 @@
 //   r = rotation of the 64 position dims           (optional; half form or interleaved pairs)
 //   scale_g = max(amax_g |n|, 1e-4) / 448, rounded up to a power of two for the "ue8m0" format
 //   code = e4m3(n / scale_g), nearest even; r is rounded to bf16 once.  All arithmetic in fp32.
+//   A group with a NaN or an infinity gets scale NaN and reads as NaN throughout.
 // A power-of-two scale makes every later use exact: code * scale has four significant bits and fits bf16, so the
 // attention over the cache and the rows read back see the same numbers.
 //
@@ -113,10 +114,11 @@ __global__ void __launch_bounds__(32 * kRowWarps) latent_write_kernel(const Late
   for (int h = 0; h < 2; ++h) {
     float amax = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[h][j]));
-    for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    float scale = __fdiv_rn(fmaxf(amax, 1e-4f), 448.0f);
+    for (int j = 0; j < 8; ++j) amax = max_nan(amax, fabsf(x[h][j]));
+    for (int o = 8; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    float scale = __fdiv_rn(max_nan(amax, 1e-4f), 448.0f);
     if (p.use_ue8m0) scale = pow2_at_least(scale);
+    if (!(amax < INFINITY)) scale = __int_as_float(0x7fffffff);   // not finite: the whole group reads as NaN
     uint2 codes;
     codes.x = quant_e4m3x4(x[h][0], x[h][1], x[h][2], x[h][3], scale);
     codes.y = quant_e4m3x4(x[h][4], x[h][5], x[h][6], x[h][7], scale);

@@ -12,13 +12,21 @@ namespace b200dsa {
 
 constexpr int kLatentRowBytes = 656;   // 512 codes, 4 fp32 scales, 64 bf16 position dims
 
+// max that keeps a NaN (fmaxf drops it)
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // Smallest power of two that is >= x (x positive): exp2(ceil(log2(x))) on the bit pattern.
 __device__ __forceinline__ float pow2_at_least(float x) {
   const uint32_t u = __float_as_uint(x);
   uint32_t e = u >> 23;
   if (e == 0) return 1.17549435e-38f;   // subnormal: the smallest normal power of two
-  if (e != 255 && (u & 0x7fffffu)) ++e; // infinity and NaN stay what they are
-  return e == 255 && (u & 0x7fffffu) ? x : __uint_as_float(e << 23);
+  if (e == 255) return x;               // infinity and NaN stay what they are
+  if (u & 0x7fffffu) ++e;
+  return __uint_as_float(e << 23);
 }
 
 // Four values over one scale as e4m3 codes, nearest even, clamped to +-448 (NaN stays NaN).

@@ -59,6 +59,19 @@ bool make_link(const b200dsa_peer_link* in, PeerLinkDev* out, const char* who) {
   return true;
 }
 
+cudaError_t current_device_info(DeviceInfo* out) {
+  static std::atomic<int> sms[64];
+  cudaError_t e = cudaGetDevice(&out->index);
+  if (e != cudaSuccess) return e;
+  std::atomic<int>& s = sms[out->index & 63];
+  out->sms = s.load(std::memory_order_relaxed);
+  if (out->sms == 0) {
+    e = cudaDeviceGetAttribute(&out->sms, cudaDevAttrMultiProcessorCount, out->index);
+    if (e == cudaSuccess) s.store(out->sms, std::memory_order_relaxed);
+  }
+  return e;
+}
+
 bool pdl_enabled() {
   static int on = -1;
   if (on < 0) {

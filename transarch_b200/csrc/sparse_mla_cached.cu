@@ -9,10 +9,9 @@
 // score buffers and Q in TMEM, the row bytes read K-major by the scores and MN-major by the values).  What differs is
 // the way of a row into shared memory: 656 bytes come from HBM into registers, are widened to bf16 (exactly, when the
 // scales are powers of two) and stored in the 128-byte-swizzled layout of the MMA operands.  Eight warps do that, eight
-// rows of a tile each, lane l the codes 16l..16l+15 of a row; the loads of tile t+1 are issued row by row as the
-// registers of tile t are stored, so a tile's worth of tensor work covers their latency.  (Staging the codes in shared
-// memory by cp.async would add 2 x 42 KB of shared-memory traffic a tile to the 208 KB that the MMAs and the widened
-// rows take, and that port is already the second busiest unit.)
+// rows of a tile each; the loads of tile t+1 are issued row by row as the registers of tile t are stored.  (Staging the
+// codes in shared memory by cp.async would add 84 KB of shared-memory traffic a tile to the 220 KB that the MMAs and
+// the widened rows take, and that port is already the second busiest unit.)
 //
 // A tree is one more tile: its 64 keys are the drafted positions in order, its validity bits are the mask itself.
 //
@@ -64,6 +63,7 @@ sparse_mla_cached_kernel(const MlaCachedParams p) {
   __shared__ uint32_t s_tmem_base;
   __shared__ int s_abort;
   __shared__ uint32_t s_mask[kMlaStages][2];  // validity bit per key of the stage
+  __shared__ float s_inv[kMlaHeadsTile];      // 1 / sum of the probabilities of a head row, 0 without a key
 
   const int split = blockIdx.x % p.splits;
   const int hh = (blockIdx.x / p.splits) % p.halves;
@@ -81,7 +81,7 @@ sparse_mla_cached_kernel(const MlaCachedParams p) {
   uint64_t* pv_done = bars + 6;                  // [1] value MMA retired (P buffer free, O stable)
   uint64_t* kv_full = bars + 7;                  // [stages] eight row warps
   uint64_t* kv_empty = bars + 7 + kMlaStages;    // [stages] value MMA retired
-  uint64_t* q_land = bars + 7 + 2 * kMlaStages;  // [1] bytes of the Q rows
+  uint64_t* q_land = bars + 7 + 2 * kMlaStages;  // [1] 256 row-warp threads: their copies of Q have landed
 
   const int tid = threadIdx.x;
   const int warp = tid >> 5;
@@ -107,7 +107,7 @@ sparse_mla_cached_kernel(const MlaCachedParams p) {
     }
     mbar_init(p_full, 128);
     mbar_init(pv_done, 1);
-    mbar_init(q_land, 1);
+    mbar_init(q_land, 32 * kMlcRowWarps);
     mbar_fence_init();
   }
   if (warp == 12) {
@@ -121,6 +121,21 @@ sparse_mla_cached_kernel(const MlaCachedParams p) {
 
   if (warp < kMlcRowWarps) {
     // ------------------------------------------------------------------ rows
+    // Q first: 64 rows of 72 16-byte pieces into the tail of the key ring, which the rows do not reach before q_full
+    // (rows padded by 16 bytes against bank conflicts; the last one spills into the P tile, unused so far).  The softmax
+    // warps move it to TMEM.  One bulk copy a row instead took 8 k clocks to issue.
+    {
+      const int have = min(kMlaHeadsTile, p.n_heads - hh * kMlaHeadsTile);
+      const uint8_t* q0 = reinterpret_cast<const uint8_t*>(
+          p.q + (static_cast<int64_t>(item) * p.n_heads + hh * kMlaHeadsTile) * kMlaD);
+#pragma unroll
+      for (int u = 0; u < kMlaHeadsTile * 72 / (32 * kMlcRowWarps); ++u) {
+        const int c = tid + u * 32 * kMlcRowWarps, r = c / 72;
+        cp_async_16(smem_base + kMlaQStageOff + r * kMlaQRowBytes + (c - 72 * r) * 16, q0 + (r < have ? c * 16 : 0),
+                    r < have);
+      }
+      cp_async_mbar_arrive(q_land);
+    }
     const int32_t* idx_row = p.indices + static_cast<int64_t>(item) * p.idx_stride;
     int req = p.row_request ? __ldg(p.row_request + item) : item;
     bool known = req >= 0 && req < p.n_requests;
@@ -134,95 +149,129 @@ sparse_mla_cached_kernel(const MlaCachedParams p) {
     int64_t last = static_cast<int64_t>(base) - 1;    // the last position that may be attended by selection
     if (p.q_pos) last = min(last, static_cast<int64_t>(__ldg(p.q_pos + item)) + p.q_pos_bias);
     const int r0 = warp * 8;
-    // position of this lane's row of tile t (lanes 0..7), -1 = none
-    auto position = [&](int t) -> int {
+    // The way of a row, one step a tile: position (five tiles ahead), page (four), slot and row to L2 (three), row to
+    // registers (one), so that no step waits for the load of the one before it.
+    auto position = [&](int t) -> int {               // of this lane's row of tile t (lanes 0..7), -1 = none
       if (lane >= 8 || t >= n_tiles || !known) return -1;
       const int tt = tile0 + t;
       if (tt < sel_tiles) {
         const int j = tt * kMlaTile + r0 + lane;
-        const int v = j < n_idx ? __ldg(idx_row + j) : -1;
-        return v >= 0 && v <= last ? v : -1;
+        return j < n_idx ? __ldg(idx_row + j) : -1;
       }
       const int64_t v = static_cast<int64_t>(base) + r0 + lane;
       return ((mask >> (r0 + lane)) & 1) && base >= 0 && v <= 0x7fffffff ? static_cast<int>(v) : -1;
     };
-    // its slot in the cache, -1 = none (a page that does not exist is reported and left out)
-    auto slot_of = [&](int pos) -> int {
-      if (pos < 0) return -1;
+    struct Key {
+      int page, off;       // page -1: outside the table; off -1: no key
+    };
+    auto page_of = [&](int pos, int t) -> Key {
+      if (pos < 0 || (pos > last && tile0 + t < sel_tiles)) return Key{-1, -1};
       const int col = pos / p.page_size;
-      const int page = col < p.table_cols ? __ldg(table + col) : -1;
-      const int64_t slot = static_cast<int64_t>(page) * p.page_size + (pos - col * p.page_size);
-      if (page < 0 || slot >= p.n_slots) {
+      return Key{col < p.table_cols ? __ldg(table + col) : -1, pos - col * p.page_size};
+    };
+    auto slot_of = [&](Key k) -> int {                // -1 = none; a page that does not exist is reported
+      if (k.off < 0) return -1;
+      const int64_t slot = static_cast<int64_t>(k.page) * p.page_size + k.off;
+      if (k.page < 0 || slot >= p.n_slots) {
         atomicMax(p.status, kDevBadIndex);
         return -1;
       }
       return static_cast<int>(slot);
     };
+    // A row's registers: lane l holds codes 16l..16l+15 and their scale, and of two rows (lane / 8 + 4 j) the 16-byte
+    // chunk lane % 8 of the position dims.  A missing key reads row 0 and is made zero when it is stored.
     uint4 code[8];
     float scale[8];
     uint4 pe[2];
-    const uint4 zero4 = make_uint4(0, 0, 0, 0);
-    auto load_row = [&](int slot, int i) {          // codes and scale of row i of the warp
-      const int s = __shfl_sync(0xffffffffu, slot, i);
-      const uint8_t* src = p.cache + static_cast<int64_t>(s < 0 ? 0 : s) * kLatentRowBytes;
-      code[i] = s < 0 ? zero4 : __ldg(reinterpret_cast<const uint4*>(src) + lane);
-      scale[i] = s < 0 ? 0.f : __ldg(reinterpret_cast<const float*>(src + 512) + (lane >> 3));
+    auto row_ptr = [&](int s) { return p.cache + static_cast<int64_t>(max(s, 0)) * kLatentRowBytes; };
+    auto load_row = [&](int slot, int i) {
+      const uint8_t* src = row_ptr(__shfl_sync(0xffffffffu, slot, i));
+      code[i] = __ldg(reinterpret_cast<const uint4*>(src) + lane);
+      scale[i] = __ldg(reinterpret_cast<const float*>(src + 512) + (lane >> 3));
     };
-    auto load_pe = [&](int slot, int j) {           // position dims: lane = chunk lane % 8 of row lane / 8 + 4 j
-      const int s = __shfl_sync(0xffffffffu, slot, (lane >> 3) + 4 * j);
-      const uint8_t* src = p.cache + static_cast<int64_t>(s < 0 ? 0 : s) * kLatentRowBytes + 528;
-      pe[j] = s < 0 ? zero4 : __ldg(reinterpret_cast<const uint4*>(src) + (lane & 7));
+    auto load_pe = [&](int slot, int j) {
+      const uint8_t* src = row_ptr(__shfl_sync(0xffffffffu, slot, (lane >> 3) + 4 * j));
+      pe[j] = __ldg(reinterpret_cast<const uint4*>(src + 528) + (lane & 7));
     };
-    int slot = slot_of(position(0));
-    int pos_next = position(1);
+    auto prefetch = [&](int slot) {                   // 656 bytes touch at most seven lines of 128
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int s = __shfl_sync(0xffffffffu, slot, (lane >> 3) + 4 * j);
+        if (s >= 0 && (lane & 7) < 7)
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(row_ptr(s) + min((lane & 7) * 128, kLatentRowBytes - 1)));
+      }
+    };
+    int pos5 = position(4);
+    Key key4 = page_of(position(3), 3);
+    int slot, s1, s2, s3;
+    {
+      const Key k0 = page_of(position(0), 0), k1 = page_of(position(1), 1), k2 = page_of(position(2), 2);
+      slot = slot_of(k0);
+      s1 = slot_of(k1);
+      s2 = slot_of(k2);
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) load_row(slot, i);
     load_pe(slot, 0);
     load_pe(slot, 1);
-    // Lane l stores 16-byte chunks 2 (l % 4) and 2 (l % 4) + 1 of the 128-byte chunk l / 4 of a row.  Lanes 4..7 of
-    // every eight store them in the other order, so that the eight lanes of a store phase hit eight different banks
-    // groups.
-    const int flip = (lane >> 2) & 1;
+    prefetch(s1);
+    prefetch(s2);
+    // Lane l stores 16-byte chunks 2 (l % 4) and 2 (l % 4) + 1 of the 128-byte chunk l / 4 of a row; lanes 4..7 of every
+    // eight take them in the other order, so that eight neighbouring lanes write eight different bank groups.
+    const bool flip = (lane >> 2) & 1;
+    auto store_rows = [&](uint32_t stage_addr, unsigned vmask, int next) {
+      const uint32_t dst0 = stage_addr + (lane >> 2) * kMlaChunkBytesK + r0 * 128;
+      const int c0 = (lane & 3) * 2 + flip;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint4 c = (vmask >> i) & 1 ? code[i] : make_uint4(0, 0, 0, 0);
+        const float sc = (vmask >> i) & 1 ? scale[i] : 0.f;
+        uint4 w0, w1;
+        dequant_e4m3x4(flip ? c.z : c.x, sc, w0.x, w0.y);
+        dequant_e4m3x4(flip ? c.w : c.y, sc, w0.z, w0.w);
+        dequant_e4m3x4(flip ? c.x : c.z, sc, w1.x, w1.y);
+        dequant_e4m3x4(flip ? c.y : c.w, sc, w1.z, w1.w);
+        load_row(next, i);
+        const uint32_t dst = dst0 + i * 128;
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + ((c0 ^ i) << 4)), "r"(w0.x), "r"(w0.y),
+                     "r"(w0.z), "r"(w0.w) : "memory");
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + ((c0 ^ 1 ^ i) << 4)), "r"(w1.x), "r"(w1.y),
+                     "r"(w1.z), "r"(w1.w) : "memory");
+      }
+    };
     for (int t = 0; t < n_tiles; ++t) {
       const int s = t % kMlaStages;
       const unsigned vmask = __ballot_sync(0xffffffffu, lane < 8 && slot >= 0);
-      const int slot_next = slot_of(pos_next);
-      pos_next = position(t + 2);
+      s3 = slot_of(key4);
+      key4 = page_of(pos5, t + 4);
+      pos5 = position(t + 5);
+      prefetch(s3);
       bool ok = mbar_wait(&kv_empty[s], ((t / kMlaStages) & 1) ^ 1, abort_flag);
       // the tail of the ring holds the Q rows until the softmax threads have moved them to TMEM
       if (t < kMlaStages && (t + 1) * kMlaStageBytes > kMlaQStageOff) ok = ok && mbar_wait(q_full, 0, abort_flag);
       if (!__all_sync(0xffffffffu, ok)) break;
       const uint32_t stage_addr = kv_addr + s * kMlaStageBytes;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        uint32_t w[8];
-        dequant_e4m3x4(code[i].x, scale[i], w[0], w[1]);
-        dequant_e4m3x4(code[i].y, scale[i], w[2], w[3]);
-        dequant_e4m3x4(code[i].z, scale[i], w[4], w[5]);
-        dequant_e4m3x4(code[i].w, scale[i], w[6], w[7]);
-        load_row(slot_next, i);
-        const uint32_t dst = stage_addr + (lane >> 2) * kMlaChunkBytesK + (r0 + i) * 128;
-        const uint32_t c0 = (((lane & 3) * 2 + flip) ^ i) << 4, c1 = (((lane & 3) * 2 + (flip ^ 1)) ^ i) << 4;
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + c0), "r"(flip ? w[4] : w[0]),
-                     "r"(flip ? w[5] : w[1]), "r"(flip ? w[6] : w[2]), "r"(flip ? w[7] : w[3]) : "memory");
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + c1), "r"(flip ? w[0] : w[4]),
-                     "r"(flip ? w[1] : w[5]), "r"(flip ? w[2] : w[6]), "r"(flip ? w[3] : w[7]) : "memory");
-      }
+      store_rows(stage_addr, vmask, s1);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int i = (lane >> 3) + 4 * j;
         const uint32_t dst = stage_addr + 8 * kMlaChunkBytesK + (r0 + i) * 128 + (((lane & 7) ^ i) << 4);
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(pe[j].x), "r"(pe[j].y), "r"(pe[j].z),
-                     "r"(pe[j].w) : "memory");
-        load_pe(slot_next, j);
+        const uint32_t keep = (vmask >> i) & 1 ? 0xffffffffu : 0u;
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(pe[j].x & keep), "r"(pe[j].y & keep),
+                     "r"(pe[j].z & keep), "r"(pe[j].w & keep) : "memory");
+        load_pe(s1, j);
       }
       if (lane == 0) reinterpret_cast<volatile uint8_t*>(&s_mask[s][0])[warp] = static_cast<uint8_t>(vmask);
-      __threadfence_block();
-      fence_proxy_async();               // the rows were written through the generic proxy; the MMAs read them
+      // The rows were written through the generic proxy; the MMAs read them.  (No thread fence here: it would wait for
+      // the loads of the next tile, 1200 clocks a tile; the arrival releases the mask.)
+      fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&kv_full[s]);
-      slot = slot_next;
+      slot = s1;
+      s1 = s2;
+      s2 = s3;
     }
+    cp_async_wait_all();     // Q, should everything have been given up early
   } else if (warp < 12) {
     // ------------------------------------------------------------------ softmax
     // lanes 16..31: score row `row`; lanes 0..15: the same row of O (partner lane = lane ^ 16)
@@ -233,41 +282,19 @@ sparse_mla_cached_kernel(const MlaCachedParams p) {
     float m_ref = -INFINITY, l = 0.f;
     bool aborted = false;
     {
-      // Q -> TMEM once: one bulk copy per head row into the tail of the key ring, which the row warps do not
-      // touch before q_full (rows padded by 16 bytes against bank conflicts; the last one spills into the P
-      // tile, unused so far), then lane 16+i stores head row 16*wq+i into the upper half-lanes (two bf16 per
-      // cell, 288 cells per row).  The lower half-lanes of these columns belong to O, not written yet.
-      const int qhead = hh * kMlaHeadsTile + row;
-      const bool have = is_s && qhead < p.n_heads;
-      const int rows_have = min(kMlaHeadsTile, p.n_heads - hh * kMlaHeadsTile);
-      if (warp == 8) {
-        if (lane == 0) mbar_arrive_expect_tx(q_land, static_cast<uint32_t>(rows_have) * (kMlaD * 2));
-        __syncwarp();
-        const __nv_bfloat16* q0 = p.q + (static_cast<int64_t>(item) * p.n_heads + hh * kMlaHeadsTile) * kMlaD;
-        for (int r = lane; r < rows_have; r += 32)
-          bulk_load_1d(smem_al + kMlaQStageOff + r * kMlaQRowBytes, q0 + static_cast<int64_t>(r) * kMlaD, kMlaD * 2, q_land);
-      }
+      // Q -> TMEM once: lane 16+i stores head row 16*wq+i into the upper half-lanes (two bf16 per cell, 288 cells per
+      // row).  The lower half-lanes of these columns belong to O, not written yet.
       const bool okq = mbar_wait(q_land, 0, abort_flag);
       aborted = !__all_sync(0xffffffffu, okq);
-      if (aborted) {                    // the copies in flight land before the shared memory is given up
-        const long long t0 = clock64();
-        while (!mbar_test(q_land, 0) && clock64() - t0 < kWaitLimitCycles) {
-        }
-      }
       const uint32_t qrow = smem_base + kMlaQStageOff + row * kMlaQRowBytes;
 #pragma unroll 1
       for (int c = 0; c < kMlaD / 64 && !aborted; ++c) {
         uint32_t qv[32];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (have) {
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(qv[4 * j]), "=r"(qv[4 * j + 1]), "=r"(qv[4 * j + 2]), "=r"(qv[4 * j + 3])
-                         : "r"(qrow + c * 128 + j * 16));
-          } else {
-            qv[4 * j] = qv[4 * j + 1] = qv[4 * j + 2] = qv[4 * j + 3] = 0u;
-          }
-        }
+        for (int j = 0; j < 8; ++j)
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(qv[4 * j]), "=r"(qv[4 * j + 1]), "=r"(qv[4 * j + 2]), "=r"(qv[4 * j + 3])
+                       : "r"(qrow + c * 128 + j * 16));
         tmem_st_32x32(tmem_base + lane_addr + 128 + c * 32, qv);
       }
       tc_wait_st();
@@ -374,53 +401,18 @@ sparse_mla_cached_kernel(const MlaCachedParams p) {
       fence_proxy_async();
       mbar_arrive(p_full);
     }
-    // ---- output: lanes 0..15 own the O rows; l and m_ref come from the partner lane
-    const float l_o = __shfl_xor_sync(0xffffffffu, l, 16);
-    const float m_o = __shfl_xor_sync(0xffffffffu, m_ref, 16);
-    const int head = hh * kMlaHeadsTile + row;
-    const int64_t out_row = static_cast<int64_t>(item) * p.n_heads + head;
-    const int64_t part_row = static_cast<int64_t>(split) * p.n_items * p.n_heads + out_row;
-    const bool write = !is_s && head < p.n_heads && !aborted;
-    // a split writes its normalised fp32 part and its log-sum-exp
-    const bool to_bf16 = p.splits == 1 && p.ctx_bf16;
-    float* ctx_row = p.splits == 1 ? static_cast<float*>(p.ctx) + out_row * kMlaDv : p.part + part_row * kMlaDv;
-    __nv_bfloat16* ctx_row_h = static_cast<__nv_bfloat16*>(p.ctx) + out_row * kMlaDv;
-    float* lse_out = p.splits == 1 ? p.lse + out_row
-                                   : p.part + static_cast<int64_t>(p.splits) * p.n_items * p.n_heads * kMlaDv + part_row;
+    // 1 / sum and the log-sum-exp of every row; the rows leave below, by all warps
     bool ok = !aborted;
     if (ok && n_tiles > 0) ok = __all_sync(0xffffffffu, mbar_wait(pv_done, (n_tiles - 1) & 1, abort_flag));
-    if (ok) {
-      tc_fence_after();
-      const bool any = n_tiles > 0 && l_o != 0.f;       // a NaN sum stays NaN in the result
-      const float inv = any ? 1.0f / l_o : 0.f;
-#pragma unroll 1
-      for (int c = 0; c < kMlaDv / 32; ++c) {
-        uint32_t o[32];
-        if (n_tiles > 0) {
-          tmem_ld_32x32(tmem_base + lane_addr + kMlaTmemO + c * 32, o);
-          tc_wait_ld();
-        }
-#pragma unroll
-        for (int j = 0; j < 32; ++j) o[j] = any ? __float_as_uint(__uint_as_float(o[j]) * inv) : 0u;
-        if (write && to_bf16) {
-#pragma unroll
-          for (int j = 0; j < 32; j += 8) {
-            uint4 v;
-            v.x = pack_bf16x2(__uint_as_float(o[j]), __uint_as_float(o[j + 1]));
-            v.y = pack_bf16x2(__uint_as_float(o[j + 2]), __uint_as_float(o[j + 3]));
-            v.z = pack_bf16x2(__uint_as_float(o[j + 4]), __uint_as_float(o[j + 5]));
-            v.w = pack_bf16x2(__uint_as_float(o[j + 6]), __uint_as_float(o[j + 7]));
-            *reinterpret_cast<uint4*>(ctx_row_h + c * 32 + j) = v;
-          }
-        } else if (write) {
-#pragma unroll
-          for (int j = 0; j < 32; j += 4)
-            *reinterpret_cast<uint4*>(ctx_row + c * 32 + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-        }
-      }
-      tc_fence_before();
-      if (write) *lse_out = any ? (m_o + log2f(l_o)) * 0.6931471805599453f : -INFINITY;
+    if (ok && is_s) {
+      const bool any = n_tiles > 0 && l != 0.f;          // a NaN sum stays NaN in the result
+      s_inv[row] = any ? 1.0f / l : 0.f;
+      const int head = hh * kMlaHeadsTile + row;
+      const int64_t out_row = static_cast<int64_t>(item) * p.n_heads + head, parts = static_cast<int64_t>(p.n_items) * p.n_heads;
+      float* lse_out = p.splits == 1 ? p.lse + out_row : p.part + p.splits * parts * kMlaDv + split * parts + out_row;
+      if (head < p.n_heads) *lse_out = any ? (m_ref + log2f(l)) * 0.6931471805599453f : -INFINITY;
     }
+    tc_fence_before();
   } else {
     // ------------------------------------------------------------------ MMA issuer (warp 12)
     // One warp issues everything, in the order S(0), S(1), PV(0), S(2), PV(1), ...: the tensor pipe runs
@@ -482,9 +474,63 @@ sparse_mla_cached_kernel(const MlaCachedParams p) {
     }
   }
 
-  // ---------------------------------------------------------------------- common tail
+  // ------------------------------------------------------------------------ output
+  // Three warps a TMEM lane quadrant bring O (lanes 0..15 of the quadrant) into the ring, which is free now, 32 columns at
+  // a time, and whole rows leave from there with every store instruction one run of 512 bytes.  (Stores straight from
+  // the softmax threads, 16 bytes at a row's pitch, took 11 k clocks a CTA; a bulk store a row 8 k.)
   tc_fence_before();
   __syncthreads();
+  tc_fence_after();
+  const bool write = *abort_flag == 0;
+  const bool to_bf16 = p.splits == 1 && p.ctx_bf16;        // a split writes its normalised fp32 part
+  const uint32_t pitch = to_bf16 ? kMlaDv * 2 + 16 : kMlaDv * 4 + 16;
+  if (write && warp < 12 && n_tiles > 0) {
+    const int wq = warp & 3, row = wq * 16 + (lane & 15);
+    const float inv = s_inv[row];
+    const uint32_t stage = smem_base + row * pitch;
+#pragma unroll 2
+    for (int c = warp >> 2; c < kMlaDv / 32; c += 3) {
+      uint32_t o[32];
+      tmem_ld_32x32(tmem_base + (static_cast<uint32_t>(wq * 32) << 16) + kMlaTmemO + c * 32, o);
+      tc_wait_ld();
+      // a row without a single key holds zeros, or nothing yet: zero times its stale cells would keep a NaN
+#pragma unroll
+      for (int j = 0; j < 32; ++j) o[j] = inv != 0.f ? __float_as_uint(__uint_as_float(o[j]) * inv) : 0u;
+      if (lane < 16 && to_bf16) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 8)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + c * 64 + j * 2),
+                       "r"(pack_bf16x2(__uint_as_float(o[j]), __uint_as_float(o[j + 1]))),
+                       "r"(pack_bf16x2(__uint_as_float(o[j + 2]), __uint_as_float(o[j + 3]))),
+                       "r"(pack_bf16x2(__uint_as_float(o[j + 4]), __uint_as_float(o[j + 5]))),
+                       "r"(pack_bf16x2(__uint_as_float(o[j + 6]), __uint_as_float(o[j + 7])))
+                       : "memory");
+      } else if (lane < 16) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 4)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + c * 128 + j * 4), "r"(o[j]),
+                       "r"(o[j + 1]), "r"(o[j + 2]), "r"(o[j + 3])
+                       : "memory");
+      }
+      __syncwarp();
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (write) {
+    const int heads = min(kMlaHeadsTile, p.n_heads - hh * kMlaHeadsTile), pieces = to_bf16 ? 2 : 4;
+    const int64_t first = (static_cast<int64_t>(p.splits > 1 ? split : 0) * p.n_items + item) * p.n_heads + hh * kMlaHeadsTile;
+    uint8_t* out = static_cast<uint8_t*>(p.splits > 1 ? static_cast<void*>(p.part) : p.ctx) + first * (pitch - 16);
+    for (int i = warp; i < heads * pieces; i += kMlcThreads / 32) {
+      const int r = i / pieces, at = (i - r * pieces) * 512 + lane * 16;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (n_tiles > 0)
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                     : "r"(smem_base + r * pitch + at));
+      *reinterpret_cast<uint4*>(out + static_cast<int64_t>(r) * (pitch - 16) + at) = v;
+    }
+  }
   tc_fence_after();
   if (warp == 12) tmem_dealloc(tmem_base, kMlaTmemCols);
   if (tid == 0 && s_abort) atomicMax(p.status, kDevWaitTimeout);
@@ -539,11 +585,11 @@ using namespace b200dsa;
 
 extern "C" int b200dsa_sparse_mla_decode_cached_splits(int32_t n_items, int32_t n_heads, int32_t n_idx, int32_t tree) {
   if (n_items < 1 || n_heads < 1 || n_idx < 0) return 1;
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  DeviceInfo dev;
+  if (current_device_info(&dev) != cudaSuccess) return 1;
   const int64_t ctas = static_cast<int64_t>(n_items) * (n_heads > kMlaHeadsTile ? 2 : 1);
   const int tiles = (n_idx + kMlaTile - 1) / kMlaTile + (tree ? 1 : 0);
-  int64_t splits = sms / ctas;
+  int64_t splits = dev.sms / ctas;
   if (splits > tiles / 2) splits = tiles / 2;          // a run of one tile costs as much in prologue and merge as it saves
   if (splits > kMlcMaxSplits) splits = kMlcMaxSplits;
   return splits < 1 ? 1 : static_cast<int>(splits);
@@ -578,7 +624,13 @@ extern "C" int b200dsa_sparse_mla_decode_cached(const void* q_bf16, const void* 
     set_last_error("b200dsa_sparse_mla_decode_cached: q, cache, ctx and workspace must be 16-byte aligned");
     return B200DSA_EALIGN;
   }
-  cudaError_t e = cudaFuncSetAttribute(sparse_mla_cached_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMlaSmemBytes);
+  DeviceInfo dev;
+  static OncePerDevice once;
+  cudaError_t e = current_device_info(&dev);
+  if (e == cudaSuccess)
+    e = once.run(dev.index, [] {
+      return cudaFuncSetAttribute(sparse_mla_cached_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMlaSmemBytes);
+    });
   if (e != cudaSuccess) return mlc_rc(e);
   MlaCachedParams p{};
   p.q = static_cast<const __nv_bfloat16*>(q_bf16);
@@ -612,9 +664,18 @@ extern "C" int b200dsa_sparse_mla_decode_cached(const void* q_bf16, const void* 
                      static_cast<cudaStream_t>(stream), p);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e == cudaSuccess && splits > 1) {
-    e = launch_chained(mla_merge_kernel, dim3(static_cast<unsigned>(rows)), dim3(128), 0,
-                       static_cast<cudaStream_t>(stream), static_cast<const float*>(p.part), static_cast<int>(rows),
-                       static_cast<int>(splits), ctx, static_cast<int>(ctx_bf16 != 0), lse);
+    // the merge becomes resident while the attention drains (it waits for it inside)
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(rows));
+    cfg.blockDim = dim3(128);
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, mla_merge_kernel, static_cast<const float*>(p.part), static_cast<int>(rows),
+                           static_cast<int>(splits), ctx, static_cast<int>(ctx_bf16 != 0), lse);
     if (e == cudaSuccess) e = cudaGetLastError();
   }
   return mlc_rc(e);

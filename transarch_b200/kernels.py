@@ -5,7 +5,6 @@ current stream.  Nothing here computes on the CPU.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from typing import Optional, Sequence, Tuple
 
@@ -978,36 +977,45 @@ def wuv_up_project(ctx: torch.Tensor, w_uv: torch.Tensor, *, out_dtype: torch.dt
 # their tensors (on its current stream) whatever device is current, and refuse tensors of different devices.
 # ------------------------------------------------------------------------------------------------------------------
 LATENT_ROW = 656                     # bytes of a cached token: 512 codes, 4 fp32 scales, 64 bf16 position dims
-_CURRENT = contextlib.nullcontext()
 
 
-def _on_device(first: torch.Tensor, *others: Optional[torch.Tensor]):
-    """Context in which `first`'s device is current; raises unless every given tensor lives there."""
+def _device_index(first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
+    """CUDA device index of a call's tensors; raises unless all of them live there."""
     dev = first.device
     if dev.type != "cuda":
         raise _lib.B200DSAError("b200dsa kernels need CUDA tensors; there is no CPU path")
     for t in others:
         if t is not None and t.device != dev:
             raise _lib.B200DSAError(f"all tensors of a call must be on one device ({dev} and {t.device} given)")
-    return _CURRENT if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+    return dev.index
 
 
 def _rows_stride(x: torch.Tensor, width: int) -> int:
     """Row stride of a 2-D tensor with unit column stride (a single row may carry any stride)."""
-    return x.stride(0) if x.shape[0] > 1 else max(width, x.stride(0))
+    return x.stride(0) if x.shape[0] > 1 else width
 
 
 def _latent_slots(cache: torch.Tensor, page_size: int) -> int:
-    if cache.dtype != torch.uint8 or not cache.is_contiguous() or page_size < 1 or cache.numel() == 0 or \
-            cache.numel() % (page_size * LATENT_ROW):
+    n = cache.numel()
+    if cache.dtype != torch.uint8 or not cache.is_contiguous() or page_size < 1 or n == 0 or \
+            n % (page_size * LATENT_ROW):
         raise _lib.B200DSAError("cache must be contiguous uint8 with page_size*656 bytes per page")
-    return cache.numel() // LATENT_ROW
+    return n // LATENT_ROW
 
 
 def _scale_fmt(scale_fmt: Optional[str]) -> int:
     if scale_fmt not in (None, "ue8m0"):
         raise _lib.B200DSAError(f"unknown scale_fmt {scale_fmt!r} (None or 'ue8m0')")
     return int(scale_fmt is not None)
+
+
+def _pages(block_table: torch.Tensor) -> Tuple[int, int, int]:
+    """(requests, pages of a request, row stride) of a block table."""
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[1] < 1 or \
+            (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise _lib.B200DSAError("block_table must be int32 [n_requests, pages] with unit column stride")
+    R, cols = block_table.shape
+    return R, cols, block_table.stride(0) if R > 1 else cols
 
 
 def latent_quant_and_cache(kv: torch.Tensor, cache: torch.Tensor, slot_mapping: torch.Tensor, page_size: int, *,
@@ -1018,7 +1026,8 @@ def latent_quant_and_cache(kv: torch.Tensor, cache: torch.Tensor, slot_mapping: 
     projection) into their cache slots in one kernel; see b200dsa_latent_quant_and_cache.  norm_weight [512] (None: no
     RMSNorm), cos / sin [n, 64] (None: no rotation).  A negative slot is a padding token; slots must be distinct."""
     fmt = _scale_fmt(scale_fmt)
-    if kv.dtype not in (torch.bfloat16, torch.float32) or kv.dim() != 2 or kv.shape[1] != 576 or kv.stride(1) != 1:
+    f32 = kv.dtype == torch.float32
+    if not (f32 or kv.dtype == torch.bfloat16) or kv.dim() != 2 or kv.shape[1] != 576 or kv.stride(1) != 1:
         raise _lib.B200DSAError("kv must be bf16 or fp32 [n, 576] with unit column stride")
     n = kv.shape[0]
     stride = _rows_stride(kv, 576)
@@ -1027,36 +1036,24 @@ def latent_quant_and_cache(kv: torch.Tensor, cache: torch.Tensor, slot_mapping: 
     if slot_mapping.dtype != torch.int64 or not slot_mapping.is_contiguous() or slot_mapping.numel() != n:
         raise _lib.B200DSAError("slot_mapping must be contiguous int64 with one entry per row of kv")
     n_slots = _latent_slots(cache, page_size)
-    if norm_weight is not None and (norm_weight.dtype not in (torch.bfloat16, torch.float32) or
-                                    not norm_weight.is_contiguous() or norm_weight.numel() != 512 or
-                                    norm_weight.data_ptr() % 16):
-        raise _lib.B200DSAError("norm_weight must be contiguous, 16-byte aligned bf16 or fp32 [512]")
-    if (cos is None) != (sin is None):
-        raise _lib.B200DSAError("cos and sin go together")
-    with _on_device(kv, cache, slot_mapping, norm_weight, cos, sin):
-        c, s_ = _f32c(cos), _f32c(sin)
-        if c is not None and (c.numel() != n * 64 or s_.numel() != n * 64):
-            raise _lib.B200DSAError("cos / sin must hold 64 values per token")
-        check(_lib.load().b200dsa_latent_quant_and_cache(
-            kv.data_ptr(), int(kv.dtype == torch.float32), stride, n, ptr(norm_weight),
-            int(norm_weight is not None and norm_weight.dtype == torch.float32), eps, ptr(c), ptr(s_), int(interleaved),
-            slot_mapping.data_ptr(), cache.data_ptr(), n_slots, fmt, status_word(kv.device).data_ptr(), stream_ptr()),
-            "b200dsa_latent_quant_and_cache")
-
-
-def latent_cache_rows(cache: torch.Tensor, slots: torch.Tensor, page_size: int, *,
-                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """bf16 rows [n, 576] of the given cache slots (int64; negative: a row of zeros); see b200dsa_latent_cache_rows."""
-    n_slots = _latent_slots(cache, page_size)
-    if slots.dtype != torch.int64 or not slots.is_contiguous():
-        raise _lib.B200DSAError("slots must be contiguous int64")
-    n = slots.numel()
-    with _on_device(cache, slots, out):
-        out = _latent_out(out, n, cache.device)
-        check(_lib.load().b200dsa_latent_cache_rows(cache.data_ptr(), n_slots, slots.data_ptr(), n, out.data_ptr(),
-                                                    status_word(cache.device).data_ptr(), stream_ptr()),
-              "b200dsa_latent_cache_rows")
-    return out
+    gain = gain_f32 = 0
+    if norm_weight is not None:
+        gain, gain_f32 = norm_weight.data_ptr(), norm_weight.dtype == torch.float32
+        if not (gain_f32 or norm_weight.dtype == torch.bfloat16) or not norm_weight.is_contiguous() or \
+                norm_weight.numel() != 512 or gain % 16:
+            raise _lib.B200DSAError("norm_weight must be contiguous, 16-byte aligned bf16 or fp32 [512]")
+    if cos is not None or sin is not None:
+        if cos is None or sin is None or cos.numel() != n * 64 or sin.numel() != n * 64:
+            raise _lib.B200DSAError("cos and sin go together and hold 64 values per token")
+    index = _device_index(kv, cache, slot_mapping, norm_weight, cos, sin)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return latent_quant_and_cache(kv, cache, slot_mapping, page_size, norm_weight=norm_weight, eps=eps, cos=cos,
+                                          sin=sin, interleaved=interleaved, scale_fmt=scale_fmt)
+    c, s_ = _f32c(cos), _f32c(sin)
+    check(_lib.load().b200dsa_latent_quant_and_cache(
+        kv.data_ptr(), f32, stride, n, gain, gain_f32, eps, ptr(c), ptr(s_), interleaved, slot_mapping.data_ptr(),
+        cache.data_ptr(), n_slots, fmt, _lib.status_ptr(index), stream_ptr()), "b200dsa_latent_quant_and_cache")
 
 
 def _latent_out(out: Optional[torch.Tensor], n: int, device) -> torch.Tensor:
@@ -1067,25 +1064,49 @@ def _latent_out(out: Optional[torch.Tensor], n: int, device) -> torch.Tensor:
     return out
 
 
+def latent_cache_rows(cache: torch.Tensor, slots: torch.Tensor, page_size: int, *,
+                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """bf16 rows [n, 576] of the given cache slots (int64; negative: a row of zeros); see b200dsa_latent_cache_rows."""
+    n_slots = _latent_slots(cache, page_size)
+    if slots.dtype != torch.int64 or not slots.is_contiguous():
+        raise _lib.B200DSAError("slots must be contiguous int64")
+    n = slots.numel()
+    if out is not None:
+        _latent_out(out, n, None)
+    index = _device_index(cache, slots, out)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return latent_cache_rows(cache, slots, page_size, out=out)
+    if out is None:
+        out = _latent_out(None, n, cache.device)
+    check(_lib.load().b200dsa_latent_cache_rows(cache.data_ptr(), n_slots, slots.data_ptr(), n, out.data_ptr(),
+                                                _lib.status_ptr(index), stream_ptr()), "b200dsa_latent_cache_rows")
+    return out
+
+
 def latent_cache_gather(cache: torch.Tensor, page_size: int, block_table: torch.Tensor, cu_rows: torch.Tensor,
                         n_rows: int, *, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """bf16 rows [n_rows, 576] of the cached prefixes of several requests, one after another: request r fills rows
     [cu_rows[r], cu_rows[r+1]) with its positions 0, 1, ... (block_table int32 [R, pages], cu_rows int32 [R+1]); see
     b200dsa_latent_cache_gather.  Rows behind the last request are not written."""
     n_slots = _latent_slots(cache, page_size)
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[1] < 1 or \
-            block_table.stride(1) != 1:
-        raise _lib.B200DSAError("block_table must be int32 [n_requests, pages] with unit column stride")
-    R = block_table.shape[0]
+    R, cols, stride = _pages(block_table)
     _i32(cu_rows, "cu_rows")
     if cu_rows.numel() != R + 1:
         raise _lib.B200DSAError("cu_rows must hold n_requests + 1 entries")
-    with _on_device(cache, block_table, cu_rows, out):
-        out = _latent_out(out, n_rows, cache.device)
-        check(_lib.load().b200dsa_latent_cache_gather(
-            cache.data_ptr(), n_slots, page_size, block_table.data_ptr(), _rows_stride(block_table, block_table.shape[1]),
-            block_table.shape[1], cu_rows.data_ptr(), R, n_rows, out.data_ptr(), status_word(cache.device).data_ptr(),
-            stream_ptr()), "b200dsa_latent_cache_gather")
+    if n_rows < 0:
+        raise _lib.B200DSAError("n_rows must not be negative")
+    if out is not None:
+        _latent_out(out, n_rows, None)
+    index = _device_index(cache, block_table, cu_rows, out)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return latent_cache_gather(cache, page_size, block_table, cu_rows, n_rows, out=out)
+    if out is None:
+        out = _latent_out(None, n_rows, cache.device)
+    check(_lib.load().b200dsa_latent_cache_gather(
+        cache.data_ptr(), n_slots, page_size, block_table.data_ptr(), stride, cols, cu_rows.data_ptr(), R, n_rows,
+        out.data_ptr(), _lib.status_ptr(index), stream_ptr()), "b200dsa_latent_cache_gather")
     return out
 
 
@@ -1095,11 +1116,13 @@ def draft_tree_masks(parents: torch.Tensor) -> torch.Tensor:
     _i32(parents, "parents")
     if parents.dim() != 2 or parents.shape[1] > 64:
         raise _lib.B200DSAError("parents must be int32 [n_trees, n_nodes <= 64]")
-    with _on_device(parents):
-        masks = torch.empty(parents.shape, dtype=torch.int64, device=parents.device)
-        check(_lib.load().b200dsa_draft_tree_masks(parents.data_ptr(), parents.shape[0], parents.shape[1],
-                                                   masks.data_ptr(), status_word(parents.device).data_ptr(),
-                                                   stream_ptr()), "b200dsa_draft_tree_masks")
+    index = _device_index(parents)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return draft_tree_masks(parents)
+    masks = torch.empty(parents.shape, dtype=torch.int64, device=parents.device)
+    check(_lib.load().b200dsa_draft_tree_masks(parents.data_ptr(), parents.shape[0], parents.shape[1], masks.data_ptr(),
+                                               _lib.status_ptr(index), stream_ptr()), "b200dsa_draft_tree_masks")
     return masks
 
 
@@ -1107,7 +1130,7 @@ def sparse_mla_cached_workspace(n_items: int, n_heads: int, n_idx: int, device, 
     """(splits, workspace or None) that sparse_mla_decode_cached takes for calls of at most this size on `device`; keep
     one for each call that may be in flight at a time."""
     with torch.cuda.device(device):
-        splits = _lib.load().b200dsa_sparse_mla_decode_cached_splits(n_items, n_heads, n_idx, int(tree))
+        splits = _lib.load().b200dsa_sparse_mla_decode_cached_splits(n_items, n_heads, n_idx, tree)
         ws = None if splits == 1 else torch.empty(splits * n_items * n_heads * 513, dtype=torch.float32, device=device)
     return splits, ws
 
@@ -1133,76 +1156,82 @@ def sparse_mla_decode_cached(q: torch.Tensor, cache: torch.Tensor, page_size: in
             (indices.shape[1] > 1 and indices.stride(1) != 1):
         raise _lib.B200DSAError("indices must be int32 [n_items, n_idx] with unit column stride")
     n_idx = indices.shape[1]
-    idx_stride = _rows_stride(indices, n_idx)
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[1] < 1 or \
-            block_table.stride(1) != 1:
-        raise _lib.B200DSAError("block_table must be int32 [n_requests, pages] with unit column stride")
-    R = block_table.shape[0]
+    R, cols, stride = _pages(block_table)
     for t_, nm in ((row_request, "row_request"), (q_pos, "q_pos"), (n_idx_item, "n_idx_item")):
-        if _i32(t_, nm) is not None and t_.numel() != n:
-            raise _lib.B200DSAError(f"{nm} must have one entry per item")
+        if t_ is not None and (t_.dtype != torch.int32 or not t_.is_contiguous() or t_.numel() != n):
+            raise _lib.B200DSAError(f"{nm} must be contiguous int32 with one entry per item")
     if row_request is None and R < n:
         raise _lib.B200DSAError("without row_request the block table needs one row per item")
-    if (tree_mask is None) != (tree_base is None):
-        raise _lib.B200DSAError("tree_mask and tree_base go together")
-    if tree_mask is not None:
-        if tree_mask.dtype != torch.int64 or not tree_mask.is_contiguous() or tree_mask.numel() != n:
+    if tree_mask is not None or tree_base is not None:
+        if tree_mask is None or tree_mask.dtype != torch.int64 or not tree_mask.is_contiguous() or tree_mask.numel() != n:
             raise _lib.B200DSAError("tree_mask must be contiguous int64 with one entry per item")
-        if _i32(tree_base, "tree_base").numel() != R:
-            raise _lib.B200DSAError("tree_base must have one entry per request")
-    with _on_device(q, cache, indices, block_table, row_request, q_pos, n_idx_item, tree_mask, tree_base, ctx, lse):
-        if ctx is None:
-            ctx = torch.empty(n, H, 512, dtype=torch.bfloat16, device=q.device)
-        elif ctx.dtype not in (torch.float32, torch.bfloat16) or not ctx.is_contiguous() or ctx.shape != (n, H, 512):
-            raise _lib.B200DSAError("ctx must be contiguous fp32 or bf16 [n_items, n_heads, 512]")
-        if lse is None:
-            lse = torch.empty(n, H, dtype=torch.float32, device=q.device)
-        elif lse.dtype != torch.float32 or not lse.is_contiguous() or lse.shape != (n, H):
-            raise _lib.B200DSAError("lse must be contiguous fp32 [n_items, n_heads]")
-        if n == 0:
-            return ctx, lse
-        lib = _lib.load()
-        if workspace is not None:
-            splits, ws = workspace
-            if splits > 1 and (ws is None or ws.device != q.device or ws.dtype != torch.float32 or
-                               not ws.is_contiguous() or ws.numel() < splits * n * H * 513):
-                raise _lib.B200DSAError("the workspace is smaller than splits * n_items * n_heads * 513 floats")
-        else:
-            splits = lib.b200dsa_sparse_mla_decode_cached_splits(n, H, n_idx, int(tree_mask is not None))
-            ws = torch.empty(splits * n * H * 513, dtype=torch.float32, device=q.device) if splits > 1 else None
-        check(lib.b200dsa_sparse_mla_decode_cached(
-            q.data_ptr(), cache.data_ptr(), n_slots, page_size, block_table.data_ptr(),
-            _rows_stride(block_table, block_table.shape[1]), block_table.shape[1], R, ptr(row_request),
-            indices.data_ptr() if n_idx else None, idx_stride, n_idx, ptr(n_idx_item), ptr(q_pos), q_pos_bias,
-            ptr(tree_mask), ptr(tree_base), n, H, sm_scale, ctx.data_ptr(), int(ctx.dtype == torch.bfloat16),
-            lse.data_ptr(), splits, ptr(ws), ws.numel() * 4 if ws is not None else 0,
-            status_word(q.device).data_ptr(), stream_ptr()), "b200dsa_sparse_mla_decode_cached")
+        if tree_base is None or tree_base.dtype != torch.int32 or not tree_base.is_contiguous() or tree_base.numel() != R:
+            raise _lib.B200DSAError("tree_base must be contiguous int32 with one entry per request")
+    if ctx is not None and (ctx.dtype not in (torch.float32, torch.bfloat16) or not ctx.is_contiguous() or
+                            ctx.shape != (n, H, 512)):
+        raise _lib.B200DSAError("ctx must be contiguous fp32 or bf16 [n_items, n_heads, 512]")
+    if lse is not None and (lse.dtype != torch.float32 or not lse.is_contiguous() or lse.shape != (n, H)):
+        raise _lib.B200DSAError("lse must be contiguous fp32 [n_items, n_heads]")
+    if not sm_scale > 0:
+        raise _lib.B200DSAError("sm_scale must be positive")
+    splits, ws = workspace if workspace is not None else (0, None)
+    index = _device_index(q, cache, indices, block_table, row_request, q_pos, n_idx_item, tree_mask, tree_base, ctx, lse, ws)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return sparse_mla_decode_cached(q, cache, page_size, indices, sm_scale, block_table=block_table,
+                                            row_request=row_request, q_pos=q_pos, q_pos_bias=q_pos_bias,
+                                            n_idx_item=n_idx_item, tree_mask=tree_mask, tree_base=tree_base, ctx=ctx,
+                                            lse=lse, workspace=workspace)
+    if ctx is None:
+        ctx = torch.empty(n, H, 512, dtype=torch.bfloat16, device=q.device)
+    if lse is None:
+        lse = torch.empty(n, H, dtype=torch.float32, device=q.device)
+    if n == 0:
+        return ctx, lse
+    lib = _lib.load()
+    if workspace is None:
+        splits = lib.b200dsa_sparse_mla_decode_cached_splits(n, H, n_idx, tree_mask is not None)
+        if splits > 1:
+            ws = torch.empty(splits * n * H * 513, dtype=torch.float32, device=q.device)
+    elif splits > 1 and (ws is None or ws.dtype != torch.float32 or not ws.is_contiguous() or
+                         ws.numel() < splits * n * H * 513):
+        raise _lib.B200DSAError("the workspace is smaller than splits * n_items * n_heads * 513 floats")
+    check(lib.b200dsa_sparse_mla_decode_cached(
+        q.data_ptr(), cache.data_ptr(), n_slots, page_size, block_table.data_ptr(), stride, cols, R, ptr(row_request),
+        indices.data_ptr(), indices.stride(0) if n > 1 else n_idx, n_idx, ptr(n_idx_item), ptr(q_pos), q_pos_bias,
+        ptr(tree_mask), ptr(tree_base), n, H, sm_scale, ctx.data_ptr(), ctx.dtype == torch.bfloat16, lse.data_ptr(),
+        splits, ptr(ws), ws.numel() * 4 if ws is not None else 0, _lib.status_ptr(index), stream_ptr()),
+        "b200dsa_sparse_mla_decode_cached")
     return ctx, lse
 
 
-def _matrix(x: torch.Tensor, name: str) -> int:
-    if x.dtype not in (torch.bfloat16, torch.float32) or x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
+def _matrix(x: torch.Tensor, name: str) -> Tuple[int, int, int, bool]:
+    """(rows, columns, row stride, is fp32) of a matrix to be quantised."""
+    f32 = x.dtype == torch.float32
+    if not (f32 or x.dtype == torch.bfloat16) or x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
         raise _lib.B200DSAError(f"{name} must be a 2-D bf16 or fp32 tensor with unit column stride")
-    if x.shape[1] < 16 or x.shape[1] % 16:
+    M, K = x.shape
+    if K < 16 or K % 16:
         raise _lib.B200DSAError(f"the columns of {name} must be a multiple of 16")
-    stride = _rows_stride(x, x.shape[1])
-    if stride < x.shape[1]:
+    stride = _rows_stride(x, K)
+    if stride < K:
         raise _lib.B200DSAError(f"the rows of {name} must not overlap")
-    return stride
+    return M, K, stride, f32
 
 
 def fp8_quantise_rows(x: torch.Tensor, *, scale_fmt: Optional[str] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """(codes float8_e4m3fn [M, K], scales fp32 [M, ceil(K/128)], stored column by column): one scale for 128 values of
     a row, max(amax, 1e-10)/448 or with "ue8m0" the power of two above it; see b200dsa_fp8_quantise_rows."""
     fmt = _scale_fmt(scale_fmt)
-    stride = _matrix(x, "x")
-    M, K = x.shape
-    with _on_device(x):
-        q = torch.empty(M, K, dtype=torch.float8_e4m3fn, device=x.device)
-        scale = torch.empty((K + 127) // 128, M, dtype=torch.float32, device=x.device)
-        check(_lib.load().b200dsa_fp8_quantise_rows(x.data_ptr(), int(x.dtype == torch.float32), stride, M, K, fmt,
-                                                    q.data_ptr(), scale.data_ptr(), M, stream_ptr()),
-              "b200dsa_fp8_quantise_rows")
+    M, K, stride, f32 = _matrix(x, "x")
+    index = _device_index(x)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return fp8_quantise_rows(x, scale_fmt=scale_fmt)
+    q = torch.empty(M, K, dtype=torch.float8_e4m3fn, device=x.device)
+    scale = torch.empty((K + 127) // 128, M, dtype=torch.float32, device=x.device)
+    check(_lib.load().b200dsa_fp8_quantise_rows(x.data_ptr(), f32, stride, M, K, fmt, q.data_ptr(), scale.data_ptr(), M,
+                                                stream_ptr()), "b200dsa_fp8_quantise_rows")
     return q, scale.t()
 
 
@@ -1210,50 +1239,85 @@ def fp8_quantise_blocks(w: torch.Tensor, *, scale_fmt: Optional[str] = None) -> 
     """(codes float8_e4m3fn [N, K], scales fp32 [ceil(N/128), ceil(K/128)]): weights with one scale for a block of
     128 x 128; see b200dsa_fp8_quantise_blocks."""
     fmt = _scale_fmt(scale_fmt)
-    stride = _matrix(w, "w")
-    N, K = w.shape
-    with _on_device(w):
-        q = torch.empty(N, K, dtype=torch.float8_e4m3fn, device=w.device)
-        scale = torch.empty((N + 127) // 128, (K + 127) // 128, dtype=torch.float32, device=w.device)
-        check(_lib.load().b200dsa_fp8_quantise_blocks(w.data_ptr(), int(w.dtype == torch.float32), stride, N, K, fmt,
-                                                      q.data_ptr(), scale.data_ptr(), stream_ptr()),
-              "b200dsa_fp8_quantise_blocks")
+    N, K, stride, f32 = _matrix(w, "w")
+    index = _device_index(w)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return fp8_quantise_blocks(w, scale_fmt=scale_fmt)
+    q = torch.empty(N, K, dtype=torch.float8_e4m3fn, device=w.device)
+    scale = torch.empty((N + 127) // 128, (K + 127) // 128, dtype=torch.float32, device=w.device)
+    check(_lib.load().b200dsa_fp8_quantise_blocks(w.data_ptr(), f32, stride, N, K, fmt, q.data_ptr(), scale.data_ptr(),
+                                                  stream_ptr()), "b200dsa_fp8_quantise_blocks")
     return q, scale
+
+
+def _fp8_weight(w: torch.Tensor, w_scale: torch.Tensor, K: int) -> int:
+    """Rows of an 8-bit weight [N, K] after its checks."""
+    if w.dtype != torch.float8_e4m3fn or w.dim() != 2 or w.stride(1) != 1:
+        raise _lib.B200DSAError("w must be float8_e4m3fn with two dims and unit column stride")
+    if w.shape[1] != K or K < 16 or K % 16:
+        raise _lib.B200DSAError("both operands must have the same number of columns, a multiple of 16")
+    N = w.shape[0]
+    if w_scale.dtype != torch.float32 or w_scale.shape != ((N + 127) // 128, (K + 127) // 128):
+        raise _lib.B200DSAError("w_scale must be fp32 [ceil(N/128), ceil(K/128)]")
+    return N
+
+
+def _fp8_result(out: Optional[torch.Tensor], out_dtype: torch.dtype, M: int, N: int) -> bool:
+    """Checks of the result's buffer and dtype; True for fp32."""
+    if out is not None:
+        out_dtype = out.dtype
+        if out.shape != (M, N) or (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
+            raise _lib.B200DSAError("out must be [M, N] with unit column stride")
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise _lib.B200DSAError("the result is bf16 or fp32")
+    return out_dtype == torch.float32
 
 
 def fp8_block_matmul(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *,
                      out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y [M, N] = (a * a_scale) @ (w * w_scale)^T for e4m3 codes a [M, K], w [N, K] with scales fp32 [M, ceil(K/128)]
     (any strides) and [ceil(N/128), ceil(K/128)]; fp32 sums, bf16 or fp32 result; see b200dsa_fp8_block_matmul."""
-    for t_, nm in ((a, "a"), (w, "w")):
-        if t_.dtype != torch.float8_e4m3fn or t_.dim() != 2 or t_.stride(1) != 1:
-            raise _lib.B200DSAError(f"{nm} must be float8_e4m3fn with two dims and unit column stride")
+    if a.dtype != torch.float8_e4m3fn or a.dim() != 2 or a.stride(1) != 1:
+        raise _lib.B200DSAError("a must be float8_e4m3fn with two dims and unit column stride")
     M, K = a.shape
-    N = w.shape[0]
-    G = (K + 127) // 128
-    if w.shape[1] != K or K < 16 or K % 16:
-        raise _lib.B200DSAError("a and w must have the same number of columns, a multiple of 16")
-    if a_scale.dtype != torch.float32 or a_scale.shape != (M, G) or w_scale.dtype != torch.float32 or \
-            w_scale.shape != ((N + 127) // 128, G):
-        raise _lib.B200DSAError("scales must be fp32 [M, ceil(K/128)] and [ceil(N/128), ceil(K/128)]")
-    with _on_device(a, a_scale, w, w_scale, out):
-        if out is None:
-            out = torch.empty(M, N, dtype=out_dtype, device=a.device)
-        elif out.shape != (M, N) or (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
-            raise _lib.B200DSAError("out must be [M, N] with unit column stride")
-        if out.dtype not in (torch.bfloat16, torch.float32):
-            raise _lib.B200DSAError("the result is bf16 or fp32")
-        check(_lib.load().b200dsa_fp8_block_matmul(
-            a.data_ptr(), a.stride(0) if M > 1 else K, a_scale.data_ptr(), a_scale.stride(0), a_scale.stride(1),
-            w.data_ptr(), w.stride(0) if N > 1 else K, w_scale.data_ptr(), w_scale.stride(0), w_scale.stride(1), M, N, K,
-            out.data_ptr(), int(out.dtype == torch.float32), _rows_stride(out, N), status_word(a.device).data_ptr(),
-            stream_ptr()), "b200dsa_fp8_block_matmul")
+    N = _fp8_weight(w, w_scale, K)
+    if a_scale.dtype != torch.float32 or a_scale.shape != (M, (K + 127) // 128):
+        raise _lib.B200DSAError("a_scale must be fp32 [M, ceil(K/128)]")
+    f32 = _fp8_result(out, out_dtype, M, N)
+    index = _device_index(a, a_scale, w, w_scale, out)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return fp8_block_matmul(a, a_scale, w, w_scale, out_dtype=out_dtype, out=out)
+    if out is None:
+        out = torch.empty(M, N, dtype=out_dtype, device=a.device)
+    sa_m, sa_g = a_scale.stride()
+    sw_r, sw_g = w_scale.stride()
+    check(_lib.load().b200dsa_fp8_block_matmul(
+        a.data_ptr(), _rows_stride(a, K), a_scale.data_ptr(), sa_m, sa_g, w.data_ptr(), _rows_stride(w, K),
+        w_scale.data_ptr(), sw_r, sw_g, M, N, K, out.data_ptr(), f32, _rows_stride(out, N), _lib.status_ptr(index),
+        stream_ptr()), "b200dsa_fp8_block_matmul")
     return out
 
 
 def fp8_block_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *, scale_fmt: Optional[str] = None,
                      out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """y = x @ (w * w_scale)^T with the activations x [M, K] (bf16 or fp32) quantised on the way:
-    fp8_block_matmul(*fp8_quantise_rows(x, scale_fmt=...), w, w_scale)."""
-    a, a_scale = fp8_quantise_rows(x, scale_fmt=scale_fmt)
-    return fp8_block_matmul(a, a_scale, w, w_scale, out_dtype=out_dtype, out=out)
+    """y = x @ (w * w_scale)^T with the activations x [M, K] (bf16 or fp32) quantised on the way: the result of
+    fp8_block_matmul(*fp8_quantise_rows(x, scale_fmt=...), w, w_scale) in one call; see b200dsa_fp8_block_linear."""
+    fmt = _scale_fmt(scale_fmt)
+    M, K, stride, x_f32 = _matrix(x, "x")
+    N = _fp8_weight(w, w_scale, K)
+    f32 = _fp8_result(out, out_dtype, M, N)
+    index = _device_index(x, w, w_scale, out)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return fp8_block_linear(x, w, w_scale, scale_fmt=scale_fmt, out_dtype=out_dtype, out=out)
+    if out is None:
+        out = torch.empty(M, N, dtype=out_dtype, device=x.device)
+    ws = torch.empty(M * (K + 4 * ((K + 127) // 128)), dtype=torch.uint8, device=x.device)   # codes, then scales
+    sw_r, sw_g = w_scale.stride()
+    check(_lib.load().b200dsa_fp8_block_linear(
+        x.data_ptr(), x_f32, stride, fmt, w.data_ptr(), _rows_stride(w, K), w_scale.data_ptr(), sw_r, sw_g, M, N, K,
+        out.data_ptr(), f32, _rows_stride(out, N), ws.data_ptr(), ws.numel(), _lib.status_ptr(index), stream_ptr()),
+        "b200dsa_fp8_block_linear")
+    return out
