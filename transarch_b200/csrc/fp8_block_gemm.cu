@@ -7,17 +7,16 @@
 // a block's product has to leave the tensor pipe before it is scaled: the inner sum of every 128-deep block is one
 // accumulator in TMEM (4 MMAs of K = 32), and fp32 registers hold the outer sum.
 //
-// Orientation: 128 weight rows are the UMMA M dimension (one TMEM lane and one epilogue thread for an output column n),
-// NT tokens are N.  A decode batch is then a narrow tile that still streams whole weight tiles, the weight scale is
-// one number for a tile and block, and the token scales are shared by all threads of the tile (read from shared memory
-// four at a time).  NT is 16 .. 256 by M.
+// Two kernels.  Few tokens (up to 128): 128 weight rows are the UMMA M dimension (one TMEM lane and one accumulating
+// thread for an output column n) and 16 .. 128 tokens are N, so that a decode batch is a narrow tile that still streams
+// whole weight tiles.  Few tiles split the blocks of K over the 2 - 8 CTAs of a cluster: each CTA keeps its partial
+// sums in its own shared memory and adds up its share of the tokens over the cluster in rank order, so the result does
+// not depend on timing and no workspace exists.
+// Many tokens: 128 tokens are M and 256 weight rows N.  A thread owns one token, so that the scale of a block is one
+// register, and the shared-memory port carries nothing but the operands (48 KB in by TMA and 48 KB out to the MMAs for
+// every 512 clocks of MMA: that port, not the tensor pipe, is what bounds this kernel).
 //
-// Few tiles (decode, narrow projections) split the blocks of K over the 2 - 8 CTAs of a cluster: each CTA keeps its
-// partial sums in its own shared memory and adds up its share of the tokens over the cluster in rank order, so the
-// result does not depend on timing and no workspace exists.
-//
-// Roles (352 threads): warp 0 TMA loads, warp 1 MMA, warp 2 scales, warps 3-10 accumulate (two warps per TMEM lane
-// quadrant, half of the token columns each).  Every wait is bounded.
+// Every wait is bounded.
 #include <stdio.h>
 
 #include "latent_cache.cuh"
@@ -38,6 +37,7 @@ struct GemmParams {
   void* out;                   // [M, N], rows ldo elements apart
   int64_t ldo;
   int out_f32, out_pair;       // out_pair: bf16 rows start on 4-byte boundaries
+  int out_vec;                 // rows of the result start on 16-byte boundaries
   int m, n, blocks;            // blocks of K
   int m_tiles, n_tiles, splits;
   int32_t* status;
@@ -46,15 +46,15 @@ struct GemmParams {
 template <int NT>
 struct GemmShape {
   static constexpr int kWBytes = 128 * 128, kABytes = NT * 128, kStageBytes = kWBytes + kABytes;
-  static constexpr int kStages = NT == 256 ? 4 : NT == 128 ? 6 : 8;
-  static constexpr int kAccBufs = NT == 256 ? 2 : 4;
+  static constexpr int kStages = NT == 128 ? 6 : 8;
+  static constexpr int kAccBufs = 4;
   static constexpr uint32_t kTmemCols = NT * kAccBufs < 32 ? 32 : NT * kAccBufs;
   static constexpr int kCols = NT / 2;                        // token columns of one accumulating warp
   static constexpr int kScaleOff = kStages * kStageBytes;
   static constexpr int kBarOff = kScaleOff + kGemmScaleSlots * NT * 4;
   static constexpr int kSmem = kBarOff + 256 + 1024;
   // partial sums of a split tile live where the operand ring was: NT tokens x 128 columns fp32
-  static_assert(NT > 128 || NT * 128 * 4 <= kStages * kStageBytes, "partial sums must fit the operand ring");
+  static_assert(NT <= 128 && NT * 128 * 4 <= kStages * kStageBytes, "partial sums must fit the operand ring");
 };
 
 __device__ __forceinline__ uint32_t gemm_cluster_rank() {
@@ -65,11 +65,13 @@ __device__ __forceinline__ uint32_t gemm_cluster_rank() {
 __device__ __forceinline__ void gemm_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float gemm_ld_cluster(uint32_t addr, uint32_t rank) {
+__device__ __forceinline__ float4 gemm_ld_cluster(uint32_t addr, uint32_t rank) {
   uint32_t r;
-  float v;
+  float4 v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(r) : "memory");
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(r));
   return v;
 }
 __device__ __forceinline__ void tmem_ld_32x8(uint32_t taddr, uint32_t (&v)[8]) {
@@ -77,6 +79,36 @@ __device__ __forceinline__ void tmem_ld_32x8(uint32_t taddr, uint32_t (&v)[8]) {
                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
                : "r"(taddr)
                : "memory");
+}
+
+template <int N>
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&v)[N]) {
+  static_assert(N == 8 || N == 16 || N == 32, "columns of one load");
+  if constexpr (N == 8) tmem_ld_32x8(taddr, v);
+  else if constexpr (N == 16) tmem_ld_32x16(taddr, v);
+  else tmem_ld_32x32(taddr, v);
+}
+
+// Two fp32 sums in one 64-bit register pair: a += (x0, x1) * s, one packed instruction.
+__device__ __forceinline__ void fma_pair(uint64_t& a, uint32_t x0, uint32_t x1, uint64_t s) {
+  asm("{\n\t.reg .b64 x;\n\t"
+      "mov.b64 x, {%1, %2};\n\t"
+      "fma.rn.f32x2 %0, x, %3, %0;\n\t}"
+      : "+l"(a)
+      : "r"(x0), "r"(x1), "l"(s));
+}
+__device__ __forceinline__ void fma_pairs(uint64_t& a, uint64_t x, uint64_t s) {
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(a) : "l"(x), "l"(s));
+}
+__device__ __forceinline__ uint64_t pair_of(float v) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
 }
 
 // One output value pair for tokens t and t + 1 of thread column n: neighbouring lanes swap one value, so that each
@@ -95,6 +127,38 @@ __device__ __forceinline__ void store_bf16_pair(const GemmParams& p, float v0, f
     o[0] = __float2bfloat16_rn(x);
     if (c + 1 < p.n) o[1] = __float2bfloat16_rn(y);
   }
+}
+
+// Sum of the cluster's partial sums of columns n .. n + 3 of a token, in rank order; `at`: where they lie in every CTA.
+__device__ __forceinline__ void add_partials(const GemmParams& p, uint32_t at, int tok, int n) {
+          float4 v[8];
+  #pragma unroll
+          for (int r = 0; r < 8; ++r)
+            if (r < p.splits) v[r] = gemm_ld_cluster(at, r);
+          float4 sum = v[0];
+  #pragma unroll
+          for (int r = 1; r < 8; ++r)
+            if (r < p.splits) {
+              sum.x += v[r].x; sum.y += v[r].y; sum.z += v[r].z; sum.w += v[r].w;
+            }
+          const int64_t o = static_cast<int64_t>(tok) * p.ldo + n;
+          const float x[4] = {sum.x, sum.y, sum.z, sum.w};
+          if (p.out_vec && n + 4 <= p.n) {
+            if (p.out_f32) {
+              *reinterpret_cast<float4*>(static_cast<float*>(p.out) + o) = sum;
+            } else {
+              const __nv_bfloat162 lo = __floats2bfloat162_rn(sum.x, sum.y), hi = __floats2bfloat162_rn(sum.z, sum.w);
+              *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + o) =
+                  make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+            }
+          } else {
+  #pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (n + j < p.n) {
+                if (p.out_f32) static_cast<float*>(p.out)[o + j] = x[j];
+                else static_cast<__nv_bfloat16*>(p.out)[o + j] = __float2bfloat16_rn(x[j]);
+              }
+          }
 }
 
 template <int NT>
@@ -153,53 +217,55 @@ fp8_block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
 
   if (warp == 0) {
     // ------------------------------------------------------------------ loads
-    int it = 0;
-    bool ok = true;
-    for (int w = first; ok && w < n_work; w += stride) {
-      const int n0 = (w % p.n_tiles) * 128, m0 = (w / p.n_tiles) * NT;
-      for (int b = b_lo; b < b_hi; ++b, ++it) {
-        const int s = it % S::kStages;
-        ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ((it / S::kStages) & 1) ^ 1, abort_flag));
-        if (!ok) break;
-        if (elect_one()) {
+    if (lane == 0) {
+      int it = 0;
+      bool ok = true;
+      for (int w = first; ok && w < n_work; w += stride) {
+        const int n0 = (w % p.n_tiles) * 128, m0 = (w / p.n_tiles) * NT;
+        for (int b = b_lo; b < b_hi; ++b, ++it) {
+          const int s = it % S::kStages;
+          ok = mbar_wait(&empty[s], ((it / S::kStages) & 1) ^ 1, abort_flag);
+          if (!ok) break;
           uint8_t* dst = smem_al + s * S::kStageBytes;
           mbar_arrive_expect_tx(&full[s], S::kStageBytes);
           tma_load_2d(dst, &tmap_w, &full[s], b * 128, n0);
           tma_load_2d(dst + S::kWBytes, &tmap_a, &full[s], b * 128, m0);
         }
-        __syncwarp();
+      }
+      // whatever ended the loop, the copies in flight land before the shared memory is given up
+      for (int j = it > S::kStages ? it - S::kStages : 0; j < it; ++j) {
+        const long long t0 = clock64();
+        while (!mbar_test(&full[j % S::kStages], (j / S::kStages) & 1) && clock64() - t0 < kWaitLimitCycles) {
+        }
       }
     }
-    // whatever ended the loop, the copies in flight land before the shared memory is given up
-    for (int j = it > S::kStages ? it - S::kStages : 0; j < it; ++j) {
-      const long long t0 = clock64();
-      while (!mbar_test(&full[j % S::kStages], (j / S::kStages) & 1) && clock64() - t0 < kWaitLimitCycles) {
-      }
-    }
+    __syncwarp();
   } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMA
-    constexpr uint32_t idesc = make_idesc(kFmtE4M3, kFmtE4M3, 128, NT);
-    int it = 0;
-    bool ok = true;
-    for (int w = first; ok && w < n_work; w += stride) {
-      for (int b = b_lo; b < b_hi; ++b, ++it) {
-        const int s = it % S::kStages, buf = it % S::kAccBufs;
-        ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[buf], ((it / S::kAccBufs) & 1) ^ 1, abort_flag) &&
-                                         mbar_wait(&full[s], (it / S::kStages) & 1, abort_flag));
-        if (!ok) break;
-        tc_fence_after();
-        if (elect_one()) {
+    // ------------------------------------------------------------------ MMA (one thread: nothing but waits and issues)
+    if (lane == 0) {
+      constexpr uint32_t idesc = make_idesc(kFmtE4M3, kFmtE4M3, 128, NT);
+      int it = 0;
+      bool ok = true;
+      for (int w = first; ok && w < n_work; w += stride) {
+        for (int b = b_lo; b < b_hi; ++b, ++it) {
+          const int s = it % S::kStages, buf = it % S::kAccBufs, sl = it % kGemmScaleSlots;
+          // the block's scales are waited for here, so that the accumulating warps have one barrier to look at
+          ok = mbar_wait(&sc_full[sl], (it / kGemmScaleSlots) & 1, abort_flag) &&
+               mbar_wait(&acc_empty[buf], ((it / S::kAccBufs) & 1) ^ 1, abort_flag) &&
+               mbar_wait(&full[s], (it / S::kStages) & 1, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
           const uint64_t wd = make_desc_k_sw128(smem_base + s * S::kStageBytes);
           const uint64_t ad = make_desc_k_sw128(smem_base + s * S::kStageBytes + S::kWBytes);
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
             mma_f8f6f4_ss(tmem_base + buf * NT, wd + 2 * kk, ad + 2 * kk, idesc, kk != 0);
-          tc_commit(&empty[s]);
           tc_commit(&acc_full[buf]);
+          tc_commit(&empty[s]);
         }
-        __syncwarp();
       }
     }
+    __syncwarp();
   } else if (warp == 2) {
     // ------------------------------------------------------------------ scales, four blocks of loads in flight
     constexpr int kPer = NT <= 32 ? 1 : NT / 32;
@@ -209,16 +275,15 @@ fp8_block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
     for (int w = first; ok && w < n_work; w += stride) {
       const int nb = w % p.n_tiles, m0 = (w / p.n_tiles) * NT;
       for (int b0 = b_lo; ok && b0 < b_hi; b0 += kAhead) {
-        float v[kAhead][kPer];
+        // every load is issued before the first is used: addresses are clamped, what lies outside becomes zero below
+        float v[kAhead][kPer], ws[kAhead];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-          const int b = b0 + u;
-          const float ws = b < b_hi ? __ldg(p.w_scale + nb * p.sw_r + b * p.sw_g) : 0.f;
+          const int b = min(b0 + u, b_hi - 1);
+          ws[u] = __ldg(p.w_scale + nb * p.sw_r + b * p.sw_g);
 #pragma unroll
-          for (int j = 0; j < kPer; ++j) {
-            const int t = m0 + lane + 32 * j;
-            v[u][j] = b < b_hi && t < p.m && lane + 32 * j < NT ? ws * __ldg(p.a_scale + t * p.sa_m + b * p.sa_g) : 0.f;
-          }
+          for (int j = 0; j < kPer; ++j)
+            v[u][j] = __ldg(p.a_scale + min(m0 + lane + 32 * j, p.m - 1) * p.sa_m + b * p.sa_g);
         }
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
@@ -228,7 +293,8 @@ fp8_block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
           if (!ok) break;
 #pragma unroll
           for (int j = 0; j < kPer; ++j)
-            if (lane + 32 * j < NT) s_scale[sl * NT + lane + 32 * j] = v[u][j];
+            if (lane + 32 * j < NT)
+              s_scale[sl * NT + lane + 32 * j] = m0 + lane + 32 * j < p.m ? ws[u] * v[u][j] : 0.f;
           mbar_arrive(&sc_full[sl]);
           ++it;
         }
@@ -239,41 +305,52 @@ fp8_block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
     const int wq = warp & 3, half = (warp - 3) >> 2;       // warps 3..6: first half of the tokens, 7..10: second
     const uint32_t lane_addr = static_cast<uint32_t>(wq * 32) << 16;
     const int row = wq * 32 + lane, col0 = half * S::kCols;
-    constexpr int kChunk = S::kCols < 16 ? 8 : 16;
+    constexpr int kChunk = S::kCols < 32 ? S::kCols : 32, kChunks = S::kCols / kChunk;
     int it = 0;
     bool ok = true;
     for (int w = first; ok && w < n_work; w += stride) {
-      float acc[S::kCols];
+      uint64_t acc[S::kCols / 2];
 #pragma unroll
-      for (int j = 0; j < S::kCols; ++j) acc[j] = 0.f;
+      for (int j = 0; j < S::kCols / 2; ++j) acc[j] = 0;
+      uint32_t v[2][kChunk];
+      auto first_columns = [&](int i) -> bool {            // wait for block product i, start on its columns
+        const bool there = __all_sync(0xffffffffu, mbar_wait(&acc_full[i % S::kAccBufs], (i / S::kAccBufs) & 1, abort_flag));
+        tc_fence_after();
+        tmem_ld_cols<kChunk>(tmem_base + lane_addr + (i % S::kAccBufs) * NT + col0, v[0]);
+        return there;
+      };
+      ok = first_columns(it);
+      if (!ok) break;
+#pragma unroll 1
       for (int b = b_lo; b < b_hi; ++b, ++it) {
         const int buf = it % S::kAccBufs, sl = it % kGemmScaleSlots;
-        ok = __all_sync(0xffffffffu, mbar_wait(&sc_full[sl], (it / kGemmScaleSlots) & 1, abort_flag) &&
-                                         mbar_wait(&acc_full[buf], (it / S::kAccBufs) & 1, abort_flag));
-        if (!ok) break;
-        tc_fence_after();
-        const float4* sc = reinterpret_cast<const float4*>(s_scale + sl * NT + col0);
+        const ulonglong2* sc = reinterpret_cast<const ulonglong2*>(s_scale + sl * NT + col0);
 #pragma unroll
-        for (int c = 0; c < S::kCols; c += kChunk) {
-          uint32_t v[kChunk];
-          if constexpr (kChunk == 8) tmem_ld_32x8(tmem_base + lane_addr + buf * NT + col0 + c, v);
-          else tmem_ld_32x16(tmem_base + lane_addr + buf * NT + col0 + c, v);
+        for (int c = 0; c < kChunks; ++c) {      // the next columns are under way while these are added
           tc_wait_ld();
+          uint64_t x[kChunk / 2];
 #pragma unroll
-          for (int j = 0; j < kChunk; j += 4) {
-            const float4 f = sc[(c + j) >> 2];
-            acc[c + j] = fmaf(__uint_as_float(v[j]), f.x, acc[c + j]);
-            acc[c + j + 1] = fmaf(__uint_as_float(v[j + 1]), f.y, acc[c + j + 1]);
-            acc[c + j + 2] = fmaf(__uint_as_float(v[j + 2]), f.z, acc[c + j + 2]);
-            acc[c + j + 3] = fmaf(__uint_as_float(v[j + 3]), f.w, acc[c + j + 3]);
+          for (int j = 0; j < kChunk / 2; ++j)
+            asm("mov.b64 %0, {%1, %2};" : "=l"(x[j]) : "r"(v[c & 1][2 * j]), "r"(v[c & 1][2 * j + 1]));
+          if (c + 1 < kChunks) {
+            tmem_ld_cols<kChunk>(tmem_base + lane_addr + buf * NT + col0 + (c + 1) * kChunk, v[(c + 1) & 1]);
+          } else {
+            tc_fence_before();                   // everything is in registers: the buffer may be written
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[buf]);
+            if (kChunks > 1 && b + 1 < b_hi) ok = first_columns(it + 1);
+          }
+#pragma unroll
+          for (int j = 0; j < kChunk / 2; j += 2) {
+            const ulonglong2 f = sc[(c * kChunk + 2 * j) >> 2];
+            fma_pairs(acc[c * kChunk / 2 + j], x[j], f.x);
+            fma_pairs(acc[c * kChunk / 2 + j + 1], x[j + 1], f.y);
           }
         }
-        tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&acc_empty[buf]);
-          mbar_arrive(&sc_empty[sl]);
-        }
+        if (lane == 0) mbar_arrive(&sc_empty[sl]);
+        if (kChunks == 1 && b + 1 < b_hi) ok = first_columns(it + 1);
+        if (!ok) break;
       }
       if (!ok) break;
       const int n = (w % p.n_tiles) * 128 + row, m0 = (w / p.n_tiles) * NT + col0;
@@ -281,14 +358,23 @@ fp8_block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
         // every MMA of this CTA has read its operands: the ring holds the partial sums now, [token][128]
         float* part = reinterpret_cast<float*>(smem_al);
 #pragma unroll
-        for (int j = 0; j < S::kCols; ++j) part[(col0 + j) * 128 + row] = acc[j];
+        for (int j = 0; j < S::kCols; j += 2) {
+          const float2 f = unpair(acc[j / 2]);
+          part[(col0 + j) * 128 + row] = f.x;
+          part[(col0 + j + 1) * 128 + row] = f.y;
+        }
       } else if (p.out_f32) {
 #pragma unroll
-        for (int j = 0; j < S::kCols; ++j)
-          if (n < p.n && m0 + j < p.m) static_cast<float*>(p.out)[static_cast<int64_t>(m0 + j) * p.ldo + n] = acc[j];
+        for (int j = 0; j < S::kCols; ++j) {
+          const float2 f = unpair(acc[j / 2]);
+          if (n < p.n && m0 + j < p.m) static_cast<float*>(p.out)[static_cast<int64_t>(m0 + j) * p.ldo + n] = j & 1 ? f.y : f.x;
+        }
       } else {
 #pragma unroll
-        for (int j = 0; j < S::kCols; j += 2) store_bf16_pair(p, acc[j], acc[j + 1], m0 + j, n, lane);
+        for (int j = 0; j < S::kCols; j += 2) {
+          const float2 f = unpair(acc[j / 2]);
+          store_bf16_pair(p, f.x, f.y, m0 + j, n, lane);
+        }
       }
     }
   }
@@ -298,27 +384,14 @@ fp8_block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
     // one tile per cluster: add the partial sums of this CTA's share of the tokens in rank order
     gemm_cluster_sync();
     if (warp >= 3) {
-      const int t = tid - 96, row = t & 127, pair = t >> 7;           // 256 threads: two token pairs at a time
       const int n0 = (first % p.n_tiles) * 128, m0 = (first / p.n_tiles) * NT;
-      const int per = (NT / 2 + p.splits - 1) / p.splits;             // token pairs of a CTA
-      const uint32_t base = smem_base + row * 4;
-      for (int q = rank * per + pair; q < min((rank + 1) * per, NT / 2); q += 2) {
-        if (m0 + 2 * q >= p.m) break;
-        float v0 = 0.f, v1 = 0.f;
-        for (int r = 0; r < p.splits; ++r) {
-          v0 += gemm_ld_cluster(base + (2 * q) * 512, r);
-          v1 += gemm_ld_cluster(base + (2 * q + 1) * 512, r);
-        }
-        if (p.out_f32) {
-          float* o = static_cast<float*>(p.out) + static_cast<int64_t>(m0 + 2 * q) * p.ldo + n0 + row;
-          if (n0 + row < p.n) {
-            o[0] = v0;
-            if (m0 + 2 * q + 1 < p.m) o[p.ldo] = v1;
-          }
-        } else {
-          store_bf16_pair(p, v0, v1, m0 + 2 * q, n0 + row, lane);
-        }
+      const int per = NT / p.splits;                                  // tokens of a CTA
+      for (int i = tid - 96; i < per * 32; i += 256) {                // a thread: four neighbouring columns of a token
+        const int tok = rank * per + (i >> 5), n = n0 + (i & 31) * 4;
+        if (m0 + tok >= p.m || n >= p.n) continue;
+        add_partials(p, smem_base + tok * 512 + (i & 31) * 16, m0 + tok, n);
       }
+      __syncwarp();
     }
     gemm_cluster_sync();               // nobody leaves while a peer reads its shared memory
   }
@@ -329,21 +402,15 @@ fp8_block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
   if (tid == 0 && s_abort) atomicMax(p.status, kDevWaitTimeout);
 }
 
-template <int NT>
-static cudaError_t gemm_launch(const CUtensorMap& mw, const CUtensorMap& ma, const GemmParams& p, const DeviceInfo& dev,
-                               bool dependent, cudaStream_t stream) {
-  using S = GemmShape<NT>;
-  static OncePerDevice once;
-  cudaError_t e = once.run(dev.index, [] {
-    return cudaFuncSetAttribute(fp8_block_gemm_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
-  });
-  if (e != cudaSuccess) return e;
-  const int sms = dev.sms;
+// Persistent CTAs over the tiles, or one cluster of p.splits CTAs a tile.
+static cudaError_t gemm_launch_config(void (*kernel)(CUtensorMap, CUtensorMap, GemmParams), int threads, int smem,
+                                      const CUtensorMap& mw, const CUtensorMap& ma, const GemmParams& p, int sms,
+                                      bool dependent, cudaStream_t stream) {
   const int tiles = p.m_tiles * p.n_tiles;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(p.splits > 1 ? tiles * p.splits : (tiles < sms ? tiles : sms));
-  cfg.blockDim = dim3(kGemmThreads);
-  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   int na = 0;
@@ -361,8 +428,293 @@ static cudaError_t gemm_launch(const CUtensorMap& mw, const CUtensorMap& ma, con
   }
   cfg.attrs = attr;
   cfg.numAttrs = na;
-  e = cudaLaunchKernelEx(&cfg, fp8_block_gemm_kernel<NT>, mw, ma, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, mw, ma, p);
   return e == cudaSuccess ? cudaGetLastError() : e;
+}
+
+template <int NT>
+static cudaError_t gemm_launch(const CUtensorMap& mw, const CUtensorMap& ma, const GemmParams& p, const DeviceInfo& dev,
+                               bool dependent, cudaStream_t stream) {
+  using S = GemmShape<NT>;
+  static OncePerDevice once;
+  cudaError_t e = once.run(dev.index, [] {
+    return cudaFuncSetAttribute(fp8_block_gemm_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+  });
+  if (e != cudaSuccess) return e;
+  return gemm_launch_config(fp8_block_gemm_kernel<NT>, kGemmThreads, S::kSmem, mw, ma, p, dev.sms, dependent, stream);
+}
+
+// ---------------------------------------------------------------------------------------- many tokens
+// 384 threads: warp 0 TMA loads, warp 1 MMA (warps 2 and 3 fill their warpgroup), warps 4-11 accumulate, two a TMEM lane
+// quadrant, 128 columns (one block of weight rows, one weight scale) each.  A thread holds 128 fp32 sums: the register
+// split gives the accumulating warps 232 registers and the others 40, or 224 and 56 in the split form, whose issuing
+// threads hold more (128 * 40 + 256 * 232 = 128 * 56 + 256 * 224 = 384 * 168).  A spill in either costs 15 - 50 %.
+constexpr int kWideThreads = 384;
+constexpr int kWideStages = 4;
+constexpr int kWideABytes = 128 * 128, kWideWBytes = 256 * 128, kWideStageBytes = kWideABytes + kWideWBytes;
+constexpr int kWideOutOff = kWideStages * kWideStageBytes;          // 8 warps x 32 rows x 128 bytes
+constexpr int kWideBarOff = kWideOutOff + 8 * 32 * 128;
+constexpr int kWideSmem = kWideBarOff + 256 + 1024;
+
+// The warp's staged 32 rows of 128 bytes to the result: a store instruction covers 128 bytes of four rows.  kElem: bytes
+// of a value.
+template <int kElem>
+__device__ __forceinline__ void wide_store(const GemmParams& p, uint32_t stage, int m0, int n0, int lane) {
+  constexpr int kPer = 16 / kElem;                  // values of a piece
+  const int n = n0 + (lane & 7) * kPer;
+  if (n >= p.n) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = 4 * i + (lane >> 3);
+    if (m0 + r >= p.m) break;
+    uint32_t v[4];
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                 : "r"(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4)));
+    uint8_t* o = static_cast<uint8_t*>(p.out) + (static_cast<int64_t>(m0 + r) * p.ldo + n) * kElem;
+    if (p.out_vec && n + kPer <= p.n) {
+      *reinterpret_cast<uint4*>(o) = make_uint4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j)
+        if (n + j < p.n) {
+          if constexpr (kElem == 4) reinterpret_cast<uint32_t*>(o)[j] = v[j];
+          else reinterpret_cast<uint16_t*>(o)[j] = static_cast<uint16_t>(v[j >> 1] >> (16 * (j & 1)));
+        }
+    }
+  }
+}
+
+template <bool kSplit>      // K cut over a cluster; a kernel of its own, because its exchange costs the other one registers
+__global__ void __launch_bounds__(kWideThreads, 1)
+fp8_block_gemm_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_a,
+                           const GemmParams p) {
+  pdl_launch_dependents();
+  extern __shared__ uint8_t smem_dyn[];
+  __shared__ uint32_t s_tmem_base;
+  __shared__ int s_abort;
+  const uint32_t smem_base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
+  uint8_t* smem_al = smem_dyn + (smem_base - smem_u32(smem_dyn));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem_al + kWideBarOff);   // [stages] bytes of an operand pair
+  uint64_t* empty = full + kWideStages;                                  // [stages] MMAs of the stage retired
+  uint64_t* acc_full = empty + kWideStages;                              // [2] block product complete
+  uint64_t* acc_empty = acc_full + 2;                                    // [2] eight warps have read it
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  volatile int* abort_flag = &s_abort;
+  if (tid == 0) {
+    s_abort = 0;
+    for (int s = 0; s < kWideStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&acc_full[s], 1);
+      mbar_init(&acc_empty[s], 8);
+    }
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&s_tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = s_tmem_base;
+  pdl_wait_prior();
+  const int n_work = p.m_tiles * p.n_tiles;
+  const int rank = kSplit ? static_cast<int>(gemm_cluster_rank()) : 0;
+  const int first = kSplit ? blockIdx.x / p.splits : blockIdx.x, stride = kSplit ? gridDim.x / p.splits : gridDim.x;
+  const int b_lo = kSplit ? static_cast<int>(static_cast<int64_t>(p.blocks) * rank / p.splits) : 0;
+  const int b_hi = kSplit ? static_cast<int>(static_cast<int64_t>(p.blocks) * (rank + 1) / p.splits) : p.blocks;
+
+  if (warp < 4) {
+    if (kSplit) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 0 && lane == 0) {
+      int it = 0;
+      bool ok = true;
+      for (int w = first; ok && w < n_work; w += stride) {
+        const int n0 = (w % p.n_tiles) * 256, m0 = (w / p.n_tiles) * 128;
+        for (int b = b_lo; b < b_hi; ++b, ++it) {
+          const int s = it % kWideStages;
+          ok = mbar_wait(&empty[s], ((it / kWideStages) & 1) ^ 1, abort_flag);
+          if (!ok) break;
+          uint8_t* dst = smem_al + s * kWideStageBytes;
+          mbar_arrive_expect_tx(&full[s], kWideStageBytes);
+          tma_load_2d(dst, &tmap_a, &full[s], b * 128, m0);
+          tma_load_2d(dst + kWideABytes, &tmap_w, &full[s], b * 128, n0);
+        }
+      }
+      // whatever ended the loop, the copies in flight land before the shared memory is given up
+      for (int j = it > kWideStages ? it - kWideStages : 0; j < it; ++j) {
+        const long long t0 = clock64();
+        while (!mbar_test(&full[j % kWideStages], (j / kWideStages) & 1) && clock64() - t0 < kWaitLimitCycles) {
+        }
+      }
+    } else if (warp == 1 && lane == 0) {
+      constexpr uint32_t idesc = make_idesc(kFmtE4M3, kFmtE4M3, 128, 256);
+      int it = 0;
+      bool ok = true;
+      for (int w = first; ok && w < n_work; w += stride) {
+        for (int b = b_lo; b < b_hi; ++b, ++it) {
+          const int s = it % kWideStages, buf = it & 1;
+          ok = mbar_wait(&acc_empty[buf], ((it >> 1) & 1) ^ 1, abort_flag) &&
+               mbar_wait(&full[s], (it / kWideStages) & 1, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t ad = make_desc_k_sw128(smem_base + s * kWideStageBytes);
+          const uint64_t wd = make_desc_k_sw128(smem_base + s * kWideStageBytes + kWideABytes);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma_f8f6f4_ss(tmem_base + buf * 256, ad + 2 * kk, wd + 2 * kk, idesc, kk != 0);
+          tc_commit(&acc_full[buf]);
+          tc_commit(&empty[s]);
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    if (kSplit) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    const int wq = warp & 3, half = (warp - 4) >> 2;
+    const uint32_t src0 = tmem_base + (static_cast<uint32_t>(wq * 32) << 16) + half * 128;
+    const uint32_t stage = smem_base + kWideOutOff + (warp - 4) * 4096;
+    int it = 0;
+    bool ok = true;
+    for (int w = first; ok && w < n_work; w += stride) {
+      const int n0 = (w % p.n_tiles) * 256 + half * 128, m0 = (w / p.n_tiles) * 128 + wq * 32;
+      const bool live = m0 + lane < p.m && n0 < p.n;
+      const float* sa = p.a_scale + static_cast<int64_t>(m0 + lane) * p.sa_m + b_lo * p.sa_g;
+      const float* sw = p.w_scale + static_cast<int64_t>(n0 >> 7) * p.sw_r + b_lo * p.sw_g;
+      // scales of the next two blocks are under way
+      float sn[2], wn[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const bool in = live && b_lo + u < b_hi;
+        sn[u] = in ? __ldg(sa + u * p.sa_g) : 0.f;
+        wn[u] = in ? __ldg(sw + u * p.sw_g) : 0.f;
+      }
+      sa += 2 * p.sa_g;
+      sw += 2 * p.sw_g;
+      uint64_t acc[64];
+#pragma unroll
+      for (int j = 0; j < 64; ++j) acc[j] = 0;
+      constexpr int kCols = 32;                            // columns of a load
+      uint32_t v[2][kCols];
+      auto first_columns = [&](int i) -> bool {            // wait for block product i, start on its columns
+        const bool there = __all_sync(0xffffffffu, mbar_wait(&acc_full[i & 1], (i >> 1) & 1, abort_flag));
+        tc_fence_after();
+        tmem_ld_cols<kCols>(src0 + (i & 1) * 256, v[0]);
+        return there;
+      };
+      ok = first_columns(it);
+      if (!ok) break;
+#pragma unroll 2
+      for (int b = b_lo; b < b_hi; ++b, ++it) {
+        const uint64_t s = pair_of(sn[0] * wn[0]);
+        sn[0] = sn[1];
+        wn[0] = wn[1];
+        const bool in = live && b + 2 < b_hi;
+        sn[1] = in ? __ldg(sa) : 0.f;
+        wn[1] = in ? __ldg(sw) : 0.f;
+        sa += p.sa_g;
+        sw += p.sw_g;
+        const int buf = it & 1;
+#pragma unroll
+        for (int c = 0; c < 128 / kCols; ++c) {
+          tc_wait_ld();
+          if (c + 1 < 128 / kCols) {
+            tmem_ld_cols<kCols>(src0 + buf * 256 + (c + 1) * kCols, v[(c + 1) & 1]);
+          } else {
+            tc_fence_before();                             // everything is in registers: the buffer may be written
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[buf]);
+            if (b + 1 < b_hi) ok = first_columns(it + 1);   // of the next block, under the additions below
+          }
+#pragma unroll
+          for (int j = 0; j < kCols; j += 2) fma_pair(acc[(c * kCols + j) / 2], v[c & 1][j], v[c & 1][j + 1], s);
+        }
+        if (!ok) break;
+      }
+      if (!ok) break;
+      if (kSplit) {
+        // every MMA of this CTA has read its operands: the ring holds the partial sums now, [token][256], 16-byte pieces
+        // swizzled by token
+        const uint32_t part = smem_base + (wq * 32 + lane) * 1024;
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          asm volatile("st.shared.v2.b64 [%0], {%1, %2};" ::"r"(part + (((half * 32 + j) ^ (lane & 7)) << 4)),
+                       "l"(acc[2 * j]), "l"(acc[2 * j + 1]) : "memory");
+        continue;
+      }
+      if (n0 >= p.n) continue;
+      if (p.out_f32) {
+        // 32 columns at a time: a lane writes its row's 128 bytes into the warp's 4 KB, 16-byte pieces swizzled by row,
+        // and reads back pieces of four rows that lie side by side
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            asm volatile("st.shared.v2.b64 [%0], {%1, %2};" ::"r"(stage + lane * 128 + ((j ^ (lane & 7)) << 4)),
+                         "l"(acc[c * 16 + j * 2]), "l"(acc[c * 16 + j * 2 + 1]) : "memory");
+          __syncwarp();
+          wide_store<4>(p, stage, m0, n0 + c * 32, lane);
+          __syncwarp();
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            uint32_t o[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const float2 f = unpair(acc[c * 32 + j * 4 + q]);
+              const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+              o[q] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 128 + ((j ^ (lane & 7)) << 4)),
+                         "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
+          }
+          __syncwarp();
+          wide_store<2>(p, stage, m0, n0 + c * 64, lane);
+          __syncwarp();
+        }
+      }
+    }
+  }
+  __syncwarp();
+  if (kSplit) {
+    // one tile per cluster: add the partial sums of this CTA's share of the tokens in rank order
+    gemm_cluster_sync();
+    if (warp >= 4) {
+      const int n0 = (first % p.n_tiles) * 256, m0 = (first / p.n_tiles) * 128, per = 128 / p.splits;
+      for (int i = tid - 128; i < per * 64; i += 256) {               // a thread: four neighbouring columns of a token
+        const int tok = rank * per + (i >> 6), n = n0 + (i & 63) * 4;
+        if (m0 + tok < p.m && n < p.n)
+          add_partials(p, smem_base + tok * 1024 + (((i & 63) ^ (tok & 7)) << 4), m0 + tok, n);
+      }
+    }
+    __syncwarp();
+    gemm_cluster_sync();               // nobody leaves while a peer reads its shared memory
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem_base, 512);
+  if (tid == 0 && s_abort) atomicMax(p.status, kDevWaitTimeout);
+}
+
+template <bool kSplit>
+static cudaError_t wide_launch(const CUtensorMap& mw, const CUtensorMap& ma, const GemmParams& p, const DeviceInfo& dev,
+                               bool dependent, cudaStream_t stream) {
+  static OncePerDevice once;
+  cudaError_t e = once.run(dev.index, [] {
+    return cudaFuncSetAttribute(fp8_block_gemm_wide_kernel<kSplit>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideSmem);
+  });
+  if (e != cudaSuccess) return e;
+  return gemm_launch_config(fp8_block_gemm_wide_kernel<kSplit>, kWideThreads, kWideSmem, mw, ma, p, dev.sms, dependent, stream);
 }
 
 // ---------------------------------------------------------------------------------------- quantisers
@@ -372,7 +724,7 @@ constexpr int kQuantPairs = 4;         // group pairs of a warp, loads of all of
 
 struct QuantRowsParams {
   const void* in;
-  int in_f32, in_vec;
+  int in_vec;                  // rows start on 16-byte boundaries
   int64_t in_stride, m;
   int k;
   uint8_t* q;                  // [m, k]
@@ -381,34 +733,39 @@ struct QuantRowsParams {
   int use_ue8m0;
 };
 
-__device__ __forceinline__ void quant_load8(const QuantRowsParams& p, int64_t i, float (&x)[8]) {
-  if (p.in_f32) {
-    const float* q = static_cast<const float*>(p.in) + i;
-    if (p.in_vec) {
-      const float4 a = __ldg(reinterpret_cast<const float4*>(q)), b = __ldg(reinterpret_cast<const float4*>(q) + 1);
-      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-      x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    } else {
+// Eight values as they lie in memory (bf16 packed: half the registers of a batch of loads), widened when they are used.
+template <bool kF32>
+struct Raw8 {
+  uint32_t w[kF32 ? 8 : 4];
+  __device__ __forceinline__ void load(const void* in, int64_t i, int vec) {
+    if (kF32) {
+      const uint32_t* q = static_cast<const uint32_t*>(in) + i;
+      if (vec) {
+        const uint4 a = __ldg(reinterpret_cast<const uint4*>(q)), b = __ldg(reinterpret_cast<const uint4*>(q) + 1);
+        w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+        w[4 % (kF32 ? 8 : 4)] = b.x; w[5 % (kF32 ? 8 : 4)] = b.y; w[6 % (kF32 ? 8 : 4)] = b.z; w[7 % (kF32 ? 8 : 4)] = b.w;
+      } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = __ldg(q + j);
-    }
-  } else {
-    const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(p.in) + i;
-    if (p.in_vec) {
-      const uint4 a = __ldg(reinterpret_cast<const uint4*>(q));
-      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[2 * j] = __uint_as_float(w[j] << 16);
-        x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+        for (int j = 0; j < (kF32 ? 8 : 4); ++j) w[j] = __ldg(q + j);
       }
     } else {
+      const uint16_t* q = static_cast<const uint16_t*>(in) + i;
+      if (vec) {
+        const uint4 a = __ldg(reinterpret_cast<const uint4*>(q));
+        w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+      } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = __bfloat162float(q[j]);
+        for (int j = 0; j < 4; ++j) w[j] = __ldg(q + 2 * j) | static_cast<uint32_t>(__ldg(q + 2 * j + 1)) << 16;
+      }
     }
   }
-}
+  __device__ __forceinline__ float operator[](int j) const {
+    if (kF32) return __uint_as_float(w[j % (kF32 ? 8 : 4)]);
+    return __uint_as_float(j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16);
+  }
+};
 
+template <bool kF32>
 __global__ void __launch_bounds__(256) fp8_quantise_rows_kernel(const QuantRowsParams p) {
   pdl_launch_dependents();
   pdl_wait_prior();
@@ -416,26 +773,25 @@ __global__ void __launch_bounds__(256) fp8_quantise_rows_kernel(const QuantRowsP
   if (row >= p.m) return;
   const int lane = threadIdx.x & 31;
   const int k0 = blockIdx.y * (kQuantPairs * 256) + lane * 8;
-  float x[kQuantPairs][8];
+  Raw8<kF32> x[kQuantPairs];
 #pragma unroll
-  for (int u = 0; u < kQuantPairs; ++u) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[u][j] = 0.f;
-    if (k0 + 256 * u < p.k) quant_load8(p, row * p.in_stride + k0 + 256 * u, x[u]);   // K is a multiple of 16
-  }
+  for (int u = 0; u < kQuantPairs; ++u)       // K is a multiple of 16; a lane behind it reads its first values again
+    x[u].load(p.in, row * p.in_stride + (k0 + 256 * u < p.k ? k0 + 256 * u : 0), p.in_vec);
 #pragma unroll
   for (int u = 0; u < kQuantPairs; ++u) {
     const int k = k0 + 256 * u;
     float amax = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[u][j]));
+    if (k >= p.k) amax = 0.f;
     for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     float scale = __fdiv_rn(fmaxf(amax, 1e-10f), 448.0f);
     if (p.use_ue8m0) scale = pow2_at_least(scale);
     if (k >= p.k) continue;
+    const float rcp = __frcp_rn(scale);
     uint2 codes;
-    codes.x = quant_e4m3x4(x[u][0], x[u][1], x[u][2], x[u][3], scale);
-    codes.y = quant_e4m3x4(x[u][4], x[u][5], x[u][6], x[u][7], scale);
+    codes.x = quant_e4m3x4(x[u][0], x[u][1], x[u][2], x[u][3], scale, rcp);
+    codes.y = quant_e4m3x4(x[u][4], x[u][5], x[u][6], x[u][7], scale, rcp);
     *reinterpret_cast<uint2*>(p.q + row * p.k + k) = codes;
     if ((lane & 15) == 0) p.scale[(k >> 7) * p.ld + row] = scale;
   }
@@ -471,11 +827,12 @@ __global__ void __launch_bounds__(256) fp8_quantise_blocks_kernel(const void* in
   for (int i = 0; i < 8; ++i) amax = fmaxf(amax, s_max[i]);
   float sc = __fdiv_rn(fmaxf(amax, 1e-10f), 448.0f);
   if (use_ue8m0) sc = pow2_at_least(sc);
+  const float rcp = __frcp_rn(sc);
 #pragma unroll
   for (int i = 0; i < 16; ++i)
     if (r0 + i < n && c0 < k)                            // K is a multiple of 16: four codes are in or out together
       *reinterpret_cast<uint32_t*>(q + static_cast<int64_t>(r0 + i) * k + c0) =
-          quant_e4m3x4(x[i][0], x[i][1], x[i][2], x[i][3], sc);
+          quant_e4m3x4(x[i][0], x[i][1], x[i][2], x[i][3], sc, rcp);
   if (threadIdx.x == 0) scale[static_cast<int64_t>(blockIdx.y) * groups + blockIdx.x] = sc;
 }
 
@@ -485,31 +842,33 @@ static int gemm_rc(cudaError_t e) {
   return B200DSA_ECUDA;
 }
 
-// Tokens of a tile and CTAs of a cluster for a product of m x n over `blocks` blocks of 128.
+// Kernel, tokens of a tile and CTAs of a cluster for a product of m x n over `blocks` blocks of 128: the least
+// estimated time.  Measured clocks of a block: narrow 830 (16 tokens) .. 1000 (128), bound by the weights from HBM or
+// by the accumulating warps; wide 930.  A wave costs 600 more, a split its barriers and the exchange of the partial sums.
+// nt = 0: the kernel for many tokens.
+constexpr double gemm_cost(int64_t tiles, int splits, int blocks, int sms, double block_clocks, double exchange) {
+  return static_cast<double>((tiles * splits + sms - 1) / sms) * ((blocks + splits - 1) / splits * block_clocks + 600.0) +
+         (splits > 1 ? 1000.0 + exchange : 0.0);
+}
 static void gemm_plan(int m, int n, int blocks, int sms, int* nt_out, int* splits_out) {
-  const int n_tiles = (n + 127) / 128;
-  int best_nt = 16, best_s = 1;
   double best = 0;
-  for (int nt = 16; nt <= 256; nt *= 2) {
-    if (nt < 256 && nt < m && nt < 128) continue;        // one token tile as long as 128 tokens hold the batch
-    if (nt > 16 && nt / 2 >= m) break;
-    const int64_t tiles = static_cast<int64_t>(n_tiles) * ((m + nt - 1) / nt);
+  for (int nt = 16; nt <= 256; nt *= 2) {                // 256 stands for the wide kernel: 128 tokens x 256 columns
+    if (nt < 128 && nt < m) continue;                    // one token tile as long as 128 tokens hold the batch
+    if (nt > 16 && (nt == 256 ? m <= 128 : nt / 2 >= m)) break;
+    const bool wide = nt == 256;
+    const int64_t tiles = wide ? static_cast<int64_t>((n + 255) / 256) * ((m + 127) / 128)
+                               : static_cast<int64_t>((n + 127) / 128) * ((m + nt - 1) / nt);
     for (int s = 1; s <= 8; s *= 2) {
-      if (s > 1 && (nt > 128 || tiles * s > sms || blocks < 2 * s)) break;
-      // clocks of a block: the MMAs (2 NT) or the operands from L2 (about 48 bytes a clock and SM); a split costs a
-      // cluster barrier pair and the exchange of the partial sums
-      const double block = nt * 2.0 > (128 + nt) * 128 / 48.0 ? nt * 2.0 : (128 + nt) * 128 / 48.0;
-      const int64_t waves = (tiles * s + sms - 1) / sms;
-      const double cost = waves * ((blocks + s - 1) / s * block + 600.0) + (s > 1 ? 1000.0 + 12.0 * nt : 0.0);
+      if (s > 1 && (tiles * s > sms || blocks < 2 * s)) break;
+      const double cost = wide ? gemm_cost(tiles, s, blocks, sms, 930.0, 3000.0)
+                               : gemm_cost(tiles, s, blocks, sms, 800.0 + 1.5 * nt, 12.0 * nt);
       if (best == 0 || cost < best) {
         best = cost;
-        best_nt = nt;
-        best_s = s;
+        *nt_out = wide ? 0 : nt;
+        *splits_out = s;
       }
     }
   }
-  *nt_out = best_nt;
-  *splits_out = best_s;
 }
 
 }  // namespace b200dsa
@@ -530,7 +889,6 @@ extern "C" int b200dsa_fp8_quantise_rows(const void* x, int32_t in_f32, int64_t 
   }
   QuantRowsParams p{};
   p.in = x;
-  p.in_f32 = in_f32 != 0;
   p.in_vec = !(reinterpret_cast<uintptr_t>(x) & 15) && !((in_stride * static_cast<int64_t>(elem)) & 15);
   p.in_stride = in_stride;
   p.m = m;
@@ -540,7 +898,8 @@ extern "C" int b200dsa_fp8_quantise_rows(const void* x, int32_t in_f32, int64_t 
   p.ld = scale_ld;
   p.use_ue8m0 = use_ue8m0 != 0;
   const dim3 grid(static_cast<unsigned>((m + 7) / 8), (k + kQuantPairs * 256 - 1) / (kQuantPairs * 256));
-  cudaError_t e = launch_chained(fp8_quantise_rows_kernel, grid, dim3(256), 0, static_cast<cudaStream_t>(stream), p);
+  cudaError_t e = launch_chained(in_f32 ? fp8_quantise_rows_kernel<true> : fp8_quantise_rows_kernel<false>, grid, dim3(256),
+                                 0, static_cast<cudaStream_t>(stream), p);
   return gemm_rc(e == cudaSuccess ? cudaGetLastError() : e);
 }
 
@@ -597,7 +956,7 @@ static int block_matmul(const void* a_e4m3, int64_t a_stride, const float* a_sca
   cuuint32_t es[2] = {1, 1};
   cuuint64_t dw[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(n)}, sw[1] = {static_cast<cuuint64_t>(w_stride)};
   cuuint64_t da[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(m)}, sa[1] = {static_cast<cuuint64_t>(a_stride)};
-  cuuint32_t bw[2] = {128, 128}, ba[2] = {128, static_cast<cuuint32_t>(nt)};
+  cuuint32_t bw[2] = {128, nt ? 128u : 256u}, ba[2] = {128, nt ? static_cast<cuuint32_t>(nt) : 128u};
   // out-of-range rows and the tail of the last block arrive as zeros
   if (enc(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(w_e4m3), dw, sw, bw, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS ||
@@ -616,12 +975,13 @@ static int block_matmul(const void* a_e4m3, int64_t a_stride, const float* a_sca
   p.out = out;
   p.ldo = out_stride;
   p.out_f32 = out_f32 != 0;
+  p.out_vec = !(reinterpret_cast<uintptr_t>(out) & 15) && !((out_stride * (out_f32 ? 4 : 2)) & 15);
   p.out_pair = !(reinterpret_cast<uintptr_t>(out) & 3) && !(out_stride & 1);
   p.m = m;
   p.n = n;
   p.blocks = blocks;
-  p.m_tiles = (m + nt - 1) / nt;
-  p.n_tiles = (n + 127) / 128;
+  p.m_tiles = nt ? (m + nt - 1) / nt : (m + 127) / 128;
+  p.n_tiles = nt ? (n + 127) / 128 : (n + 255) / 256;
   p.splits = splits;
   p.status = status;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -630,7 +990,7 @@ static int block_matmul(const void* a_e4m3, int64_t a_stride, const float* a_sca
     case 32: return gemm_rc(gemm_launch<32>(mw, ma, p, dev, dependent, st));
     case 64: return gemm_rc(gemm_launch<64>(mw, ma, p, dev, dependent, st));
     case 128: return gemm_rc(gemm_launch<128>(mw, ma, p, dev, dependent, st));
-    default: return gemm_rc(gemm_launch<256>(mw, ma, p, dev, dependent, st));
+    default: return gemm_rc(splits > 1 ? wide_launch<true>(mw, ma, p, dev, dependent, st) : wide_launch<false>(mw, ma, p, dev, dependent, st));
   }
 }
 

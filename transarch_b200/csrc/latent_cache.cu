@@ -119,9 +119,10 @@ __global__ void __launch_bounds__(32 * kRowWarps) latent_write_kernel(const Late
     float scale = __fdiv_rn(max_nan(amax, 1e-4f), 448.0f);
     if (p.use_ue8m0) scale = pow2_at_least(scale);
     if (!(amax < INFINITY)) scale = __int_as_float(0x7fffffff);   // not finite: the whole group reads as NaN
+    const float rcp = __frcp_rn(scale);
     uint2 codes;
-    codes.x = quant_e4m3x4(x[h][0], x[h][1], x[h][2], x[h][3], scale);
-    codes.y = quant_e4m3x4(x[h][4], x[h][5], x[h][6], x[h][7], scale);
+    codes.x = quant_e4m3x4(x[h][0], x[h][1], x[h][2], x[h][3], scale, rcp);
+    codes.y = quant_e4m3x4(x[h][4], x[h][5], x[h][6], x[h][7], scale, rcp);
     *reinterpret_cast<uint2*>(row + 256 * h + 8 * lane) = codes;
     if ((lane & 15) == 0) *reinterpret_cast<float*>(row + 512 + 4 * (2 * h + (lane >> 4))) = scale;
   }
