@@ -587,12 +587,22 @@ extern "C" int b200dsa_sparse_mla_decode_cached_splits(int32_t n_items, int32_t 
   if (n_items < 1 || n_heads < 1 || n_idx < 0) return 1;
   DeviceInfo dev;
   if (current_device_info(&dev) != cudaSuccess) return 1;
+  // The least estimated time, in clocks: waves of CTAs over the SMs, 3500 a tile and 12000 around them (prologue, Q, first
+  // rows, output), and for the merge 6000 and the traffic of the parts (2 KB a row written and read, 2 KB a clock).
   const int64_t ctas = static_cast<int64_t>(n_items) * (n_heads > kMlaHeadsTile ? 2 : 1);
   const int tiles = (n_idx + kMlaTile - 1) / kMlaTile + (tree ? 1 : 0);
-  int64_t splits = dev.sms / ctas;
-  if (splits > tiles / 2) splits = tiles / 2;          // a run of one tile costs as much in prologue and merge as it saves
-  if (splits > kMlcMaxSplits) splits = kMlcMaxSplits;
-  return splits < 1 ? 1 : static_cast<int>(splits);
+  int best = 1;
+  double least = 0;
+  for (int s = 1; s <= kMlcMaxSplits && (s == 1 || s <= tiles); ++s) {
+    const double waves = static_cast<double>((ctas * s + dev.sms - 1) / dev.sms);
+    const double cost = waves * ((tiles + s - 1) / s * 3500.0 + 12000.0) +
+                        (s > 1 ? 6000.0 + 2.0 * s * n_items * n_heads : 0.0);
+    if (s == 1 || cost < least) {
+      least = cost;
+      best = s;
+    }
+  }
+  return best;
 }
 
 extern "C" int b200dsa_sparse_mla_decode_cached(const void* q_bf16, const void* cache, int64_t n_slots, int32_t page_size,
