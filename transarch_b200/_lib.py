@@ -135,7 +135,7 @@ def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 def stream_ptr() -> int:
     """Current stream of the current device (the raw handle: building a Stream object costs 3 us a call)."""
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def check(rc: int, what: str) -> None:

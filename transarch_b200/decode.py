@@ -61,6 +61,8 @@ class SparseDecodeStep:
       k_cache uint8 paged FP8 index-key cache (this rank's pages), block_table int32 [B, pages]
       context_lens int32 [B] (global lengths), kv bf16 [rows, 576] latent cache (this rank's rows),
       kv_row_base int64 [B] row of each request's first local position.
+    latent_page_size > 0 (one GPU): the latent cache is the quantised, paged one; `kv` is then its uint8 pages
+    (page_size * 656 bytes, kernels.latent_quant_and_cache) and `kv_row_base` its block table int32 [B, pages].
     """
 
     def __init__(self, batch: int, max_local_ctx: int, *, page_size: int = 64, topk: int = 2048,
@@ -68,7 +70,7 @@ class SparseDecodeStep:
                  device: Optional[torch.device] = None, shard: Optional[ShardInfo] = None, backend=None,
                  sorted_topk: bool = False, wire: str = "bf16", ctx_dtype: torch.dtype = torch.float32,
                  combine: str = "auto", fused_select: bool = True, keep_logits: bool = True,
-                 result: str = "replicated"):
+                 result: str = "replicated", latent_page_size: int = 0):
         if backend is None:
             from . import kernels as backend  # the CUDA kernels; fails loudly without the library
         self.K = backend
@@ -87,6 +89,11 @@ class SparseDecodeStep:
         self.result = result
         dev = device if device is not None else torch.device("cuda")
         self.dev = dev
+        self.latent_page_size = latent_page_size
+        if latent_page_size:
+            if self.shard.world_size > 1:
+                raise ValueError("the quantised latent cache is not key-sharded: latent_page_size needs a single rank")
+            self.latent_workspace = backend.sparse_mla_cached_workspace(batch, n_heads, topk, dev)
         f32, i32 = torch.float32, torch.int32
         n = self.shard.world_size
         self.max_cols = max_local_ctx
@@ -226,6 +233,10 @@ class SparseDecodeStep:
         q_pos + q_pos_bias are masked (context lengths with a bias of -1 save a subtraction kernel).
         signal=False: do not tell the peers that the partial is ready (combine() then does, as when the
         exchanges are separate kernels)."""
+        if self.latent_page_size:
+            return self.K.sparse_mla_decode_cached(q_lat, kv, self.latent_page_size, indices, self.attn_scale,
+                                                   block_table=kv_row_base, q_pos=q_pos, q_pos_bias=q_pos_bias,
+                                                   ctx=self.ctx, lse=self.lse, workspace=self.latent_workspace)
         count = None
         self._signalled = False
         if self.peer_fused and indices is self.merged:

@@ -12,7 +12,9 @@ two fused kernels: LayerNorm + RoPE on the key rows, RoPE on the (token, head) q
 `forward_quantised` is the serving form of the same producer (MiSAIndexer.forward,
 MISA_preprint/misa_vllm_patch_2stage/misa_vllm_patch/misa_deepseek_v2.py:228-292, where the rope dims
 come FIRST): it returns the FP8 queries with their scales folded into the head weights, and writes the
-new keys, quantised, straight into the paged cache.
+new keys, quantised, straight into the paged cache.  After `quantise_projections()` its query and key projections run in
+8 bits with block scales (kernels.fp8_block_linear: half the weight bytes, no library GEMM); the head weights' narrow
+projection stays as it is.
 """
 from __future__ import annotations
 
@@ -40,6 +42,29 @@ class LightningIndexer(nn.Module):
         self.wk = nn.Linear(hidden_size, head_dim, bias=False, dtype=dtype)
         self.k_norm = nn.LayerNorm(head_dim, dtype=dtype)
         self.w_proj = nn.Linear(hidden_size, n_heads, bias=False, dtype=dtype)
+        self._fp8 = {}            # quantise_projections(): name -> (codes, scales, the weight, its version and dtype)
+        self._fp8_fmt: Optional[str] = None
+
+    @torch.no_grad()
+    def quantise_projections(self, scale_fmt: Optional[str] = None) -> None:
+        """Keep 8-bit copies of wq and wk (one scale for a block of 128 x 128) for forward_quantised; the activations are
+        quantised on the way, with `scale_fmt` scales for 128 values of a row.  The parameters stay as they are; once
+        they change, or move, forward_quantised refuses to run until this has been called again."""
+        held = {}
+        for name, lin in (("wq", self.wq), ("wk", self.wk)):
+            codes, scale = K.fp8_quantise_blocks(lin.weight.detach(), scale_fmt=scale_fmt)
+            held[name] = (codes, scale, lin.weight, lin.weight._version, lin.weight.dtype)
+        self._fp8, self._fp8_fmt = held, scale_fmt
+
+    def _project(self, name: str, x: torch.Tensor) -> torch.Tensor:
+        lin = getattr(self, name)
+        if name not in self._fp8:
+            return lin(x)
+        codes, scale, weight, version, dtype = self._fp8[name]
+        if lin.weight is not weight or weight._version != version or weight.dtype != dtype or \
+                weight.device != codes.device:
+            raise B200DSAError(f"{name} has changed since quantise_projections(): call it again")
+        return K.fp8_block_linear(x, codes, scale, scale_fmt=self._fp8_fmt, out_dtype=x.dtype)
 
     @torch.no_grad()
     def forward(self, hidden_states, q_input, cos, sin):
@@ -63,8 +88,8 @@ class LightningIndexer(nn.Module):
         w_proj(h) * q_scale * softmax_scale * H^-0.5) and inserts the T new keys into `cache`."""
         T = hidden_states.shape[0]
         H, d = self.n_heads, self.head_dim
-        q = self.wq(q_input).view(T, H, d).contiguous()
-        k = self.wk(hidden_states).view(T, d).contiguous()
+        q = self._project("wq", q_input).view(T, H, d).contiguous()
+        k = self._project("wk", hidden_states).view(T, d).contiguous()
         w = self.w_proj(hidden_states)
         q_fp8, weights = K.indexer_q_rope(q, cos, sin, rope_first=rope_first, want_rows=False, w=w,
                                           fold=self.softmax_scale * H ** -0.5, ue8m0=scale_fmt is not None)

@@ -981,13 +981,13 @@ LATENT_ROW = 656                     # bytes of a cached token: 512 codes, 4 fp3
 
 def _device_index(first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
     """CUDA device index of a call's tensors; raises unless all of them live there."""
-    dev = first.device
-    if dev.type != "cuda":
+    index = first.get_device()
+    if index < 0:
         raise _lib.B200DSAError("b200dsa kernels need CUDA tensors; there is no CPU path")
     for t in others:
-        if t is not None and t.device != dev:
-            raise _lib.B200DSAError(f"all tensors of a call must be on one device ({dev} and {t.device} given)")
-    return dev.index
+        if t is not None and t.get_device() != index:
+            raise _lib.B200DSAError(f"all tensors of a call must be on one device ({first.device} and {t.device} given)")
+    return index
 
 
 def _rows_stride(x: torch.Tensor, width: int) -> int:
@@ -997,8 +997,7 @@ def _rows_stride(x: torch.Tensor, width: int) -> int:
 
 def _latent_slots(cache: torch.Tensor, page_size: int) -> int:
     n = cache.numel()
-    if cache.dtype != torch.uint8 or not cache.is_contiguous() or page_size < 1 or n == 0 or \
-            n % (page_size * LATENT_ROW):
+    if cache.dtype != torch.uint8 or page_size < 1 or n == 0 or n % (page_size * LATENT_ROW) or not cache.is_contiguous():
         raise _lib.B200DSAError("cache must be contiguous uint8 with page_size*656 bytes per page")
     return n // LATENT_ROW
 
@@ -1011,11 +1010,17 @@ def _scale_fmt(scale_fmt: Optional[str]) -> int:
 
 def _pages(block_table: torch.Tensor) -> Tuple[int, int, int]:
     """(requests, pages of a request, row stride) of a block table."""
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[1] < 1 or \
-            (block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        raise _lib.B200DSAError("block_table must be int32 [n_requests, pages] with unit column stride")
-    R, cols = block_table.shape
-    return R, cols, block_table.stride(0) if R > 1 else cols
+    if block_table.dtype == torch.int32 and block_table.dim() == 2:
+        R, cols = block_table.shape
+        row, col = block_table.stride()
+        if cols == 1 or (cols > 1 and col == 1):
+            return R, cols, row if R > 1 else cols
+    raise _lib.B200DSAError("block_table must be int32 [n_requests, pages] with unit column stride")
+
+
+def _fp32(t: torch.Tensor) -> torch.Tensor:
+    """t as contiguous fp32 (itself where it is that already)."""
+    return t if t.dtype == torch.float32 and t.is_contiguous() else t.to(torch.float32).contiguous()
 
 
 def latent_quant_and_cache(kv: torch.Tensor, cache: torch.Tensor, slot_mapping: torch.Tensor, page_size: int, *,
@@ -1027,11 +1032,15 @@ def latent_quant_and_cache(kv: torch.Tensor, cache: torch.Tensor, slot_mapping: 
     RMSNorm), cos / sin [n, 64] (None: no rotation).  A negative slot is a padding token; slots must be distinct."""
     fmt = _scale_fmt(scale_fmt)
     f32 = kv.dtype == torch.float32
-    if not (f32 or kv.dtype == torch.bfloat16) or kv.dim() != 2 or kv.shape[1] != 576 or kv.stride(1) != 1:
+    if not (f32 or kv.dtype == torch.bfloat16) or kv.dim() != 2:
         raise _lib.B200DSAError("kv must be bf16 or fp32 [n, 576] with unit column stride")
-    n = kv.shape[0]
-    stride = _rows_stride(kv, 576)
-    if stride < 576:
+    n, width = kv.shape
+    stride, col = kv.stride()
+    if width != 576 or col != 1:
+        raise _lib.B200DSAError("kv must be bf16 or fp32 [n, 576] with unit column stride")
+    if n <= 1:
+        stride = 576                      # a single row may carry any stride
+    elif stride < 576:
         raise _lib.B200DSAError("the rows of kv must not overlap")
     if slot_mapping.dtype != torch.int64 or not slot_mapping.is_contiguous() or slot_mapping.numel() != n:
         raise _lib.B200DSAError("slot_mapping must be contiguous int64 with one entry per row of kv")
@@ -1050,9 +1059,12 @@ def latent_quant_and_cache(kv: torch.Tensor, cache: torch.Tensor, slot_mapping: 
         with torch.cuda.device(index):
             return latent_quant_and_cache(kv, cache, slot_mapping, page_size, norm_weight=norm_weight, eps=eps, cos=cos,
                                           sin=sin, interleaved=interleaved, scale_fmt=scale_fmt)
-    c, s_ = _f32c(cos), _f32c(sin)
+    c = s_ = None
+    if cos is not None:
+        cos, sin = _fp32(cos), _fp32(sin)
+        c, s_ = cos.data_ptr(), sin.data_ptr()
     check(_lib.load().b200dsa_latent_quant_and_cache(
-        kv.data_ptr(), f32, stride, n, gain, gain_f32, eps, ptr(c), ptr(s_), interleaved, slot_mapping.data_ptr(),
+        kv.data_ptr(), f32, stride, n, gain, gain_f32, eps, c, s_, interleaved, slot_mapping.data_ptr(),
         cache.data_ptr(), n_slots, fmt, _lib.status_ptr(index), stream_ptr()), "b200dsa_latent_quant_and_cache")
 
 
@@ -1147,15 +1159,18 @@ def sparse_mla_decode_cached(q: torch.Tensor, cache: torch.Tensor, page_size: in
     item's request (row_request int32 [n]; item i is request i without it), -1 = none, block_table int32 [R, pages].
     tree_mask int64 [n] + tree_base int32 [R]: the item also attends the drafted tokens at positions tree_base + bit.
     workspace: what sparse_mla_cached_workspace returned (allocated for the call when not given)."""
-    if q.dtype != torch.bfloat16 or not q.is_contiguous() or q.dim() != 3 or q.shape[2] != 576 or \
-            not 1 <= q.shape[1] <= 128:
+    n, H, width = q.shape if q.dim() == 3 else (0, 0, 0)
+    if q.dtype != torch.bfloat16 or width != 576 or not 1 <= H <= 128 or not q.is_contiguous():
         raise _lib.B200DSAError("q must be contiguous bf16 [n_items, n_heads <= 128, 576]")
-    n, H, _ = q.shape
     n_slots = _latent_slots(cache, page_size)
-    if indices.dtype != torch.int32 or indices.dim() != 2 or indices.shape[0] != n or \
-            (indices.shape[1] > 1 and indices.stride(1) != 1):
+    items, n_idx = indices.shape if indices.dim() == 2 else (-1, 0)
+    if indices.dtype != torch.int32 or items != n:
         raise _lib.B200DSAError("indices must be int32 [n_items, n_idx] with unit column stride")
-    n_idx = indices.shape[1]
+    idx_stride, col = indices.stride()
+    if n_idx > 1 and col != 1:
+        raise _lib.B200DSAError("indices must be int32 [n_items, n_idx] with unit column stride")
+    if n == 1:
+        idx_stride = n_idx
     R, cols, stride = _pages(block_table)
     for t_, nm in ((row_request, "row_request"), (q_pos, "q_pos"), (n_idx_item, "n_idx_item")):
         if t_ is not None and (t_.dtype != torch.int32 or not t_.is_contiguous() or t_.numel() != n):
@@ -1198,7 +1213,7 @@ def sparse_mla_decode_cached(q: torch.Tensor, cache: torch.Tensor, page_size: in
         raise _lib.B200DSAError("the workspace is smaller than splits * n_items * n_heads * 513 floats")
     check(lib.b200dsa_sparse_mla_decode_cached(
         q.data_ptr(), cache.data_ptr(), n_slots, page_size, block_table.data_ptr(), stride, cols, R, ptr(row_request),
-        indices.data_ptr(), indices.stride(0) if n > 1 else n_idx, n_idx, ptr(n_idx_item), ptr(q_pos), q_pos_bias,
+        indices.data_ptr(), idx_stride, n_idx, ptr(n_idx_item), ptr(q_pos), q_pos_bias,
         ptr(tree_mask), ptr(tree_base), n, H, sm_scale, ctx.data_ptr(), ctx.dtype == torch.bfloat16, lse.data_ptr(),
         splits, ptr(ws), ws.numel() * 4 if ws is not None else 0, _lib.status_ptr(index), stream_ptr()),
         "b200dsa_sparse_mla_decode_cached")
@@ -1208,12 +1223,12 @@ def sparse_mla_decode_cached(q: torch.Tensor, cache: torch.Tensor, page_size: in
 def _matrix(x: torch.Tensor, name: str) -> Tuple[int, int, int, bool]:
     """(rows, columns, row stride, is fp32) of a matrix to be quantised."""
     f32 = x.dtype == torch.float32
-    if not (f32 or x.dtype == torch.bfloat16) or x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
+    if not (f32 or x.dtype == torch.bfloat16) or x.dim() != 2 or x.stride(1) != 1:
         raise _lib.B200DSAError(f"{name} must be a 2-D bf16 or fp32 tensor with unit column stride")
     M, K = x.shape
     if K < 16 or K % 16:
         raise _lib.B200DSAError(f"the columns of {name} must be a multiple of 16")
-    stride = _rows_stride(x, K)
+    stride = x.stride(0) if M > 1 else K
     if stride < K:
         raise _lib.B200DSAError(f"the rows of {name} must not overlap")
     return M, K, stride, f32
@@ -1251,16 +1266,24 @@ def fp8_quantise_blocks(w: torch.Tensor, *, scale_fmt: Optional[str] = None) -> 
     return q, scale
 
 
-def _fp8_weight(w: torch.Tensor, w_scale: torch.Tensor, K: int) -> int:
-    """Rows of an 8-bit weight [N, K] after its checks."""
-    if w.dtype != torch.float8_e4m3fn or w.dim() != 2 or w.stride(1) != 1:
-        raise _lib.B200DSAError("w must be float8_e4m3fn with two dims and unit column stride")
-    if w.shape[1] != K or K < 16 or K % 16:
-        raise _lib.B200DSAError("both operands must have the same number of columns, a multiple of 16")
-    N = w.shape[0]
+def _fp8_codes(t: torch.Tensor, name: str) -> Tuple[int, int, int]:
+    """(rows, columns, row stride) of an e4m3 operand after its checks."""
+    if t.dtype == torch.float8_e4m3fn and t.dim() == 2:
+        rows, K = t.shape
+        stride, col = t.stride()
+        if col == 1 and K >= 16 and K % 16 == 0:
+            return rows, K, stride if rows > 1 else K
+    raise _lib.B200DSAError(f"{name} must be float8_e4m3fn with two dims, unit column stride and a multiple of 16 columns")
+
+
+def _fp8_weight(w: torch.Tensor, w_scale: torch.Tensor, K: int) -> Tuple[int, int]:
+    """(rows, row stride) of an 8-bit weight [N, K] after its checks."""
+    N, k, stride = _fp8_codes(w, "w")
+    if k != K:
+        raise _lib.B200DSAError("both operands must have the same number of columns")
     if w_scale.dtype != torch.float32 or w_scale.shape != ((N + 127) // 128, (K + 127) // 128):
         raise _lib.B200DSAError("w_scale must be fp32 [ceil(N/128), ceil(K/128)]")
-    return N
+    return N, stride
 
 
 def _fp8_result(out: Optional[torch.Tensor], out_dtype: torch.dtype, M: int, N: int) -> bool:
@@ -1278,10 +1301,8 @@ def fp8_block_matmul(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_
                      out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y [M, N] = (a * a_scale) @ (w * w_scale)^T for e4m3 codes a [M, K], w [N, K] with scales fp32 [M, ceil(K/128)]
     (any strides) and [ceil(N/128), ceil(K/128)]; fp32 sums, bf16 or fp32 result; see b200dsa_fp8_block_matmul."""
-    if a.dtype != torch.float8_e4m3fn or a.dim() != 2 or a.stride(1) != 1:
-        raise _lib.B200DSAError("a must be float8_e4m3fn with two dims and unit column stride")
-    M, K = a.shape
-    N = _fp8_weight(w, w_scale, K)
+    M, K, a_stride = _fp8_codes(a, "a")
+    N, w_stride = _fp8_weight(w, w_scale, K)
     if a_scale.dtype != torch.float32 or a_scale.shape != (M, (K + 127) // 128):
         raise _lib.B200DSAError("a_scale must be fp32 [M, ceil(K/128)]")
     f32 = _fp8_result(out, out_dtype, M, N)
@@ -1294,9 +1315,8 @@ def fp8_block_matmul(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_
     sa_m, sa_g = a_scale.stride()
     sw_r, sw_g = w_scale.stride()
     check(_lib.load().b200dsa_fp8_block_matmul(
-        a.data_ptr(), _rows_stride(a, K), a_scale.data_ptr(), sa_m, sa_g, w.data_ptr(), _rows_stride(w, K),
-        w_scale.data_ptr(), sw_r, sw_g, M, N, K, out.data_ptr(), f32, _rows_stride(out, N), _lib.status_ptr(index),
-        stream_ptr()), "b200dsa_fp8_block_matmul")
+        a.data_ptr(), a_stride, a_scale.data_ptr(), sa_m, sa_g, w.data_ptr(), w_stride, w_scale.data_ptr(), sw_r, sw_g, M,
+        N, K, out.data_ptr(), f32, _rows_stride(out, N), _lib.status_ptr(index), stream_ptr()), "b200dsa_fp8_block_matmul")
     return out
 
 
@@ -1306,7 +1326,7 @@ def fp8_block_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *,
     fp8_block_matmul(*fp8_quantise_rows(x, scale_fmt=...), w, w_scale) in one call; see b200dsa_fp8_block_linear."""
     fmt = _scale_fmt(scale_fmt)
     M, K, stride, x_f32 = _matrix(x, "x")
-    N = _fp8_weight(w, w_scale, K)
+    N, w_stride = _fp8_weight(w, w_scale, K)
     f32 = _fp8_result(out, out_dtype, M, N)
     index = _device_index(x, w, w_scale, out)
     if index != torch.cuda.current_device():
@@ -1317,7 +1337,7 @@ def fp8_block_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *,
     ws = torch.empty(M * (K + 4 * ((K + 127) // 128)), dtype=torch.uint8, device=x.device)   # codes, then scales
     sw_r, sw_g = w_scale.stride()
     check(_lib.load().b200dsa_fp8_block_linear(
-        x.data_ptr(), x_f32, stride, fmt, w.data_ptr(), _rows_stride(w, K), w_scale.data_ptr(), sw_r, sw_g, M, N, K,
+        x.data_ptr(), x_f32, stride, fmt, w.data_ptr(), w_stride, w_scale.data_ptr(), sw_r, sw_g, M, N, K,
         out.data_ptr(), f32, _rows_stride(out, N), ws.data_ptr(), ws.numel(), _lib.status_ptr(index), stream_ptr()),
         "b200dsa_fp8_block_linear")
     return out
