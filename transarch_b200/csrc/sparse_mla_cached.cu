@@ -18,7 +18,9 @@
 // Work split: CTA = (item, 64-head half, split).  Small batches cut an item's tiles into `splits` runs whose partial
 // contexts (normalised, fp32) and log-sum-exps are merged by mla_merge_kernel; large ones have splits = 1 and no merge.
 //
-// Roles (416 threads): warps 0-7 rows, warps 8-11 softmax, warp 12 MMAs.  All waits are bounded.
+// Roles (448 threads): warps 0-7 rows, warps 8-11 softmax, warp 12 MMAs, warp 13 keys: it turns positions into slots, up
+// to four tiles ahead of the rows, and has their bytes brought into L2 meanwhile.  (The row warps did that themselves at
+// first: 16 of 79 us at 64 x 128 x 2048.)  All waits are bounded.
 #include "latent_cache.cuh"
 #include "sparse_mla.cuh"
 
@@ -26,9 +28,10 @@ namespace b200dsa {
 
 void set_last_error(const char* msg);
 
-constexpr int kMlcThreads = 416;
+constexpr int kMlcThreads = 448;
 constexpr int kMlcRowWarps = 8;
 constexpr int kMlcMaxSplits = 32;
+constexpr int kMlcKeyTiles = 4;      // tiles whose slots are held in shared memory
 
 struct MlaCachedParams {
   const __nv_bfloat16* q;        // [n_items, n_heads, 576]
@@ -63,6 +66,7 @@ sparse_mla_cached_kernel(const MlaCachedParams p) {
   __shared__ uint32_t s_tmem_base;
   __shared__ int s_abort;
   __shared__ uint32_t s_mask[kMlaStages][2];  // validity bit per key of the stage
+  __shared__ int s_slot[kMlcKeyTiles][kMlaTile];
   __shared__ float s_inv[kMlaHeadsTile];      // 1 / sum of the probabilities of a head row, 0 without a key
 
   const int split = blockIdx.x % p.splits;
@@ -81,6 +85,8 @@ sparse_mla_cached_kernel(const MlaCachedParams p) {
   uint64_t* pv_done = bars + 6;                  // [1] value MMA retired (P buffer free, O stable)
   uint64_t* kv_full = bars + 7;                  // [stages] eight row warps
   uint64_t* kv_empty = bars + 7 + kMlaStages;    // [stages] value MMA retired
+  uint64_t* key_full = bars + 8 + 2 * kMlaStages;  // [kMlcKeyTiles] slots of a tile written
+  uint64_t* key_empty = key_full + kMlcKeyTiles;   // [kMlcKeyTiles] eight row warps have read them
   uint64_t* q_land = bars + 7 + 2 * kMlaStages;  // [1] 256 row-warp threads: their copies of Q have landed
 
   const int tid = threadIdx.x;
@@ -108,6 +114,10 @@ sparse_mla_cached_kernel(const MlaCachedParams p) {
     mbar_init(p_full, 128);
     mbar_init(pv_done, 1);
     mbar_init(q_land, 32 * kMlcRowWarps);
+    for (int s = 0; s < kMlcKeyTiles; ++s) {
+      mbar_init(&key_full[s], 1);
+      mbar_init(&key_empty[s], kMlcRowWarps);
+    }
     mbar_fence_init();
   }
   if (warp == 12) {
@@ -136,48 +146,7 @@ sparse_mla_cached_kernel(const MlaCachedParams p) {
       }
       cp_async_mbar_arrive(q_land);
     }
-    const int32_t* idx_row = p.indices + static_cast<int64_t>(item) * p.idx_stride;
-    int req = p.row_request ? __ldg(p.row_request + item) : item;
-    bool known = req >= 0 && req < p.n_requests;
-    if (!known) {
-      if (tid == 0) atomicMax(p.status, kDevBadIndex);
-      req = 0;
-    }
-    const int32_t* table = p.table + static_cast<int64_t>(req) * p.table_stride;
-    const unsigned long long mask = p.tree_mask ? static_cast<unsigned long long>(__ldg(p.tree_mask + item)) : 0ull;
-    const int base = p.tree_mask ? __ldg(p.tree_base + req) : 0x7fffffff;
-    int64_t last = static_cast<int64_t>(base) - 1;    // the last position that may be attended by selection
-    if (p.q_pos) last = min(last, static_cast<int64_t>(__ldg(p.q_pos + item)) + p.q_pos_bias);
     const int r0 = warp * 8;
-    // The way of a row, one step a tile: position (five tiles ahead), page (four), slot and row to L2 (three), row to
-    // registers (one), so that no step waits for the load of the one before it.
-    auto position = [&](int t) -> int {               // of this lane's row of tile t (lanes 0..7), -1 = none
-      if (lane >= 8 || t >= n_tiles || !known) return -1;
-      const int tt = tile0 + t;
-      if (tt < sel_tiles) {
-        const int j = tt * kMlaTile + r0 + lane;
-        return j < n_idx ? __ldg(idx_row + j) : -1;
-      }
-      const int64_t v = static_cast<int64_t>(base) + r0 + lane;
-      return ((mask >> (r0 + lane)) & 1) && base >= 0 && v <= 0x7fffffff ? static_cast<int>(v) : -1;
-    };
-    struct Key {
-      int page, off;       // page -1: outside the table; off -1: no key
-    };
-    auto page_of = [&](int pos, int t) -> Key {
-      if (pos < 0 || (pos > last && tile0 + t < sel_tiles)) return Key{-1, -1};
-      const int col = pos / p.page_size;
-      return Key{col < p.table_cols ? __ldg(table + col) : -1, pos - col * p.page_size};
-    };
-    auto slot_of = [&](Key k) -> int {                // -1 = none; a page that does not exist is reported
-      if (k.off < 0) return -1;
-      const int64_t slot = static_cast<int64_t>(k.page) * p.page_size + k.off;
-      if (k.page < 0 || slot >= p.n_slots) {
-        atomicMax(p.status, kDevBadIndex);
-        return -1;
-      }
-      return static_cast<int>(slot);
-    };
     // A row's registers: lane l holds codes 16l..16l+15 and their scale, and of two rows (lane / 8 + 4 j) the 16-byte
     // chunk lane % 8 of the position dims.  A missing key reads row 0 and is made zero when it is stored.
     uint4 code[8];
@@ -193,29 +162,23 @@ sparse_mla_cached_kernel(const MlaCachedParams p) {
       const uint8_t* src = row_ptr(__shfl_sync(0xffffffffu, slot, (lane >> 3) + 4 * j));
       pe[j] = __ldg(reinterpret_cast<const uint4*>(src + 528) + (lane & 7));
     };
-    auto prefetch = [&](int slot) {                   // 656 bytes touch at most seven lines of 128
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int s = __shfl_sync(0xffffffffu, slot, (lane >> 3) + 4 * j);
-        if (s >= 0 && (lane & 7) < 7)
-          asm volatile("prefetch.global.L2 [%0];" ::"l"(row_ptr(s) + min((lane & 7) * 128, kLatentRowBytes - 1)));
-      }
+    // this lane's slot of tile t (lanes 0..7: the warp's rows), -1 = none; false when the wait gave up
+    auto key_slot = [&](int t, int& slot) -> bool {
+      slot = -1;
+      if (t >= n_tiles) return true;
+      const int ring = t % kMlcKeyTiles;
+      const bool ok = __all_sync(0xffffffffu, mbar_wait(&key_full[ring], (t / kMlcKeyTiles) & 1, abort_flag));
+      if (lane < 8) slot = s_slot[ring][r0 + lane];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&key_empty[ring]);
+      return ok;
     };
-    int pos5 = position(4);
-    Key key4 = page_of(position(3), 3);
-    int slot, s1, s2, s3;
-    {
-      const Key k0 = page_of(position(0), 0), k1 = page_of(position(1), 1), k2 = page_of(position(2), 2);
-      slot = slot_of(k0);
-      s1 = slot_of(k1);
-      s2 = slot_of(k2);
-    }
+    int slot, next;
+    bool ok = key_slot(0, slot);
 #pragma unroll
     for (int i = 0; i < 8; ++i) load_row(slot, i);
     load_pe(slot, 0);
     load_pe(slot, 1);
-    prefetch(s1);
-    prefetch(s2);
     // Lane l stores 16-byte chunks 2 (l % 4) and 2 (l % 4) + 1 of the 128-byte chunk l / 4 of a row; lanes 4..7 of every
     // eight take them in the other order, so that eight neighbouring lanes write eight different bank groups.
     const bool flip = (lane >> 2) & 1;
@@ -239,19 +202,16 @@ sparse_mla_cached_kernel(const MlaCachedParams p) {
                      "r"(w1.z), "r"(w1.w) : "memory");
       }
     };
-    for (int t = 0; t < n_tiles; ++t) {
+    for (int t = 0; ok && t < n_tiles; ++t) {
       const int s = t % kMlaStages;
       const unsigned vmask = __ballot_sync(0xffffffffu, lane < 8 && slot >= 0);
-      s3 = slot_of(key4);
-      key4 = page_of(pos5, t + 4);
-      pos5 = position(t + 5);
-      prefetch(s3);
-      bool ok = mbar_wait(&kv_empty[s], ((t / kMlaStages) & 1) ^ 1, abort_flag);
+      ok = key_slot(t + 1, next) && mbar_wait(&kv_empty[s], ((t / kMlaStages) & 1) ^ 1, abort_flag);
       // the tail of the ring holds the Q rows until the softmax threads have moved them to TMEM
       if (t < kMlaStages && (t + 1) * kMlaStageBytes > kMlaQStageOff) ok = ok && mbar_wait(q_full, 0, abort_flag);
-      if (!__all_sync(0xffffffffu, ok)) break;
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
       const uint32_t stage_addr = kv_addr + s * kMlaStageBytes;
-      store_rows(stage_addr, vmask, s1);
+      store_rows(stage_addr, vmask, next);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int i = (lane >> 3) + 4 * j;
@@ -259,7 +219,7 @@ sparse_mla_cached_kernel(const MlaCachedParams p) {
         const uint32_t keep = (vmask >> i) & 1 ? 0xffffffffu : 0u;
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(pe[j].x & keep), "r"(pe[j].y & keep),
                      "r"(pe[j].z & keep), "r"(pe[j].w & keep) : "memory");
-        load_pe(s1, j);
+        load_pe(next, j);
       }
       if (lane == 0) reinterpret_cast<volatile uint8_t*>(&s_mask[s][0])[warp] = static_cast<uint8_t>(vmask);
       // The rows were written through the generic proxy; the MMAs read them.  (No thread fence here: it would wait for
@@ -267,9 +227,7 @@ sparse_mla_cached_kernel(const MlaCachedParams p) {
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&kv_full[s]);
-      slot = s1;
-      s1 = s2;
-      s2 = s3;
+      slot = next;
     }
     cp_async_wait_all();     // Q, should everything have been given up early
   } else if (warp < 12) {
@@ -413,6 +371,87 @@ sparse_mla_cached_kernel(const MlaCachedParams p) {
       if (head < p.n_heads) *lse_out = any ? (m_ref + log2f(l)) * 0.6931471805599453f : -INFINITY;
     }
     tc_fence_before();
+  } else if (warp == 13) {
+    // ------------------------------------------------------------------ keys
+    const int32_t* idx_row = p.indices + static_cast<int64_t>(item) * p.idx_stride;
+    int req = p.row_request ? __ldg(p.row_request + item) : item;
+    bool known = req >= 0 && req < p.n_requests;
+    if (!known) {
+      if (lane == 0) atomicMax(p.status, kDevBadIndex);
+      req = 0;
+    }
+    const int32_t* table = p.table + static_cast<int64_t>(req) * p.table_stride;
+    const unsigned long long mask = p.tree_mask ? static_cast<unsigned long long>(__ldg(p.tree_mask + item)) : 0ull;
+    const int base = p.tree_mask ? __ldg(p.tree_base + req) : 0x7fffffff;
+    int64_t last = static_cast<int64_t>(base) - 1;    // the last position that may be attended by selection
+    if (p.q_pos) last = min(last, static_cast<int64_t>(__ldg(p.q_pos + item)) + p.q_pos_bias);
+    struct Key {
+      int page, off;       // page -1: outside the table; off -1: no key
+    };
+    // Positions of keys lane and lane + 32 of tile t, -1 = none.  Positions are fetched two tiles ahead of the pages'
+    // entries, those one ahead of the slots, so that no step waits for the load of the one before it.
+    auto positions = [&](int t, int (&pos)[2]) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int tt = tile0 + t, i = lane + 32 * h;
+        pos[h] = -1;
+        if (t >= n_tiles || !known) continue;
+        if (tt < sel_tiles) {
+          const int j = tt * kMlaTile + i;
+          if (j < n_idx) pos[h] = __ldg(idx_row + j);
+        } else {
+          const int64_t v = static_cast<int64_t>(base) + i;
+          if (((mask >> i) & 1) && base >= 0 && v <= 0x7fffffff) pos[h] = static_cast<int>(v);
+        }
+      }
+    };
+    auto pages = [&](int t, const int (&pos)[2], Key (&key)[2]) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int v = pos[h];
+        key[h].page = key[h].off = -1;
+        if (v < 0 || (v > last && tile0 + t < sel_tiles)) continue;
+        const int col = v / p.page_size;
+        key[h].off = v - col * p.page_size;
+        if (col < p.table_cols) key[h].page = __ldg(table + col);
+      }
+    };
+    auto slot_of = [&](const Key& k) -> int {         // -1 = none; a page that does not exist is reported
+      if (k.off < 0) return -1;
+      const int64_t slot = static_cast<int64_t>(k.page) * p.page_size + k.off;
+      if (k.page < 0 || slot >= p.n_slots) {
+        atomicMax(p.status, kDevBadIndex);
+        return -1;
+      }
+      return static_cast<int>(slot);
+    };
+    int pos[2][2];
+    Key key[2];
+    positions(0, pos[0]);
+    pages(0, pos[0], key);
+    positions(1, pos[1]);
+    positions(2, pos[0]);
+    bool ok = true;
+#pragma unroll 2
+    for (int t = 0; ok && t < n_tiles; ++t) {
+      const int ring = t % kMlcKeyTiles;
+      const int a = slot_of(key[0]), b = slot_of(key[1]);
+      pages(t + 1, pos[(t + 1) & 1], key);
+      positions(t + 3, pos[(t + 1) & 1]);
+      ok = __all_sync(0xffffffffu, mbar_wait(&key_empty[ring], ((t / kMlcKeyTiles) & 1) ^ 1, abort_flag));
+      if (!ok) break;
+      s_slot[ring][lane] = a;
+      s_slot[ring][lane + 32] = b;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&key_full[ring]);
+      // 656 bytes lie in at most seven lines of 128; the first tiles are loaded at once
+      for (int i = 0; t >= 2 && i < 16; ++i) {
+        const int r = 4 * i + (lane >> 3), s = s_slot[ring][r];
+        if (s >= 0 && (lane & 7) < 7)
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(p.cache + static_cast<int64_t>(s) * kLatentRowBytes +
+                                                       min((lane & 7) * 128, kLatentRowBytes - 1)));
+      }
+    }
   } else {
     // ------------------------------------------------------------------ MMA issuer (warp 12)
     // One warp issues everything, in the order S(0), S(1), PV(0), S(2), PV(1), ...: the tensor pipe runs
