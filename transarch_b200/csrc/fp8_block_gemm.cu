@@ -241,20 +241,22 @@ fp8_block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
     }
     __syncwarp();
   } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMA (one thread: nothing but waits and issues)
-    if (lane == 0) {
-      constexpr uint32_t idesc = make_idesc(kFmtE4M3, kFmtE4M3, 128, NT);
-      int it = 0;
-      bool ok = true;
-      for (int w = first; ok && w < n_work; w += stride) {
-        for (int b = b_lo; b < b_hi; ++b, ++it) {
-          const int s = it % S::kStages, buf = it % S::kAccBufs, sl = it % kGemmScaleSlots;
-          // the block's scales are waited for here, so that the accumulating warps have one barrier to look at
-          ok = mbar_wait(&sc_full[sl], (it / kGemmScaleSlots) & 1, abort_flag) &&
-               mbar_wait(&acc_empty[buf], ((it / S::kAccBufs) & 1) ^ 1, abort_flag) &&
-               mbar_wait(&full[s], (it / S::kStages) & 1, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
+    // ------------------------------------------------------------------ MMA
+    // The whole warp waits, one elected lane issues: in a loop of a single thread the descriptors are not in uniform
+    // registers and every MMA takes longer to issue.
+    constexpr uint32_t idesc = make_idesc(kFmtE4M3, kFmtE4M3, 128, NT);
+    int it = 0;
+    bool ok = true;
+    for (int w = first; ok && w < n_work; w += stride) {
+      for (int b = b_lo; b < b_hi; ++b, ++it) {
+        const int s = it % S::kStages, buf = it % S::kAccBufs, sl = it % kGemmScaleSlots;
+        // the block's scales are waited for here, so that the accumulating warps have one barrier to look at
+        ok = __all_sync(0xffffffffu, mbar_wait(&sc_full[sl], (it / kGemmScaleSlots) & 1, abort_flag) &&
+                                         mbar_wait(&acc_empty[buf], ((it / S::kAccBufs) & 1) ^ 1, abort_flag) &&
+                                         mbar_wait(&full[s], (it / S::kStages) & 1, abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
           const uint64_t wd = make_desc_k_sw128(smem_base + s * S::kStageBytes);
           const uint64_t ad = make_desc_k_sw128(smem_base + s * S::kStageBytes + S::kWBytes);
 #pragma unroll
@@ -263,9 +265,9 @@ fp8_block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
           tc_commit(&acc_full[buf]);
           tc_commit(&empty[s]);
         }
+        __syncwarp();
       }
     }
-    __syncwarp();
   } else if (warp == 2) {
     // ------------------------------------------------------------------ scales, four blocks of loads in flight
     constexpr int kPer = NT <= 32 ? 1 : NT / 32;
@@ -552,24 +554,27 @@ fp8_block_gemm_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __g
         while (!mbar_test(&full[j % kWideStages], (j / kWideStages) & 1) && clock64() - t0 < kWaitLimitCycles) {
         }
       }
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1) {
       constexpr uint32_t idesc = make_idesc(kFmtE4M3, kFmtE4M3, 128, 256);
       int it = 0;
       bool ok = true;
       for (int w = first; ok && w < n_work; w += stride) {
         for (int b = b_lo; b < b_hi; ++b, ++it) {
           const int s = it % kWideStages, buf = it & 1;
-          ok = mbar_wait(&acc_empty[buf], ((it >> 1) & 1) ^ 1, abort_flag) &&
-               mbar_wait(&full[s], (it / kWideStages) & 1, abort_flag);
+          ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[buf], ((it >> 1) & 1) ^ 1, abort_flag) &&
+                                           mbar_wait(&full[s], (it / kWideStages) & 1, abort_flag));
           if (!ok) break;
           tc_fence_after();
-          const uint64_t ad = make_desc_k_sw128(smem_base + s * kWideStageBytes);
-          const uint64_t wd = make_desc_k_sw128(smem_base + s * kWideStageBytes + kWideABytes);
+          if (elect_one()) {
+            const uint64_t ad = make_desc_k_sw128(smem_base + s * kWideStageBytes);
+            const uint64_t wd = make_desc_k_sw128(smem_base + s * kWideStageBytes + kWideABytes);
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            mma_f8f6f4_ss(tmem_base + buf * 256, ad + 2 * kk, wd + 2 * kk, idesc, kk != 0);
-          tc_commit(&acc_full[buf]);
-          tc_commit(&empty[s]);
+            for (int kk = 0; kk < 4; ++kk)
+              mma_f8f6f4_ss(tmem_base + buf * 256, ad + 2 * kk, wd + 2 * kk, idesc, kk != 0);
+            tc_commit(&acc_full[buf]);
+            tc_commit(&empty[s]);
+          }
+          __syncwarp();
         }
       }
     }

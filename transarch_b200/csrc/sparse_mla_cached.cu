@@ -454,11 +454,11 @@ sparse_mla_cached_kernel(const MlaCachedParams p) {
     }
   } else {
     // ------------------------------------------------------------------ MMA issuer (warp 12)
-    // One warp issues everything, in the order S(0), S(1), PV(0), S(2), PV(1), ...: the tensor pipe runs
-    // its instructions in issue order, so S(t+1) keeps it busy while the softmax of tile t runs, and the
-    // ring stage that PV(t-1) frees is not needed before S(t+2), a whole tile of tensor work later, which
-    // is the time the gather of tile t+2 has to land.  (Issuing the scores as early as their buffers allow
-    // puts S(t+2) directly behind PV(t-1) and exposes the whole gather latency on every tile.)
+    // One warp issues everything, in the order S(0), S(1), PV(0), S(2), PV(1), ...: the tensor pipe runs its instructions
+    // in issue order, so S(t+1) keeps it busy while the softmax of tile t runs, and the ring stage that PV(t-1) frees is
+    // not needed before S(t+2), a whole tile of tensor work later.  The rows and P were made visible to the MMAs by the
+    // threads that wrote them (fence, then arrival), so no fence is needed here.  The whole warp waits and one elected
+    // lane issues: a loop of a single thread is slower by a fifth (its descriptors are not in uniform registers).
     constexpr uint32_t idesc_s = make_idesc(kFmtBF16, kFmtBF16, kMlaHeadsTile, kMlaTile);
     constexpr uint32_t idesc_pv = make_idesc(kFmtBF16, kFmtBF16, kMlaHeadsTile, 256, 0, 1);
     auto issue_scores = [&](int t) -> bool {
@@ -466,7 +466,6 @@ sparse_mla_cached_kernel(const MlaCachedParams p) {
       const bool w = mbar_wait(&kv_full[s], (t / kMlaStages) & 1, abort_flag) &&
                      mbar_wait(&s_empty[sb], ((t >> 1) & 1) ^ 1, abort_flag);
       if (!__all_sync(0xffffffffu, w)) return false;
-      fence_proxy_async();  // gathered rows were written through the generic proxy
       tc_fence_after();
       if (elect_one()) {
         const uint32_t d = tmem_base + kMlaTmemS + sb * kMlaTile;
@@ -475,25 +474,21 @@ sparse_mla_cached_kernel(const MlaCachedParams p) {
 #pragma unroll
         for (int c = 0; c < kMlaChunks; ++c) {
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {
-            mma_f16_ts(d, tmem_base + kMlaTmemQ + c * 32 + kk * 8, b0 + ((c * kMlaChunkBytesK + kk * 32) >> 4),
-                       idesc_s, (c | kk) != 0);
-          }
+          for (int kk = 0; kk < 4; ++kk)
+            mma_f16_ts(d, tmem_base + kMlaTmemQ + c * 32 + kk * 8, b0 + ((c * kMlaChunkBytesK + kk * 32) >> 4), idesc_s,
+                       (c | kk) != 0);
         }
         tc_commit(&s_full[sb]);
       }
       __syncwarp();
       return true;
     };
-    bool ok = mbar_wait(q_full, 0, abort_flag);
-    ok = __all_sync(0xffffffffu, ok);
+    bool ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0, abort_flag));
     if (ok && n_tiles > 0) ok = issue_scores(0);
     for (int t = 0; ok && t < n_tiles; ++t) {
       if (t + 1 < n_tiles && !issue_scores(t + 1)) break;
       const int s = t % kMlaStages;
-      const bool w = mbar_wait(p_full, t & 1, abort_flag);
-      if (!__all_sync(0xffffffffu, w)) break;
-      fence_proxy_async();
+      if (!__all_sync(0xffffffffu, mbar_wait(p_full, t & 1, abort_flag))) break;
       tc_fence_after();
       if (elect_one()) {
         const uint64_t pa0 = make_desc_k_noswz(p_addr, 128, kMlaTile / 8 * 128);
@@ -501,10 +496,9 @@ sparse_mla_cached_kernel(const MlaCachedParams p) {
 #pragma unroll
         for (int j = 0; j < kMlaTile / 16; ++j) {  // 16 keys per MMA
 #pragma unroll
-          for (int nh = 0; nh < 2; ++nh) {        // value dims [256*nh, 256*nh+256)
+          for (int nh = 0; nh < 2; ++nh)           // value dims [256*nh, 256*nh+256)
             mma_f16_ss(tmem_base + kMlaTmemO + nh * 256, pa0 + ((j * 256) >> 4),
                        vb0 + (((4 * nh) * kMlaChunkBytesK + j * 2048) >> 4), idesc_pv, (t | j) != 0);
-          }
         }
         tc_commit(&kv_empty[s]);
         tc_commit(pv_done);
