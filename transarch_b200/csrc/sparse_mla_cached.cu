@@ -21,8 +21,7 @@
 // Roles (448 threads): warps 0-7 rows, warps 8-11 softmax, warp 12 MMAs, warp 13 keys: it turns positions into slots, up
 // to four tiles ahead of the rows, and has their bytes brought into L2 meanwhile.  (The row warps did that themselves at
 // first: 16 of 79 us at 64 x 128 x 2048.)  All waits are bounded.
-#include "latent_cache.cuh"
-#include "sparse_mla.cuh"
+#include "sparse_mla_cached.cuh"
 
 namespace b200dsa {
 
@@ -33,30 +32,11 @@ constexpr int kMlcRowWarps = 8;
 constexpr int kMlcMaxSplits = 32;
 constexpr int kMlcKeyTiles = 4;      // tiles whose slots are held in shared memory
 
-struct MlaCachedParams {
-  const __nv_bfloat16* q;        // [n_items, n_heads, 576]
-  const uint8_t* cache;
-  int64_t n_slots;
-  const int32_t* table;          // [n_requests, table_stride] pages
-  int64_t table_stride;
-  int table_cols, page_size, n_requests;
-  const int32_t* row_request;    // nullable [n_items]
-  const int32_t* indices;        // [n_items, idx_stride]
-  int64_t idx_stride;
-  int n_idx;
-  const int32_t* n_idx_item;     // nullable [n_items]
-  const int32_t* q_pos;          // nullable [n_items]
-  int q_pos_bias;
-  const int64_t* tree_mask;      // nullable [n_items]
-  const int32_t* tree_base;      // [n_requests] with tree_mask
-  int n_items, n_heads, halves, splits;
-  float scale_log2;
-  void* ctx;
-  int ctx_bf16;
-  float* lse;
-  float* part;                   // splits > 1: [splits, n_items, n_heads, 512] then [splits, n_items, n_heads]
-  int32_t* status;
-};
+__device__ __align__(16) uint8_t g_zero_row[kLatentRowBytes];   // what a missing key reads
+
+__device__ __forceinline__ void st_shared_v4(uint32_t addr, const uint4& v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w));
+}
 
 __global__ void __launch_bounds__(kMlcThreads, 1)
 sparse_mla_cached_kernel(const MlaCachedParams p) {
@@ -148,11 +128,12 @@ sparse_mla_cached_kernel(const MlaCachedParams p) {
     }
     const int r0 = warp * 8;
     // A row's registers: lane l holds codes 16l..16l+15 and their scale, and of two rows (lane / 8 + 4 j) the 16-byte
-    // chunk lane % 8 of the position dims.  A missing key reads row 0 and is made zero when it is stored.
+    // chunk lane % 8 of the position dims.  A missing key reads a row of zeros: whatever lies in the cache, its products
+    // with a probability of zero are zero.
     uint4 code[8];
     float scale[8];
     uint4 pe[2];
-    auto row_ptr = [&](int s) { return p.cache + static_cast<int64_t>(max(s, 0)) * kLatentRowBytes; };
+    auto row_ptr = [&](int s) { return s >= 0 ? p.cache + static_cast<int64_t>(s) * kLatentRowBytes : g_zero_row; };
     auto load_row = [&](int slot, int i) {
       const uint8_t* src = row_ptr(__shfl_sync(0xffffffffu, slot, i));
       code[i] = __ldg(reinterpret_cast<const uint4*>(src) + lane);
@@ -182,24 +163,32 @@ sparse_mla_cached_kernel(const MlaCachedParams p) {
     // Lane l stores 16-byte chunks 2 (l % 4) and 2 (l % 4) + 1 of the 128-byte chunk l / 4 of a row; lanes 4..7 of every
     // eight take them in the other order, so that eight neighbouring lanes write eight different bank groups.
     const bool flip = (lane >> 2) & 1;
-    auto store_rows = [&](uint32_t stage_addr, unsigned vmask, int next) {
+    constexpr int kBatch = 2;
+    auto store_rows = [&](uint32_t stage_addr, int next) {
       const uint32_t dst0 = stage_addr + (lane >> 2) * kMlaChunkBytesK + r0 * 128;
       const int c0 = (lane & 3) * 2 + flip;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint4 c = (vmask >> i) & 1 ? code[i] : make_uint4(0, 0, 0, 0);
-        const float sc = (vmask >> i) & 1 ? scale[i] : 0.f;
-        uint4 w0, w1;
-        dequant_e4m3x4(flip ? c.z : c.x, sc, w0.x, w0.y);
-        dequant_e4m3x4(flip ? c.w : c.y, sc, w0.z, w0.w);
-        dequant_e4m3x4(flip ? c.x : c.z, sc, w1.x, w1.y);
-        dequant_e4m3x4(flip ? c.y : c.w, sc, w1.z, w1.w);
-        load_row(next, i);
-        const uint32_t dst = dst0 + i * 128;
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + ((c0 ^ i) << 4)), "r"(w0.x), "r"(w0.y),
-                     "r"(w0.z), "r"(w0.w) : "memory");
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + ((c0 ^ 1 ^ i) << 4)), "r"(w1.x), "r"(w1.y),
-                     "r"(w1.z), "r"(w1.w) : "memory");
+      for (int i0 = 0; i0 < 8; i0 += kBatch) {
+        uint4 w0[kBatch], w1[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const int i = i0 + u;
+          const uint4 c = code[i];
+          const float sc = scale[i];
+          dequant_e4m3x4(flip ? c.z : c.x, sc, w0[u].x, w0[u].y);
+          dequant_e4m3x4(flip ? c.w : c.y, sc, w0[u].z, w0[u].w);
+          dequant_e4m3x4(flip ? c.x : c.z, sc, w1[u].x, w1[u].y);
+          dequant_e4m3x4(flip ? c.y : c.w, sc, w1[u].z, w1[u].w);
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) load_row(next, i0 + u);
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const int i = i0 + u;
+          const uint32_t dst = dst0 + i * 128;
+          st_shared_v4(dst + ((c0 ^ i) << 4), w0[u]);
+          st_shared_v4(dst + ((c0 ^ 1 ^ i) << 4), w1[u]);
+        }
       }
     };
     for (int t = 0; ok && t < n_tiles; ++t) {
@@ -211,14 +200,12 @@ sparse_mla_cached_kernel(const MlaCachedParams p) {
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       const uint32_t stage_addr = kv_addr + s * kMlaStageBytes;
-      store_rows(stage_addr, vmask, next);
+      store_rows(stage_addr, next);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int i = (lane >> 3) + 4 * j;
         const uint32_t dst = stage_addr + 8 * kMlaChunkBytesK + (r0 + i) * 128 + (((lane & 7) ^ i) << 4);
-        const uint32_t keep = (vmask >> i) & 1 ? 0xffffffffu : 0u;
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(pe[j].x & keep), "r"(pe[j].y & keep),
-                     "r"(pe[j].z & keep), "r"(pe[j].w & keep) : "memory");
+        st_shared_v4(dst, pe[j]);
         load_pe(next, j);
       }
       if (lane == 0) reinterpret_cast<volatile uint8_t*>(&s_mask[s][0])[warp] = static_cast<uint8_t>(vmask);
@@ -373,85 +360,7 @@ sparse_mla_cached_kernel(const MlaCachedParams p) {
     tc_fence_before();
   } else if (warp == 13) {
     // ------------------------------------------------------------------ keys
-    const int32_t* idx_row = p.indices + static_cast<int64_t>(item) * p.idx_stride;
-    int req = p.row_request ? __ldg(p.row_request + item) : item;
-    bool known = req >= 0 && req < p.n_requests;
-    if (!known) {
-      if (lane == 0) atomicMax(p.status, kDevBadIndex);
-      req = 0;
-    }
-    const int32_t* table = p.table + static_cast<int64_t>(req) * p.table_stride;
-    const unsigned long long mask = p.tree_mask ? static_cast<unsigned long long>(__ldg(p.tree_mask + item)) : 0ull;
-    const int base = p.tree_mask ? __ldg(p.tree_base + req) : 0x7fffffff;
-    int64_t last = static_cast<int64_t>(base) - 1;    // the last position that may be attended by selection
-    if (p.q_pos) last = min(last, static_cast<int64_t>(__ldg(p.q_pos + item)) + p.q_pos_bias);
-    struct Key {
-      int page, off;       // page -1: outside the table; off -1: no key
-    };
-    // Positions of keys lane and lane + 32 of tile t, -1 = none.  Positions are fetched two tiles ahead of the pages'
-    // entries, those one ahead of the slots, so that no step waits for the load of the one before it.
-    auto positions = [&](int t, int (&pos)[2]) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int tt = tile0 + t, i = lane + 32 * h;
-        pos[h] = -1;
-        if (t >= n_tiles || !known) continue;
-        if (tt < sel_tiles) {
-          const int j = tt * kMlaTile + i;
-          if (j < n_idx) pos[h] = __ldg(idx_row + j);
-        } else {
-          const int64_t v = static_cast<int64_t>(base) + i;
-          if (((mask >> i) & 1) && base >= 0 && v <= 0x7fffffff) pos[h] = static_cast<int>(v);
-        }
-      }
-    };
-    auto pages = [&](int t, const int (&pos)[2], Key (&key)[2]) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int v = pos[h];
-        key[h].page = key[h].off = -1;
-        if (v < 0 || (v > last && tile0 + t < sel_tiles)) continue;
-        const int col = v / p.page_size;
-        key[h].off = v - col * p.page_size;
-        if (col < p.table_cols) key[h].page = __ldg(table + col);
-      }
-    };
-    auto slot_of = [&](const Key& k) -> int {         // -1 = none; a page that does not exist is reported
-      if (k.off < 0) return -1;
-      const int64_t slot = static_cast<int64_t>(k.page) * p.page_size + k.off;
-      if (k.page < 0 || slot >= p.n_slots) {
-        atomicMax(p.status, kDevBadIndex);
-        return -1;
-      }
-      return static_cast<int>(slot);
-    };
-    int pos[2][2];
-    Key key[2];
-    positions(0, pos[0]);
-    pages(0, pos[0], key);
-    positions(1, pos[1]);
-    positions(2, pos[0]);
-    bool ok = true;
-#pragma unroll 2
-    for (int t = 0; ok && t < n_tiles; ++t) {
-      const int ring = t % kMlcKeyTiles;
-      const int a = slot_of(key[0]), b = slot_of(key[1]);
-      pages(t + 1, pos[(t + 1) & 1], key);
-      positions(t + 3, pos[(t + 1) & 1]);
-      ok = __all_sync(0xffffffffu, mbar_wait(&key_empty[ring], ((t / kMlcKeyTiles) & 1) ^ 1, abort_flag));
-      if (!ok) break;
-      s_slot[ring][lane] = a;
-      s_slot[ring][lane + 32] = b;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&key_full[ring]);
-      // 656 bytes lie in at most seven lines of 128; the first tiles are loaded at once
-      for (int i = 0; t >= 2 && i < 16; ++i) {
-        const int r = 4 * i + (lane >> 3), s = s_slot[ring][r];
-        if (s >= 0 && (lane & 7) < 7)
-          asm volatile("prefetch.global.L2 [%0];" ::"l"(p.cache + static_cast<int64_t>(s) * kLatentRowBytes +
-                                                       min((lane & 7) * 128, kLatentRowBytes - 1)));
-      }
-    }
+    mlc_key_warp<kMlaTile, kMlcKeyTiles>(p, item, tile0, n_tiles, n_idx, &s_slot[0][0], key_full, key_empty, abort_flag);
   } else {
     // ------------------------------------------------------------------ MMA issuer (warp 12)
     // One warp issues everything, in the order S(0), S(1), PV(0), S(2), PV(1), ...: the tensor pipe runs its instructions
