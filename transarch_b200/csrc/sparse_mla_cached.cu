@@ -529,15 +529,19 @@ extern "C" int b200dsa_sparse_mla_decode_cached_splits(int32_t n_items, int32_t 
   if (n_items < 1 || n_heads < 1 || n_idx < 0) return 1;
   DeviceInfo dev;
   if (current_device_info(&dev) != cudaSuccess) return 1;
-  // The least estimated time, in clocks: waves of CTAs over the SMs, 3500 a tile and 12000 around them (prologue, Q, first
-  // rows, output), and for the merge 6000 and the traffic of the parts (2 KB a row written and read, 2 KB a clock).
+  // The least estimated time, in clocks: waves of CTAs over the SMs, so much a tile (64 keys; 128 in the kernel for few
+  // heads) and around them (prologue, Q, first rows, output), and for the merge 6000 and the traffic of the parts (2 KB a
+  // row written and read, 2 KB a clock).
+  const bool few = n_heads <= kMlcFewHeads;
   const int64_t ctas = static_cast<int64_t>(n_items) * (n_heads > kMlaHeadsTile ? 2 : 1);
-  const int tiles = (n_idx + kMlaTile - 1) / kMlaTile + (tree ? 1 : 0);
+  const int keys = few ? 2 * kMlaTile : kMlaTile;
+  const int tiles = (n_idx + keys - 1) / keys + (tree ? 1 : 0);
+  const double tile_clocks = few ? 2800.0 : 3200.0;
   int best = 1;
   double least = 0;
   for (int s = 1; s <= kMlcMaxSplits && (s == 1 || s <= tiles); ++s) {
     const double waves = static_cast<double>((ctas * s + dev.sms - 1) / dev.sms);
-    const double cost = waves * ((tiles + s - 1) / s * 3500.0 + 12000.0) +
+    const double cost = waves * ((tiles + s - 1) / s * tile_clocks + 12000.0) +
                         (s > 1 ? 6000.0 + 2.0 * s * n_items * n_heads : 0.0);
     if (s == 1 || cost < least) {
       least = cost;
@@ -577,9 +581,10 @@ extern "C" int b200dsa_sparse_mla_decode_cached(const void* q_bf16, const void* 
     return B200DSA_EALIGN;
   }
   DeviceInfo dev;
-  static OncePerDevice once;
   cudaError_t e = current_device_info(&dev);
-  if (e == cudaSuccess)
+  const bool few = n_heads <= kMlcFewHeads;
+  static OncePerDevice once;
+  if (e == cudaSuccess && !few)
     e = once.run(dev.index, [] {
       return cudaFuncSetAttribute(sparse_mla_cached_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMlaSmemBytes);
     });
@@ -612,8 +617,10 @@ extern "C" int b200dsa_sparse_mla_decode_cached(const void* q_bf16, const void* 
   p.lse = lse;
   p.part = static_cast<float*>(workspace);
   p.status = status;
-  e = launch_chained(sparse_mla_cached_kernel, dim3(n_items * p.halves * splits), dim3(kMlcThreads), kMlaSmemBytes,
-                     static_cast<cudaStream_t>(stream), p);
+  // Few heads: their codes are multiplied as they are (@RULE@).
+  e = few ? mla_cached_few_launch(p, dev.index, static_cast<cudaStream_t>(stream))
+          : launch_chained(sparse_mla_cached_kernel, dim3(n_items * p.halves * splits), dim3(kMlcThreads), kMlaSmemBytes,
+                           static_cast<cudaStream_t>(stream), p);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e == cudaSuccess && splits > 1) {
     // the merge becomes resident while the attention drains (it waits for it inside)

@@ -1,0 +1,486 @@
+// Sparse MLA attention over the quantised latent cache for up to 16 heads (a tensor-parallel share of a model's heads, or
+// a draft model): the codes go into the tensor cores as they are.
+//
+// With 64 heads a CTA (sparse_mla_cached.cu) the 64 x 64 tiles of a 16-head item would be three quarters empty, and the
+// time of a tile is set by widening 64 rows to bf16.  Here the keys are the UMMA M dimension and the heads are N:
+//
+//   S^T_g [128 keys x 32]  = K_g [128 x 128 dims, e4m3] * (Q_hi | Q_lo)_g      for each group g of 128 dims
+//   R^T   [128 keys x 16]  = K_pe [128 x 64, bf16] * Q_pe
+//   s[key, h] = q_scale[h] * sum_g scale_g[key] * (S_hi + S_lo) + R            one thread a key: its scales are its own
+//   p = 2^(s - m[h]),   P_g = p * scale_g / ref * 2^7 as hi + lo                for each group, because the scales of V differ by group
+//   O^T_g [128 dims x 32] += V_g^T [128 dims x 128 keys, the same bytes read MN-major] * (P_hi | P_lo)_g
+//
+// An 8-bit number has four significant bits, a bf16 number eight: q over a power of two and p are split into two e4m3
+// numbers, hi = e4m3(x) and lo = e4m3(x - hi), so that the products carry bf16's precision down to 2^-17 of the largest
+// value; hi and lo stand side by side in N and are added in fp32.  The position dims stay bf16.  A tile of 128 keys
+// takes 36 MMAs of at most 32 columns, where two tiles of the other kernel take 88 and 128 widened rows.
+//
+// The running maximum m[h] and the reference scale ref (a power of two) are common to the CTA; they are renewed, and O and
+// the sums rescaled, when a score exceeds m by 1.5 or a scale exceeds ref, so that P stays below 2^8.5 < 448.
+//
+// Work split: CTA = (item, split), as in the other kernel.  Roles (512 threads): warps 0-3 rows (16-byte asynchronous
+// copies straight into the operand layout), warp 4 keys, warp 5 MMAs, warps 8-15 softmax (thread = key, eight heads).
+// All waits are bounded.
+#include "sparse_mla_cached.cuh"
+
+namespace b200dsa {
+
+constexpr int kFewThreads = 512;
+constexpr int kFewTile = 128;
+constexpr int kFewHeads = kMlcFewHeads;
+constexpr int kFewStages = 2;
+constexpr int kFewKeyTiles = 4;
+constexpr int kFewGroupBytes = kFewTile * 128;                      // 128 keys x 128 codes
+constexpr int kFewPeOff = 4 * kFewGroupBytes;                       // 128 keys x 64 bf16
+constexpr int kFewScaleOff = kFewPeOff + kFewTile * 128;            // 128 keys x 4 fp32
+constexpr int kFewStageBytes = kFewScaleOff + kFewTile * 16;
+static_assert(kFewStageBytes % 1024 == 0, "stages start on swizzle atoms");
+constexpr int kFewPOff = kFewStages * kFewStageBytes;               // 4 groups x 32 rows (hi, lo) x 128 keys
+constexpr int kFewQOff = kFewPOff + 4 * 32 * 128;                   // 4 groups x 32 rows (hi, lo) x 128 dims
+constexpr int kFewQpeOff = kFewQOff + 4 * 32 * 128;                 // 16 rows x 64 bf16
+constexpr int kFewBarOff = kFewQpeOff + 16 * 128;
+constexpr int kFewSmem = kFewBarOff + 256 + 1024;
+constexpr uint32_t kFewTmemS = 128;                                 // O in columns 0..127, two score buffers of 144 behind
+constexpr uint32_t kFewSCols = 144;                                 // 4 groups x (16 hi + 16 lo), 16 position products
+constexpr float kFewLift = 128.0f;                                  // P = p * 2^7: e4m3's small numbers start at 2^-6
+
+__device__ __align__(16) uint8_t g_few_zero[16];
+
+__device__ __forceinline__ void few_ld8(uint32_t taddr, float (&v)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void few_st8(uint32_t taddr, const float (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "f"(v[0]),
+               "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
+}
+// a and b as e4m3 hi and lo codes: (hi a, hi b) and (lo a, lo b)
+__device__ __forceinline__ void split_e4m3x2(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(hi), __NV_E4M3);
+  const float2 f = __half22float2(__half2(h));
+  lo = __nv_cvt_float2_to_fp8x2(make_float2(a - f.x, b - f.y), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ void few_st_u8(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared.u8 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
+__global__ void __launch_bounds__(kFewThreads, 1)
+sparse_mla_cached_few_kernel(const MlaCachedParams p) {
+  pdl_launch_dependents();
+  pdl_wait_prior();
+  extern __shared__ uint8_t smem_dyn[];
+  __shared__ uint32_t s_tmem_base;
+  __shared__ int s_abort;
+  __shared__ int s_slot[kFewKeyTiles][kFewTile];
+  __shared__ uint32_t s_mask[kFewStages][4];      // validity bit per key of the stage
+  __shared__ int s_renew[3];                      // somebody's key exceeds the references (tile % 3)
+  __shared__ float s_top[4][kFewHeads];           // maxima of the four lane quadrants
+  __shared__ float s_ref[4];                      // largest scales of the four quadrants
+  __shared__ float s_sum[4][kFewHeads];
+  __shared__ float s_qscale[kFewHeads];
+
+  const int split = blockIdx.x % p.splits;
+  const int item = blockIdx.x / p.splits;
+  const uint32_t smem_base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
+  uint8_t* smem_al = smem_dyn + (smem_base - smem_u32(smem_dyn));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem_al + kFewBarOff);
+  uint64_t* kv_full = bars;                       // [stages] 128 row threads: their copies have landed
+  uint64_t* kv_empty = bars + kFewStages;         // [stages] value MMAs retired
+  uint64_t* s_full = bars + 2 * kFewStages;       // [2] score MMAs retired
+  uint64_t* s_empty = s_full + 2;                 // [2] 256 softmax threads have read the scores
+  uint64_t* p_full = s_empty + 2;                 // [1] 256 softmax threads: P written
+  uint64_t* pv_done = p_full + 1;                 // [1] value MMAs retired (P free, O stable)
+  uint64_t* q_full = pv_done + 1;                 // [1] 256 softmax threads: Q written
+  uint64_t* meet = q_full + 1;                    // [1] rendezvous of the eight softmax warps
+  uint64_t* key_full = meet + 1;                  // [kFewKeyTiles]
+  uint64_t* key_empty = key_full + kFewKeyTiles;  // [kFewKeyTiles] four row warps
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int n_idx = p.n_idx_item ? max(0, min(p.n_idx, p.n_idx_item[item])) : p.n_idx;
+  const int all_tiles = (n_idx + kFewTile - 1) / kFewTile + (p.tree_mask ? 1 : 0);
+  const int tile0 = static_cast<int>(static_cast<int64_t>(all_tiles) * split / p.splits);
+  const int n_tiles = static_cast<int>(static_cast<int64_t>(all_tiles) * (split + 1) / p.splits) - tile0;
+  volatile int* abort_flag = &s_abort;
+
+  if (tid == 0) {
+    s_abort = 0;
+    s_renew[0] = s_renew[1] = s_renew[2] = 0;
+    for (int s = 0; s < kFewStages; ++s) {
+      mbar_init(&kv_full[s], 128);
+      mbar_init(&kv_empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&s_empty[s], 256);
+    }
+    mbar_init(p_full, 256);
+    mbar_init(pv_done, 1);
+    mbar_init(q_full, 256);
+    mbar_init(meet, 8);
+    for (int s = 0; s < kFewKeyTiles; ++s) {
+      mbar_init(&key_full[s], 1);
+      mbar_init(&key_empty[s], 4);
+    }
+    mbar_fence_init();
+  }
+  if (warp == 5) {
+    tmem_alloc(&s_tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = s_tmem_base;
+
+  if (warp < 4) {
+    // ------------------------------------------------------------------ rows: warp w the rows 32w .. 32w+31 of a tile
+    for (int t = 0; t < n_tiles; ++t) {
+      const int s = t % kFewStages, ring = t % kFewKeyTiles;
+      const bool ok = mbar_wait(&key_full[ring], (t / kFewKeyTiles) & 1, abort_flag) &&
+                      mbar_wait(&kv_empty[s], ((t / kFewStages) & 1) ^ 1, abort_flag);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      const int mine = s_slot[ring][warp * 32 + lane];
+      const unsigned vmask = __ballot_sync(0xffffffffu, mine >= 0);
+      const uint32_t stage = smem_base + s * kFewStageBytes;
+      // codes: lane l copies 16 bytes l of a row, i.e. piece l % 8 of group l / 8
+      const uint32_t dst0 = stage + (lane >> 3) * kFewGroupBytes + warp * 32 * 128;
+#pragma unroll 8
+      for (int i = 0; i < 32; ++i) {
+        const int slot = __shfl_sync(0xffffffffu, mine, i);
+        const uint8_t* src = slot >= 0 ? p.cache + static_cast<int64_t>(slot) * kLatentRowBytes + lane * 16 : g_few_zero;
+        cp_async_16(dst0 + i * 128 + (((lane & 7) ^ (i & 7)) << 4), src, slot >= 0);
+      }
+      // scales (16 bytes) and position dims (8 pieces) of the rows: 288 pieces
+#pragma unroll
+      for (int u = 0; u < 9; ++u) {
+        const int c = u * 32 + lane, r = c / 9, piece = c - 9 * r;
+        const int slot = __shfl_sync(0xffffffffu, mine, r);
+        const uint8_t* src = slot >= 0 ? p.cache + static_cast<int64_t>(slot) * kLatentRowBytes + 512 + piece * 16 : g_few_zero;
+        const int row = warp * 32 + r;
+        const uint32_t dst = piece == 0 ? stage + kFewScaleOff + row * 16
+                                        : stage + kFewPeOff + row * 128 + (((piece - 1) ^ (row & 7)) << 4);
+        cp_async_16(dst, src, slot >= 0);
+      }
+      if (lane == 0) {
+        s_mask[s][warp] = vmask;
+        mbar_arrive(&key_empty[ring]);
+      }
+      __threadfence_block();
+      __syncwarp();
+      cp_async_mbar_arrive(&kv_full[s]);       // this thread's arrival once all its copies above have landed
+    }
+    cp_async_wait_all();
+  } else if (warp == 4) {
+    mlc_key_warp<kFewTile, kFewKeyTiles>(p, item, tile0, n_tiles, n_idx, &s_slot[0][0], key_full, key_empty, abort_flag);
+  } else if (warp == 5) {
+    // ------------------------------------------------------------------ MMAs, in the order S(0), S(1), PV(0), S(2), ...
+    constexpr uint32_t idesc_s = make_idesc(kFmtE4M3, kFmtE4M3, 128, 32);
+    constexpr uint32_t idesc_r = make_idesc(kFmtBF16, kFmtBF16, 128, 16);
+    constexpr uint32_t idesc_pv = make_idesc(kFmtE4M3, kFmtE4M3, 128, 32, 1, 0);     // A read MN-major: dims x keys
+    auto issue_scores = [&](int t) -> bool {
+      const int s = t % kFewStages, sb = t & 1;
+      const bool w = mbar_wait(&kv_full[s], (t / kFewStages) & 1, abort_flag) &&
+                     mbar_wait(&s_empty[sb], ((t >> 1) & 1) ^ 1, abort_flag);
+      if (!__all_sync(0xffffffffu, w)) return false;
+      fence_proxy_async();               // the rows were copied through the generic proxy
+      tc_fence_after();
+      if (elect_one()) {
+        const uint32_t d = tmem_base + kFewTmemS + sb * kFewSCols;
+        const uint64_t k0 = make_desc_k_sw128(smem_base + s * kFewStageBytes);
+        const uint64_t q0 = make_desc_k_sw128(smem_base + kFewQOff);
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma_f8f6f4_ss(d + g * 32, k0 + ((g * kFewGroupBytes + kk * 32) >> 4), q0 + ((g * 4096 + kk * 32) >> 4), idesc_s,
+                          kk != 0);
+        const uint64_t r0 = make_desc_k_sw128(smem_base + s * kFewStageBytes + kFewPeOff);
+        const uint64_t qr = make_desc_k_sw128(smem_base + kFewQpeOff);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) mma_f16_ss(d + 128, r0 + 2 * kk, qr + 2 * kk, idesc_r, kk != 0);
+        tc_commit(&s_full[sb]);
+      }
+      __syncwarp();
+      return true;
+    };
+    bool ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0, abort_flag));
+    if (ok && n_tiles > 0) ok = issue_scores(0);
+    for (int t = 0; ok && t < n_tiles; ++t) {
+      if (t + 1 < n_tiles && !issue_scores(t + 1)) break;
+      const int s = t % kFewStages;
+      if (!__all_sync(0xffffffffu, mbar_wait(p_full, t & 1, abort_flag))) break;
+      tc_fence_after();
+      if (elect_one()) {
+        // 32 keys an MMA: four atoms of 8 keys x 128 dims, 1024 bytes apart
+        const uint64_t v0 = make_desc_mn_sw128(smem_base + s * kFewStageBytes, kFewGroupBytes, 1024);
+        const uint64_t p0 = make_desc_k_sw128(smem_base + kFewPOff);
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma_f8f6f4_ss(tmem_base + g * 32, v0 + ((g * kFewGroupBytes + kk * 4096) >> 4), p0 + ((g * 4096 + kk * 32) >> 4),
+                          idesc_pv, (t | kk) != 0);
+        tc_commit(&kv_empty[s]);
+        tc_commit(pv_done);
+      }
+      __syncwarp();
+    }
+  } else if (warp >= 8) {
+    // ------------------------------------------------------------------ softmax: thread = key, heads hb .. hb + 7
+    const int wq = warp & 3, hb = ((warp >> 2) & 1) * 8;
+    const int key = wq * 32 + lane;
+    const uint32_t lane_addr = static_cast<uint32_t>(wq * 32) << 16;
+    bool ok = true;
+    uint32_t meets = 0;
+    // rendezvous of the softmax warps, bounded like every wait (a warp that gave up does not come)
+    auto rendezvous = [&]() -> bool {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(meet);
+      return __all_sync(0xffffffffu, mbar_wait(meet, meets++ & 1, abort_flag));
+    };
+    {
+      // Q: warps 8-15 two heads each.  q over a power of two that brings the row's largest value below 448, as hi and lo
+#pragma unroll 1
+      for (int u = 0; u < 2; ++u) {
+        const int h = (warp - 8) * 2 + u;
+        const __nv_bfloat16* row = p.q + (static_cast<int64_t>(item) * p.n_heads + h) * kMlaD;
+        const bool have = h < p.n_heads;
+        float x[16];                                      // dims 8 l + j of either half
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (have) v = __ldg(reinterpret_cast<const uint4*>(row + 256 * half) + lane);
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            x[half * 8 + 2 * j] = __uint_as_float(w[j] << 16);
+            x[half * 8 + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+          }
+        }
+        uint32_t pe = 0;
+        if (have) pe = __ldg(reinterpret_cast<const uint32_t*>(row + 512) + lane);
+        float top = 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) top = max_nan(top, fabsf(x[j]));
+        for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float sc = pow2_at_least(__fdiv_rn(max_nan(top, 1e-30f), 448.0f));
+        const float inv = 1.0f / sc;
+        if (lane == 0) s_qscale[h] = sc;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            split_e4m3x2(x[half * 8 + 2 * j] * inv, x[half * 8 + 2 * j + 1] * inv, hi[j], lo[j]);
+          // dims 256 half + 8 lane: group 2 half + lane / 16, bytes 8 (lane % 16) of its 128
+          const uint32_t at = smem_base + kFewQOff + (2 * half + (lane >> 4)) * 4096 + ((lane & 1) << 3);
+          const uint32_t piece = (lane & 15) >> 1;
+          asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + h * 128 + ((piece ^ (h & 7)) << 4)),
+                       "r"(hi[0] | hi[1] << 16), "r"(hi[2] | hi[3] << 16) : "memory");
+          const int l = 16 + h;
+          asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + l * 128 + ((piece ^ (l & 7)) << 4)),
+                       "r"(lo[0] | lo[1] << 16), "r"(lo[2] | lo[3] << 16) : "memory");
+        }
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(smem_base + kFewQpeOff + h * 128 + (((lane >> 2) ^ (h & 7)) << 4) + (lane & 3) * 4),
+                     "r"(pe) : "memory");
+      }
+      fence_proxy_async();
+      mbar_arrive(q_full);
+      ok = rendezvous();                                   // s_qscale
+    }
+    float qs[8], m[8], l[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      qs[j] = s_qscale[hb + j] * p.scale_log2;
+      m[j] = -INFINITY;
+      l[j] = 0.f;
+    }
+    float ref = 0.f, inv_ref = 0.f;                        // reference scale (a power of two, 0 before the first key)
+    for (int t = 0; ok && t < n_tiles; ++t) {
+      const int sb = t & 1, st = t % kFewStages;
+      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[sb], (t >> 1) & 1, abort_flag) &&
+                                       mbar_wait(&kv_full[st], (t / kFewStages) & 1, abort_flag));   // scales, mask
+      if (!ok) break;
+      {
+        tc_fence_after();
+        const uint32_t src = tmem_base + lane_addr + kFewTmemS + sb * kFewSCols + hb;
+        const bool valid = (s_mask[st][wq] >> lane) & 1;
+        float sc[4];
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(sc[0]), "=f"(sc[1]), "=f"(sc[2]), "=f"(sc[3])
+                     : "r"(smem_base + st * kFewStageBytes + kFewScaleOff + key * 16));
+        float r[8], hi[4][8], lo[4][8];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          few_ld8(src + g * 32, hi[g]);
+          few_ld8(src + g * 32 + 16, lo[g]);
+        }
+        few_ld8(src + 128, r);
+        tc_wait_ld();
+        float s[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float a = 0.f;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) a = fmaf(sc[g], hi[g][j] + lo[g][j], a);
+          s[j] = valid ? fmaf(a, qs[j], r[j] * p.scale_log2) : -INFINITY;
+        }
+        tc_fence_before();
+        mbar_arrive(&s_empty[sb]);
+        // the scale that a value of this key may be multiplied by, as a power of two
+        float big = max_nan(max_nan(fabsf(sc[0]), fabsf(sc[1])), max_nan(fabsf(sc[2]), fabsf(sc[3])));
+        if (!valid) big = 0.f;
+        bool over = !(big <= ref);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) over = over || s[j] > m[j] + 1.5f;
+        if (__any_sync(0xffffffffu, over) && lane == 0) *reinterpret_cast<volatile int*>(&s_renew[t % 3]) = 1;
+        ok = rendezvous();
+        if (!ok) break;
+        if (tid == 256) s_renew[(t + 2) % 3] = 0;           // read by everyone before this barrier, set after the next
+        if (*reinterpret_cast<volatile int*>(&s_renew[t % 3])) {
+          // new references: the largest score of every head and the largest scale among the tile's 128 keys
+          float top[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) top[j] = s[j];
+          for (int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], o));
+            big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, o));
+          }
+          if (lane == 0) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s_top[wq][hb + j] = top[j];
+            if (hb == 0) s_ref[wq] = big;
+          }
+          ok = rendezvous();
+          if (!ok) break;
+          float f[8];
+          const float all = max_nan(max_nan(s_ref[0], s_ref[1]), max_nan(s_ref[2], s_ref[3]));
+          const float new_ref = all <= ref ? ref : pow2_at_least(all);
+          const float shrink = ref > 0.f ? ref / new_ref : 0.f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float n = fmaxf(m[j], fmaxf(fmaxf(s_top[0][hb + j], s_top[1][hb + j]), fmaxf(s_top[2][hb + j], s_top[3][hb + j])));
+            f[j] = m[j] == -INFINITY ? 0.f : exp2f(m[j] - n);
+            m[j] = n;
+            l[j] *= f[j];
+            f[j] *= shrink;
+          }
+          ref = new_ref;
+          inv_ref = ref > 0.f ? 1.0f / ref : 0.f;
+          if (t > 0) {
+            ok = __all_sync(0xffffffffu, mbar_wait(pv_done, (t - 1) & 1, abort_flag));
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {                   // group c / 2, hi or lo
+              float o[8];
+              const uint32_t at = tmem_base + lane_addr + c * 16 + hb;
+              few_ld8(at, o);
+              tc_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 8; ++j) o[j] *= f[j];
+              few_st8(at, o);
+            }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            tc_fence_before();
+          }
+        } else if (t > 0) {
+          ok = __all_sync(0xffffffffu, mbar_wait(pv_done, (t - 1) & 1, abort_flag));    // P is free
+        }
+        // P: row h (hi) and 16 + h (lo) of group g, byte `key`
+        float pr[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float neg = m[j] == -INFINITY ? 0.f : -m[j];
+          const float e = fast_exp2(s[j] + neg);
+          l[j] += e;
+          pr[j] = e * kFewLift;
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float w = valid ? sc[g] * inv_ref : 0.f;
+          const uint32_t base = smem_base + kFewPOff + g * 4096 + (key & 15);
+          const uint32_t piece = key >> 4;
+#pragma unroll
+          for (int j = 0; j < 8; j += 2) {
+            uint32_t h2, l2;
+            split_e4m3x2(pr[j] * w, pr[j + 1] * w, h2, l2);
+            const int r0 = hb + j, r1 = hb + j + 1;         // r & 7 = j: hb and 16 are multiples of eight
+            few_st_u8(base + r0 * 128 + ((piece ^ j) << 4), h2);
+            few_st_u8(base + r1 * 128 + ((piece ^ (j + 1)) << 4), h2 >> 8);
+            few_st_u8(base + (16 + r0) * 128 + ((piece ^ j) << 4), l2);
+            few_st_u8(base + (16 + r1) * 128 + ((piece ^ (j + 1)) << 4), l2 >> 8);
+          }
+        }
+        fence_proxy_async();
+        mbar_arrive(p_full);
+      }
+    }
+    // ---- output: sums over the keys, then thread = dim
+    if (ok && n_tiles > 0) ok = __all_sync(0xffffffffu, mbar_wait(pv_done, (n_tiles - 1) & 1, abort_flag));
+    tc_fence_after();
+    for (int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) l[j] += __shfl_xor_sync(0xffffffffu, l[j], o);
+    }
+    if (lane == 0) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s_sum[wq][hb + j] = l[j];
+    }
+    if (ok) ok = rendezvous();
+    if (ok) {
+      const int64_t parts = static_cast<int64_t>(p.n_items) * p.n_heads;
+      const int64_t row0 = static_cast<int64_t>(item) * p.n_heads + hb;
+      float k[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float sum = s_sum[0][hb + j] + s_sum[1][hb + j] + s_sum[2][hb + j] + s_sum[3][hb + j];
+        const bool any = n_tiles > 0 && sum != 0.f;         // a NaN sum stays NaN in the result
+        k[j] = any ? ref * (1.0f / kFewLift) / sum : 0.f;
+        if (key == 0 && hb + j < p.n_heads) {
+          float* lse = p.splits == 1 ? p.lse + row0 + j : p.part + p.splits * parts * kMlaDv + split * parts + row0 + j;
+          *lse = any ? (m[j] + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+        }
+      }
+#pragma unroll 1
+      for (int g = 0; g < 4; ++g) {
+        float a[8], b[8];
+        if (n_tiles > 0) {
+          few_ld8(tmem_base + lane_addr + g * 32 + hb, a);
+          few_ld8(tmem_base + lane_addr + g * 32 + 16 + hb, b);
+          tc_wait_ld();
+        }
+        const int dim = g * 128 + key;                      // the lane is a dim of the group here
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (hb + j >= p.n_heads) continue;
+          const float v = k[j] != 0.f ? (a[j] + b[j]) * k[j] : 0.f;
+          if (p.splits > 1) p.part[(split * parts + row0 + j) * kMlaDv + dim] = v;
+          else if (p.ctx_bf16) static_cast<__nv_bfloat16*>(p.ctx)[(row0 + j) * kMlaDv + dim] = __float2bfloat16_rn(v);
+          else static_cast<float*>(p.ctx)[(row0 + j) * kMlaDv + dim] = v;
+        }
+        __syncwarp();
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 5) tmem_dealloc(tmem_base, 512);
+  if (tid == 0 && s_abort) atomicMax(p.status, kDevWaitTimeout);
+}
+
+cudaError_t mla_cached_few_launch(const MlaCachedParams& p, int device, cudaStream_t stream) {
+  static OncePerDevice once;
+  cudaError_t e = once.run(device, [] {
+    return cudaFuncSetAttribute(sparse_mla_cached_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem);
+  });
+  if (e != cudaSuccess) return e;
+  return launch_chained(sparse_mla_cached_few_kernel, dim3(p.n_items * p.splits), dim3(kFewThreads), kFewSmem, stream, p);
+}
+
+}  // namespace b200dsa
