@@ -7,7 +7,7 @@
 //   S^T_g [128 keys x 32]  = K_g [128 x 128 dims, e4m3] * (Q_hi | Q_lo)_g      for each group g of 128 dims
 //   R^T   [128 keys x 16]  = K_pe [128 x 64, bf16] * Q_pe
 //   s[key, h] = q_scale[h] * sum_g scale_g[key] * (S_hi + S_lo) + R            one thread a key: its scales are its own
-//   p = 2^(s - m[h]),   P_g = p * scale_g / ref * 2^7 as hi + lo                for each group, because the scales of V differ by group
+//   p = 2^(s - m[h]),   P_g = 16 p * scale_g / ref as hi + lo                for each group, because the scales of V differ by group
 //   O^T_g [128 dims x 32] += V_g^T [128 dims x 128 keys, the same bytes read MN-major] * (P_hi | P_lo)_g
 //
 // An 8-bit number has four significant bits, a bf16 number eight: q over a power of two and p are split into two e4m3
@@ -16,11 +16,13 @@
 // takes 36 MMAs of at most 32 columns, where two tiles of the other kernel take 88 and 128 widened rows.
 //
 // The running maximum m[h] and the reference scale ref (a power of two) are common to the CTA; they are renewed, and O and
-// the sums rescaled, when a score exceeds m by 1.5 or a scale exceeds ref, so that P stays below 2^8.5 < 448.
+// the sums rescaled, when a score exceeds m by 4.5 (base 2) or a scale exceeds ref.
 //
 // Work split: CTA = (item, split), as in the other kernel.  Roles (512 threads): warps 0-3 rows (16-byte asynchronous
-// copies straight into the operand layout), warp 4 keys, warp 5 MMAs, warps 8-15 softmax (thread = key, eight heads).
-// All waits are bounded.
+// copies straight into the operand layout), warp 4 keys, warps 5 and 6 MMAs, warps 8-15 softmax (thread = key, eight heads).
+// All waits are bounded.  148 items x 16 heads x 2048 keys: 52 us (77 us in the kernel for 64 heads), 2.5 us a tile; what
+// bounds it is the way of the rows into shared memory: 164 copies of 512 bytes a tile at 18 clocks each, and two stages,
+// since three do not fit beside P and Q.
 #include "sparse_mla_cached.cuh"
 
 namespace b200dsa {
@@ -42,7 +44,8 @@ constexpr int kFewBarOff = kFewQpeOff + 16 * 128;
 constexpr int kFewSmem = kFewBarOff + 256 + 1024;
 constexpr uint32_t kFewTmemS = 128;                                 // O in columns 0..127, two score buffers of 144 behind
 constexpr uint32_t kFewSCols = 144;                                 // 4 groups x (16 hi + 16 lo), 16 position products
-constexpr float kFewLift = 128.0f;                                  // P = p * 2^7: e4m3's small numbers start at 2^-6
+constexpr float kFewLift = 16.0f;                                   // P = 16 p: probabilities down to 2^-13 keep a digit,
+constexpr float kFewHeadroom = 4.5f;                                // and 16 * 2^4.5 = 362 is the largest P (e4m3 ends at 448)
 
 __device__ __align__(16) uint8_t g_few_zero[16];
 
@@ -177,15 +180,15 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p) {
   } else if (warp == 4) {
     mlc_key_warp<kFewTile, kFewKeyTiles>(p, item, tile0, n_tiles, n_idx, &s_slot[0][0], key_full, key_empty, abort_flag);
   } else if (warp == 5) {
-    // ------------------------------------------------------------------ MMAs, in the order S(0), S(1), PV(0), S(2), ...
+    // ------------------------------------------------------------------ score MMAs
     constexpr uint32_t idesc_s = make_idesc(kFmtE4M3, kFmtE4M3, 128, 32);
     constexpr uint32_t idesc_r = make_idesc(kFmtBF16, kFmtBF16, 128, 16);
-    constexpr uint32_t idesc_pv = make_idesc(kFmtE4M3, kFmtE4M3, 128, 32, 1, 0);     // A read MN-major: dims x keys
-    auto issue_scores = [&](int t) -> bool {
+    bool ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0, abort_flag));
+    for (int t = 0; ok && t < n_tiles; ++t) {
       const int s = t % kFewStages, sb = t & 1;
-      const bool w = mbar_wait(&kv_full[s], (t / kFewStages) & 1, abort_flag) &&
-                     mbar_wait(&s_empty[sb], ((t >> 1) & 1) ^ 1, abort_flag);
-      if (!__all_sync(0xffffffffu, w)) return false;
+      ok = __all_sync(0xffffffffu, mbar_wait(&kv_full[s], (t / kFewStages) & 1, abort_flag) &&
+                                       mbar_wait(&s_empty[sb], ((t >> 1) & 1) ^ 1, abort_flag));
+      if (!ok) break;
       fence_proxy_async();               // the rows were copied through the generic proxy
       tc_fence_after();
       if (elect_one()) {
@@ -205,24 +208,29 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p) {
         tc_commit(&s_full[sb]);
       }
       __syncwarp();
-      return true;
-    };
-    bool ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0, abort_flag));
-    if (ok && n_tiles > 0) ok = issue_scores(0);
+    }
+  } else if (warp == 6) {
+    // ------------------------------------------------------------------ value MMAs.  A warp of their own: behind S(t+1) in
+    // one warp's order they would wait for the rows of tile t+1, which wait for the stage that these MMAs free.
+    constexpr uint32_t idesc_pv = make_idesc(kFmtE4M3, kFmtE4M3, 128, 32, 1, 1);     // both read MN-major: dims x keys x heads
+    bool ok = true;
     for (int t = 0; ok && t < n_tiles; ++t) {
-      if (t + 1 < n_tiles && !issue_scores(t + 1)) break;
       const int s = t % kFewStages;
-      if (!__all_sync(0xffffffffu, mbar_wait(p_full, t & 1, abort_flag))) break;
+      ok = __all_sync(0xffffffffu, mbar_wait(&kv_full[s], (t / kFewStages) & 1, abort_flag) &&
+                                       mbar_wait(p_full, t & 1, abort_flag));
+      if (!ok) break;
+      fence_proxy_async();               // this warp's MMAs read the copied rows too
       tc_fence_after();
       if (elect_one()) {
         // 32 keys an MMA: four atoms of 8 keys x 128 dims, 1024 bytes apart
         const uint64_t v0 = make_desc_mn_sw128(smem_base + s * kFewStageBytes, kFewGroupBytes, 1024);
-        const uint64_t p0 = make_desc_k_sw128(smem_base + kFewPOff);
+        // P without swizzle: 128 bytes between core matrices along the heads, 256 along the keys
+        const uint64_t p0 = make_desc_k_noswz(smem_base + kFewPOff, 256, 128);
 #pragma unroll
         for (int g = 0; g < 4; ++g)
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
-            mma_f8f6f4_ss(tmem_base + g * 32, v0 + ((g * kFewGroupBytes + kk * 4096) >> 4), p0 + ((g * 4096 + kk * 32) >> 4),
+            mma_f8f6f4_ss(tmem_base + g * 32, v0 + ((g * kFewGroupBytes + kk * 4096) >> 4), p0 + ((g * 4096 + kk * 1024) >> 4),
                           idesc_pv, (t | kk) != 0);
         tc_commit(&kv_empty[s]);
         tc_commit(pv_done);
@@ -336,7 +344,7 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p) {
         if (!valid) big = 0.f;
         bool over = !(big <= ref);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) over = over || s[j] > m[j] + 1.5f;
+        for (int j = 0; j < 8; ++j) over = over || s[j] > m[j] + kFewHeadroom;
         if (__any_sync(0xffffffffu, over) && lane == 0) *reinterpret_cast<volatile int*>(&s_renew[t % 3]) = 1;
         ok = rendezvous();
         if (!ok) break;
@@ -391,7 +399,8 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p) {
         } else if (t > 0) {
           ok = __all_sync(0xffffffffu, mbar_wait(pv_done, (t - 1) & 1, abort_flag));    // P is free
         }
-        // P: row h (hi) and 16 + h (lo) of group g, byte `key`
+        // P of group g, MN-major: core matrices of 8 keys x 16 bytes, hi and lo of the 16 heads side by side.  (Stored
+        // K-major, one byte a store, it took 64 stores a thread.)
         float pr[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -400,21 +409,17 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p) {
           l[j] += e;
           pr[j] = e * kFewLift;
         }
+        const uint32_t row = smem_base + kFewPOff + (key >> 3) * 256 + (key & 7) * 16 + hb;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const float w = valid ? sc[g] * inv_ref : 0.f;
-          const uint32_t base = smem_base + kFewPOff + g * 4096 + (key & 15);
-          const uint32_t piece = key >> 4;
+          uint32_t h2[4], l2[4];
 #pragma unroll
-          for (int j = 0; j < 8; j += 2) {
-            uint32_t h2, l2;
-            split_e4m3x2(pr[j] * w, pr[j + 1] * w, h2, l2);
-            const int r0 = hb + j, r1 = hb + j + 1;         // r & 7 = j: hb and 16 are multiples of eight
-            few_st_u8(base + r0 * 128 + ((piece ^ j) << 4), h2);
-            few_st_u8(base + r1 * 128 + ((piece ^ (j + 1)) << 4), h2 >> 8);
-            few_st_u8(base + (16 + r0) * 128 + ((piece ^ j) << 4), l2);
-            few_st_u8(base + (16 + r1) * 128 + ((piece ^ (j + 1)) << 4), l2 >> 8);
-          }
+          for (int j = 0; j < 4; ++j) split_e4m3x2(pr[2 * j] * w, pr[2 * j + 1] * w, h2[j], l2[j]);
+          asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(row + g * 4096), "r"(h2[0] | h2[1] << 16),
+                       "r"(h2[2] | h2[3] << 16) : "memory");
+          asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(row + g * 4096 + 128), "r"(l2[0] | l2[1] << 16),
+                       "r"(l2[2] | l2[3] << 16) : "memory");
         }
         fence_proxy_async();
         mbar_arrive(p_full);
