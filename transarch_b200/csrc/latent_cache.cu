@@ -37,7 +37,6 @@ struct LatentWriteParams {
   const int64_t* slot_mapping;
   uint8_t* cache;
   int64_t n_slots;
-  int use_ue8m0;
   int32_t* status;
 };
 
@@ -67,6 +66,7 @@ __device__ __forceinline__ void latent_load8(const void* p, int64_t i, int f32, 
   }
 }
 
+template <bool kPow2>
 __global__ void __launch_bounds__(32 * kRowWarps) latent_write_kernel(const LatentWriteParams p) {
   pdl_launch_dependents();
   pdl_wait_prior();
@@ -116,13 +116,12 @@ __global__ void __launch_bounds__(32 * kRowWarps) latent_write_kernel(const Late
 #pragma unroll
     for (int j = 0; j < 8; ++j) amax = max_nan(amax, fabsf(x[h][j]));
     for (int o = 8; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    float scale = __fdiv_rn(max_nan(amax, 1e-4f), 448.0f);
-    if (p.use_ue8m0) scale = pow2_at_least(scale);
-    if (!(amax < INFINITY)) scale = __int_as_float(0x7fffffff);   // not finite: the whole group reads as NaN
-    const float rcp = __frcp_rn(scale);
+    GroupScale g = kPow2 ? group_scale_pow2(max_nan(amax, 1e-4f)) : group_scale(max_nan(amax, 1e-4f));
+    if (!(amax < INFINITY)) g.scale = __int_as_float(0x7fffffff);   // not finite: the whole group reads as NaN
+    const float scale = g.scale;
     uint2 codes;
-    codes.x = quant_e4m3x4(x[h][0], x[h][1], x[h][2], x[h][3], scale, rcp);
-    codes.y = quant_e4m3x4(x[h][4], x[h][5], x[h][6], x[h][7], scale, rcp);
+    codes.x = quant_e4m3x4<kPow2>(x[h][0], x[h][1], x[h][2], x[h][3], g);
+    codes.y = quant_e4m3x4<kPow2>(x[h][4], x[h][5], x[h][6], x[h][7], g);
     *reinterpret_cast<uint2*>(row + 256 * h + 8 * lane) = codes;
     if ((lane & 15) == 0) *reinterpret_cast<float*>(row + 512 + 4 * (2 * h + (lane >> 4))) = scale;
   }
@@ -269,9 +268,8 @@ extern "C" int b200dsa_latent_quant_and_cache(const void* kv, int32_t in_f32, in
   p.slot_mapping = slot_mapping;
   p.cache = static_cast<uint8_t*>(cache);
   p.n_slots = n_slots;
-  p.use_ue8m0 = use_ue8m0 != 0;
   p.status = status;
-  return cuda_rc(launch_chained(latent_write_kernel, dim3(static_cast<unsigned>((n_tokens + kRowWarps - 1) / kRowWarps)),
+  return cuda_rc(launch_chained(use_ue8m0 ? latent_write_kernel<true> : latent_write_kernel<false>, dim3(static_cast<unsigned>((n_tokens + kRowWarps - 1) / kRowWarps)),
                                 dim3(32 * kRowWarps), 0, static_cast<cudaStream_t>(stream), p));
 }
 

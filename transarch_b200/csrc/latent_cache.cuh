@@ -29,6 +29,27 @@ __device__ __forceinline__ float pow2_at_least(float x) {
   return __uint_as_float(e << 23);
 }
 
+// The scale of a group whose largest value is amax (not below the format's floor) and its reciprocal, for the e4m3 range
+// of 448 = 1.75 * 2^8: amax / 448, or the smallest power of two that is not below it, which the bits of amax give (its
+// exponent less 8, one more above 1.75) without a division.  An infinite amax gives an infinite scale.
+struct GroupScale {
+  float scale, rcp;
+};
+__device__ __forceinline__ GroupScale group_scale_pow2(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  const uint32_t e = (u >> 23) - 8u + ((u & 0x7fffffu) > 0x600000u ? 1u : 0u);
+  GroupScale g;
+  g.scale = u < 0x7f800000u ? __uint_as_float(e << 23) : amax;
+  g.rcp = u < 0x7f800000u ? __uint_as_float((254u - e) << 23) : 0.f;
+  return g;
+}
+__device__ __forceinline__ GroupScale group_scale(float amax) {
+  GroupScale g;
+  g.scale = __fdiv_rn(amax, 448.0f);
+  g.rcp = __frcp_rn(g.scale);
+  return g;
+}
+
 // x / scale for a scale whose correctly rounded reciprocal r is at hand: q = x r, then q + (x - q scale) r, the remainder
 // exact by FMA.  Correctly rounded by Markstein's theorem (IBM J. Res. Dev. 34, 1990) wherever nothing underflows, at a
 // third of the instructions of a division; quotients that could underflow are far below the smallest code.
@@ -37,12 +58,13 @@ __device__ __forceinline__ float div_by(float x, float scale, float r) {
   return fmaf(fmaf(-q, scale, x), r, q);
 }
 
-// Four values over one scale (r = 1 / scale) as e4m3 codes, nearest even, clamped to +-448 (NaN stays NaN).
-__device__ __forceinline__ uint32_t quant_e4m3x4(float a, float b, float c, float d, float scale, float r) {
-  const __nv_fp8x2_storage_t lo =
-      __nv_cvt_float2_to_fp8x2(make_float2(div_by(a, scale, r), div_by(b, scale, r)), __NV_SATFINITE, __NV_E4M3);
-  const __nv_fp8x2_storage_t hi =
-      __nv_cvt_float2_to_fp8x2(make_float2(div_by(c, scale, r), div_by(d, scale, r)), __NV_SATFINITE, __NV_E4M3);
+// Four values over one scale as e4m3 codes, nearest even, clamped to +-448 (NaN stays NaN).  Over a power of two the
+// product with the reciprocal is exact already.
+template <bool kPow2>
+__device__ __forceinline__ uint32_t quant_e4m3x4(float a, float b, float c, float d, GroupScale g) {
+  auto over = [&](float x) { return kPow2 ? x * g.rcp : div_by(x, g.scale, g.rcp); };
+  const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(make_float2(over(a), over(b)), __NV_SATFINITE, __NV_E4M3);
+  const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(make_float2(over(c), over(d)), __NV_SATFINITE, __NV_E4M3);
   return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
 }
 
