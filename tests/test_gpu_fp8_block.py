@@ -166,3 +166,27 @@ def test_product_captured_and_on_another_stream():
         x.copy_(rows(40, 2048, g))
         graph.replay()
         assert torch.equal(y, K.fp8_block_linear(x, w, ws))
+
+
+@pytest.mark.parametrize("m,n,k", [(5, 20000, 144), (70, 20000, 144), (2049, 2600, 144), (129, 128, 7168), (400, 300, 2064)])
+def test_product_more_tiles_than_multiprocessors_and_split_wide(m, n, k):
+    """Persistent CTAs that take several tiles, in both kernels, and the wide kernel with K cut over a cluster."""
+    from transarch_b200 import kernels as K
+    g = torch.Generator().manual_seed(m + n + k)
+    a, sa, w, sw = operands(m, n, k, g)
+    dev = [t.to(DEV) for t in (a, sa, w, sw)]
+    for dtype in (torch.bfloat16, torch.float32):
+        check_product(a, sa, w, sw, K.fp8_block_matmul(*dev, out_dtype=dtype))
+    assert _status() == 0
+
+
+def test_division_is_correctly_rounded():
+    """Codes of values over plain scales equal those of a true fp32 division, over many magnitudes."""
+    from transarch_b200 import kernels as K
+    g = torch.Generator().manual_seed(11)
+    x = torch.randn(512, 1280, generator=g) * torch.exp2(torch.randint(-20, 20, (512, 1), generator=g).float())
+    q, sc = K.fp8_quantise_rows(x.to(DEV))
+    s = sc.cpu().repeat_interleave(128, 1)
+    ref = (x / s).clamp(-448, 448).to(torch.float8_e4m3fn)                # CPU division: correctly rounded
+    assert torch.equal(q.cpu().view(torch.uint8), ref.view(torch.uint8))
+    assert torch.equal(sc.cpu(), x.view(512, 10, 128).abs().amax(2) / 448)

@@ -429,3 +429,119 @@ def test_long_cache_offsets():
     ref, ref_lse, mass, qk = L.attend(q[0], L.cache_rows(part, local), 0.05)
     assert bool(((out[0].double().cpu() - ref).abs() <= (2 * BF16 + 1e-3) * mass + BF16 * ref.abs()).all())
     assert _status() == 0
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# up to 16 heads: codes multiplied as they are, queries and probabilities as two e4m3 numbers
+# ------------------------------------------------------------------------------------------------------------------
+def check_few(c, ctx, lse, items=None, limit=None):
+    """check_attend with what two e4m3 numbers add: a query value is off by at most 2^-18 of its row's largest, and a
+    probability by 2^-14 (half of e4m3's smallest step, of 16 p), times the largest scale over the key's own."""
+    n, H, _ = c["q"].shape
+    for i in items if items is not None else range(n):
+        r = int(c["req"][i])
+        idx = c["idx"][i] if limit is None else c["idx"][i, :max(0, int(limit[i]))]
+        base = int(c["lens"][r]) if c["mask"] is not None else None
+        slots = L.item_keys(idx, c["table"][r], c["page"], int(c["qpos"][i]), base,
+                            None if c["mask"] is None else int(c["mask"][i]))
+        rows = L.cache_rows(c["cache"], slots)
+        ref, ref_lse, mass, qk = L.attend(c["q"][i], rows, c["scale"])
+        if slots.numel() == 0:
+            assert bool((ctx[i] == 0).all()) and bool((lse[i] == float("-inf")).all())
+            continue
+        k = slots.numel()
+        sc = L.cache_scales(c["cache"], slots).double().repeat_interleave(128, 1)
+        loose = (rows[:, :512].abs() / sc * sc.max()).sum(0)                       # sum |code| * largest scale
+        top = torch.exp((c["q"][i].double() @ rows.t() * c["scale"]).amax(1) - ref_lse).view(-1, 1)
+        q_off = 2.0 ** -18 * c["q"][i].double().abs().amax(1) * rows.abs().sum(1).max() * c["scale"]
+        d = (576 * F32 * qk + q_off).view(-1, 1) + 1e-6
+        step = BF16 if ctx.dtype == torch.bfloat16 else F32
+        bound = (BF16 + 2 * d + k * F32) * mass + 2.0 ** -14 * loose * top + step * ref.abs() + 1e-30
+        got = ctx[i].double().cpu()
+        assert bool(((got - ref).abs() <= bound).all()), (i, float(((got - ref).abs() / bound).max()))
+        lim = d.view(-1) + k * F32 + 8 * F32 * ref_lse.abs() + 2e-7
+        assert bool(((lse[i].double().cpu() - ref_lse).abs() <= lim).all())
+
+
+@pytest.mark.parametrize("requests,per,H,k,ctx,page", [
+    (1, 1, 16, 1, 5, 16), (1, 1, 9, 2048, 4000, 64), (3, 2, 8, 128, 300, 16), (2, 1, 16, 129, 400, 32), (200, 1, 1, 300, 500, 64)])
+def test_few_heads(requests, per, H, k, ctx, page):
+    c = attend_case(requests + k, requests, per, H, k, ctx, page)
+    out, lse = run_attend(c)
+    assert _status() == 0
+    check_few(c, out, lse, items=range(0, requests * per, max(1, requests * per // 8)))
+
+
+@pytest.mark.parametrize("splits", [1, 3, 16])
+def test_few_heads_splits_fp32_and_lengths(splits):
+    c = attend_case(61, 2, 3, 12, 900, 1200, 32)
+    c["idx"][1, 128:640] = -1                                  # whole tiles without a key
+    c["idx"][2] = -1                                           # an item without keys
+    limit = torch.tensor([900, 900, 900, 0, 1, 300], dtype=torch.int32)
+    ws = (splits, torch.empty(splits * 6 * 12 * 513, device=DEV))
+    out, lse = run_attend(c, ctx=torch.empty(6, 12, 512, device=DEV), workspace=ws, n_idx_item=limit.to(DEV))
+    assert _status() == 0
+    check_few(c, out, lse, limit=limit)
+    out16, lse16 = run_attend(c, workspace=ws, n_idx_item=limit.to(DEV))
+    assert torch.equal(out16, out.bfloat16()) and torch.equal(lse16, lse)
+
+
+def test_few_heads_growing_scores_and_scales():
+    """Scores and scales that grow from tile to tile: both references are renewed, the accumulators rescaled."""
+    c = attend_case(62, 1, 1, 16, 640, 640, 64, holes=False)
+    c["lens"][:], c["qpos"][:] = 640, 639
+    sc = torch.exp2(torch.linspace(-12, -3, 640).floor()).view(-1, 1).repeat(1, 4)
+    slots = L.item_keys(torch.arange(640), c["table"][0], 64, 639)
+    c["cache"] = c["cache"].clone()
+    c["cache"][slots, 512:528] = sc.contiguous().view(torch.uint8)
+    c["scale"], c["idx"] = 0.3, torch.arange(640, dtype=torch.int32).view(1, -1)
+    for ws in (None, (1, None)):
+        out, lse = run_attend(c, workspace=ws)
+        assert _status() == 0
+        check_few(c, out, lse)
+    c["idx"] = c["idx"].flip(1).contiguous()                    # and falling ones
+    out, lse = run_attend(c, workspace=(1, None))
+    check_few(c, out, lse)
+
+
+def test_few_heads_plain_scales_mixed_sizes_and_foreign_rows():
+    """Scales that are no powers of two, differing by group; NaN in rows that nobody selects; a row of NaN that one item
+    selects reaches that item alone."""
+    c = attend_case(63, 2, 2, 16, 300, 500, 16, pow2=False, drafts=2)
+    used = set()
+    for i in range(4):
+        r = int(c["req"][i])
+        used |= set(L.item_keys(c["idx"][i], c["table"][r], 16, int(c["qpos"][i]), int(c["lens"][r]), int(c["mask"][i])).tolist())
+    rest = [s for s in range(c["cache"].shape[0]) if s not in used]
+    c["cache"][rest, :512] = 0x7f
+    c["cache"][rest, 512:528] = torch.full((1, 4), float("nan")).view(torch.uint8)
+    c["cache"][rest, 528:] = torch.full((1, 64), float("inf"), dtype=torch.bfloat16).view(torch.uint8)
+    out, lse = run_attend(c)
+    assert _status() == 0
+    check_few(c, out, lse)
+    clean = out.clone()
+    own = L.item_keys(c["idx"][0], c["table"][0], 16, int(c["qpos"][0]), int(c["lens"][0]), None)
+    others = L.item_keys(c["idx"][1], c["table"][0], 16, int(c["qpos"][1]), int(c["lens"][0]), int(c["mask"][1]))
+    lone = next(int(s) for s in own if int(s) not in set(others.tolist()))
+    c["cache"][lone, 512:516] = torch.full((1,), float("nan")).view(torch.uint8)
+    out, lse = run_attend(c)
+    assert bool(torch.isnan(out[0]).all()) and torch.equal(out[1:], clean[1:])
+
+
+@pytest.mark.parametrize("H", [16, 128])
+def test_calls_in_flight_on_two_streams(H):
+    """Two split calls at once: each has a workspace of its own."""
+    cases = [attend_case(70 + i, 2, 1, H, 1500, 2000, 64) for i in range(2)]
+    alone = [run_attend(c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        for c, st in zip(cases, streams):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                got.append(run_attend(c))
+    torch.cuda.synchronize()
+    for i, (out, lse) in enumerate(got):
+        assert torch.equal(out, alone[i % 2][0]) and torch.equal(lse, alone[i % 2][1])
+    assert _status() == 0
