@@ -152,3 +152,24 @@ def test_indexer_projections_in_8_bits(dtype):
     mod._fp8 = {}
     b = mod(h.view(1, T, -1), qi.view(1, T, -1), *c4)
     assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_indexer_projections_of_a_module_made_for_inference():
+    """Parameters made under inference_mode carry no version counter."""
+    from transarch_b200.indexer_module import LightningIndexer
+    g = torch.Generator().manual_seed(34)
+    T, hidden, H, page = 5, 144, 8, 64
+    h = torch.randn(T, hidden, generator=g).bfloat16().to(DEV)
+    cos, sin = torch.ones(T, 64, device=DEV), torch.zeros(T, 64, device=DEV)
+    slots = torch.arange(T, device=DEV)
+    outs = []
+    for inference in (False, True):
+        torch.manual_seed(35)
+        with torch.inference_mode(inference):
+            mod = LightningIndexer(hidden, n_heads=H).to(DEV)
+            mod.quantise_projections()
+            cache = torch.zeros(1, page * 132, dtype=torch.uint8, device=DEV)
+            q, w = mod.forward_quantised(h, h, cos, sin, cache, slots, page)
+            outs.append((q.view(torch.uint8).clone(), w.clone(), cache))
+    for x, y in zip(*outs):
+        assert torch.equal(x.cpu(), y.cpu())

@@ -563,7 +563,7 @@ extern "C" int b200dsa_sparse_mla_decode_cached(const void* q_bf16, const void* 
                                                 void* stream) {
   if (n_items == 0) return B200DSA_OK;
   if (!q_bf16 || !cache || !block_table || (!indices && n_idx > 0) || !ctx || !lse || !status || n_items < 0 ||
-      n_heads < 1 || n_heads > kMlaMaxHeads || n_idx < 0 || idx_stride < n_idx || n_slots < 1 ||
+      n_heads < 1 || n_heads > kMlaMaxHeads || n_idx < 0 || n_idx > (1 << 30) || idx_stride < n_idx || n_slots < 1 ||
       n_slots > 0x7fffffffll || page_size < 1 || table_cols < 1 || table_stride < table_cols || n_requests < 1 ||
       (!row_request && n_requests < n_items) || !(sm_scale > 0.f) || (tree_mask && !tree_base) || splits < 1 || splits > kMlcMaxSplits ||
       static_cast<int64_t>(n_items) * 2 * splits > 0x7fffffffll) {

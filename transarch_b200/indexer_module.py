@@ -27,6 +27,11 @@ from . import kernels as K
 from ._lib import B200DSAError
 
 
+def _version(t: torch.Tensor) -> int:
+    """Counter of in-place writes to t (inference tensors have none)."""
+    return -1 if t.is_inference() else t._version
+
+
 class LightningIndexer(nn.Module):
     def __init__(self, hidden_size: int, n_heads: int = 8, head_dim: int = 128, rope_dim: int = 64,
                  q_input_dim: Optional[int] = None, dtype: torch.dtype = torch.bfloat16):
@@ -49,11 +54,12 @@ class LightningIndexer(nn.Module):
     def quantise_projections(self, scale_fmt: Optional[str] = None) -> None:
         """Keep 8-bit copies of wq and wk (one scale for a block of 128 x 128) for forward_quantised; the activations are
         quantised on the way, with `scale_fmt` scales for 128 values of a row.  The parameters stay as they are; once
-        they change, or move, forward_quantised refuses to run until this has been called again."""
+        they change, or move, forward_quantised refuses to run until this has been called again.  (Writes through `.data`
+        or to parameters made under inference_mode carry no version: after those, call this again yourself.)"""
         held = {}
         for name, lin in (("wq", self.wq), ("wk", self.wk)):
             codes, scale = K.fp8_quantise_blocks(lin.weight.detach(), scale_fmt=scale_fmt)
-            held[name] = (codes, scale, lin.weight, lin.weight._version, lin.weight.dtype)
+            held[name] = (codes, scale, lin.weight, _version(lin.weight), lin.weight.dtype)
         self._fp8, self._fp8_fmt = held, scale_fmt
 
     def _project(self, name: str, x: torch.Tensor) -> torch.Tensor:
@@ -61,7 +67,7 @@ class LightningIndexer(nn.Module):
         if name not in self._fp8:
             return lin(x)
         codes, scale, weight, version, dtype = self._fp8[name]
-        if lin.weight is not weight or weight._version != version or weight.dtype != dtype or \
+        if lin.weight is not weight or _version(weight) != version or weight.dtype != dtype or \
                 weight.device != codes.device:
             raise B200DSAError(f"{name} has changed since quantise_projections(): call it again")
         return K.fp8_block_linear(x, codes, scale, scale_fmt=self._fp8_fmt, out_dtype=x.dtype)
