@@ -190,3 +190,32 @@ def test_division_is_correctly_rounded():
     ref = (x / s).clamp(-448, 448).to(torch.float8_e4m3fn)                # CPU division: correctly rounded
     assert torch.equal(q.cpu().view(torch.uint8), ref.view(torch.uint8))
     assert torch.equal(sc.cpu(), x.view(512, 10, 128).abs().amax(2) / 448)
+
+
+@pytest.mark.parametrize("m,over,k,out", [
+    (5, 2, 2064, torch.bfloat16), (30, 7, 2064, torch.float32), (40, 2, 2064, torch.bfloat16), (128, 18, 2064, torch.bfloat16),
+    (200, 1, 4112, torch.float32), (200, 17, 7184, torch.bfloat16)])
+def test_product_whose_last_tiles_are_a_second_launch(m, over, k, out):
+    """A few tiles more than whole waves of multiprocessors, eager, captured and with the activations quantised on the way."""
+    from transarch_b200 import kernels as K
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    n = (sms // 2 + over) * 256 - 40 if m > 128 else (sms + over) * 128 - 40
+    g = torch.Generator().manual_seed(m + over)
+    a, sa, w, sw = operands(m, n, k, g)
+    d = [t.to(DEV) for t in (a, sa, w, sw)]
+    y = K.fp8_block_matmul(*d, out_dtype=out)
+    check_product(a, sa, w, sw, y)
+    x = torch.randn(m, k, generator=g).bfloat16().to(DEV)
+    lin = K.fp8_block_linear(x, d[2], d[3], out_dtype=out)
+    assert torch.equal(lin, K.fp8_block_matmul(*K.fp8_quantise_rows(x), d[2], d[3], out_dtype=out))
+    got, got_lin = torch.zeros_like(y), torch.zeros_like(y)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        K.fp8_block_matmul(*d, out=got)
+        K.fp8_block_linear(x, d[2], d[3], out=got_lin)
+    for _ in range(3):
+        got.zero_()
+        got_lin.zero_()
+        graph.replay()
+        assert torch.equal(got, y) and torch.equal(got_lin, lin)
+    assert _status() == 0

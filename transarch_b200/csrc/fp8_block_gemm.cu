@@ -15,8 +15,8 @@
 // Many tokens: 128 tokens are M and 256 weight rows N.  A thread owns one token, so that the scale of a block is one
 // register and the shared-memory port carries nothing but the operands (48 KB in by TMA and 48 KB out to the MMAs a block).
 //
-// Measured: 4096 x 7168 x 7168 in 193 us (2.18 PFLOP/s; 920 clocks a block where its MMAs take 512: the tensor pipe waits
-// for the accumulating warps, and 896 tiles are seven waves of 148 SMs); 16 x 18944 x 7168 in 27 us (5.1 TB/s of weights);
+// Measured: 4096 x 7168 x 7168 in 192 us (2.2 PFLOP/s; 920 clocks a block where its MMAs take 512: the tensor pipe waits
+// for the accumulating warps); 16 x 18944 x 7168 in 27 us (5.1 TB/s of weights);
 // 64 x 8192 x 1536 in 8 us, of which the blocks are 3.
 //
 // Narrow kernel, 352 threads: warp 0 TMA loads, warp 1 MMAs, warp 2 scales, warps 3-10 accumulate (two a TMEM lane
@@ -44,6 +44,7 @@ struct GemmParams {
   int out_vec;                 // rows of the result start on 16-byte boundaries
   int m, n, blocks;            // blocks of K
   int m_tiles, n_tiles, splits;
+  int work0, work;             // tiles work0 .. work - 1 are this launch's
   int32_t* status;
 };
 
@@ -213,9 +214,9 @@ fp8_block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
   pdl_wait_prior();      // nothing above touches global memory: as a dependent launch it overlaps the previous kernel
 
   // tiles: neighbouring CTAs share a token tile's neighbours in N, i.e. the same activations
-  const int n_work = p.m_tiles * p.n_tiles;
+  const int n_work = p.work;
   const int rank = p.splits > 1 ? static_cast<int>(gemm_cluster_rank()) : 0;
-  const int first = blockIdx.x / p.splits, stride = gridDim.x / p.splits;
+  const int first = p.work0 + blockIdx.x / p.splits, stride = gridDim.x / p.splits;
   const int b_lo = static_cast<int>(static_cast<int64_t>(p.blocks) * rank / p.splits);
   const int b_hi = static_cast<int>(static_cast<int64_t>(p.blocks) * (rank + 1) / p.splits);
 
@@ -412,7 +413,7 @@ fp8_block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
 static cudaError_t gemm_launch_config(void (*kernel)(CUtensorMap, CUtensorMap, GemmParams), int threads, int smem,
                                       const CUtensorMap& mw, const CUtensorMap& ma, const GemmParams& p, int sms,
                                       bool dependent, cudaStream_t stream) {
-  const int tiles = p.m_tiles * p.n_tiles;
+  const int tiles = p.work - p.work0;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(p.splits > 1 ? tiles * p.splits : (tiles < sms ? tiles : sms));
   cfg.blockDim = dim3(threads);
@@ -528,9 +529,9 @@ fp8_block_gemm_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __g
   tc_fence_after();
   const uint32_t tmem_base = s_tmem_base;
   pdl_wait_prior();
-  const int n_work = p.m_tiles * p.n_tiles;
+  const int n_work = p.work;
   const int rank = kSplit ? static_cast<int>(gemm_cluster_rank()) : 0;
-  const int first = kSplit ? blockIdx.x / p.splits : blockIdx.x, stride = kSplit ? gridDim.x / p.splits : gridDim.x;
+  const int first = kSplit ? p.work0 + blockIdx.x / p.splits : blockIdx.x, stride = kSplit ? gridDim.x / p.splits : gridDim.x;
   const int b_lo = kSplit ? static_cast<int>(static_cast<int64_t>(p.blocks) * rank / p.splits) : 0;
   const int b_hi = kSplit ? static_cast<int>(static_cast<int64_t>(p.blocks) * (rank + 1) / p.splits) : p.blocks;
 
@@ -868,12 +869,21 @@ static int gemm_rc(cudaError_t e) {
 // Kernel, tokens of a tile and CTAs of a cluster for a product of m x n over `blocks` blocks of 128: the least
 // estimated time.  Measured clocks of a block: narrow 830 (16 tokens) .. 1000 (128), bound by the weights from HBM or
 // by the accumulating warps; wide 930.  A wave costs 600 more, a split its barriers and the exchange of the partial sums.
-// nt = 0: the kernel for many tokens.
+// Tiles that would start one more, mostly empty wave can be a launch of their own, their K split over clusters:
+// 256 x 19200 x 7168 69 -> 50 us, 2048 x 4736 x 7168 75 -> 67, 16 x 19200 x 7168 51 -> 35, 4096 x 7168 x 7168 (six waves
+// and 8 tiles) 194.5 -> 192.  An estimated gain below 7 % was none: 8192 x 7168 x 7168 370 -> 377, 64 x 19200 x 1536 13.4 ->
+// 14.0 (after many full waves the tensor pipes are at the power limit, and an idle last wave is paid back in clocks).
+struct GemmPlan {
+  int nt;             // tokens of a tile; 0 = the kernel for many tokens
+  int splits;
+  int rest_splits;    // above 1: the tiles behind the last full wave are a second launch with so many splits
+};
 constexpr double gemm_cost(int64_t tiles, int splits, int blocks, int sms, double block_clocks, double exchange) {
   return static_cast<double>((tiles * splits + sms - 1) / sms) * ((blocks + splits - 1) / splits * block_clocks + 600.0) +
          (splits > 1 ? 1000.0 + exchange : 0.0);
 }
-static void gemm_plan(int m, int n, int blocks, int sms, int* nt_out, int* splits_out) {
+static GemmPlan gemm_plan(int m, int n, int blocks, int sms) {
+  GemmPlan plan{};
   double best = 0;
   for (int nt = 16; nt <= 256; nt *= 2) {                // 256 stands for the wide kernel: 128 tokens x 256 columns
     if (nt < 128 && nt < m) continue;                    // one token tile as long as 128 tokens hold the batch
@@ -881,17 +891,23 @@ static void gemm_plan(int m, int n, int blocks, int sms, int* nt_out, int* split
     const bool wide = nt == 256;
     const int64_t tiles = wide ? static_cast<int64_t>((n + 255) / 256) * ((m + 127) / 128)
                                : static_cast<int64_t>((n + 127) / 128) * ((m + nt - 1) / nt);
-    for (int s = 1; s <= 8; s *= 2) {
-      if (s > 1 && (tiles * s > sms || blocks < 2 * s)) break;
-      const double cost = wide ? gemm_cost(tiles, s, blocks, sms, 930.0, 3000.0)
-                               : gemm_cost(tiles, s, blocks, sms, 800.0 + 1.5 * nt, 12.0 * nt);
+    const double block_clocks = wide ? 930.0 : 800.0 + 1.5 * nt, exchange = wide ? 3000.0 : 12.0 * nt;
+    const double second_launch = wide ? 16000.0 : 6000.0;
+    auto consider = [&](double cost, int splits, int rest_splits) {
       if (best == 0 || cost < best) {
         best = cost;
-        *nt_out = wide ? 0 : nt;
-        *splits_out = s;
+        plan = GemmPlan{wide ? 0 : nt, splits, rest_splits};
       }
+    };
+    const int64_t rest = tiles % sms;
+    for (int s = 1; s <= 8; s *= 2) {
+      if (s == 1 || (tiles * s <= sms && blocks >= 2 * s)) consider(gemm_cost(tiles, s, blocks, sms, block_clocks, exchange), s, 1);
+      if (s > 1 && tiles > sms && rest > 0 && rest * s <= sms && blocks >= 2 * s)
+        consider(1.07 * (gemm_cost(tiles - rest, 1, blocks, sms, block_clocks, exchange) +
+                         gemm_cost(rest, s, blocks, sms, block_clocks, exchange) + second_launch), 1, s);
     }
   }
+  return plan;
 }
 
 }  // namespace b200dsa
@@ -971,9 +987,9 @@ static int block_matmul(const void* a_e4m3, int64_t a_stride, const float* a_sca
   if (!enc) return B200DSA_ECUDA;
   DeviceInfo dev;
   if (cudaError_t e = current_device_info(&dev)) return gemm_rc(e);
-  int nt = 0, splits = 1;
   const int blocks = (k + 127) / 128;
-  gemm_plan(m, n, blocks, dev.sms, &nt, &splits);
+  const GemmPlan plan = gemm_plan(m, n, blocks, dev.sms);
+  const int nt = plan.nt;
   CUtensorMap mw, ma;
   cuuint32_t es[2] = {1, 1};
   cuuint64_t dw[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(n)}, sw[1] = {static_cast<cuuint64_t>(w_stride)};
@@ -1004,16 +1020,25 @@ static int block_matmul(const void* a_e4m3, int64_t a_stride, const float* a_sca
   p.blocks = blocks;
   p.m_tiles = nt ? (m + nt - 1) / nt : (m + 127) / 128;
   p.n_tiles = nt ? (n + 127) / 128 : (n + 255) / 256;
-  p.splits = splits;
   p.status = status;
-  const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  switch (nt) {
-    case 16: return gemm_rc(gemm_launch<16>(mw, ma, p, dev, dependent, st));
-    case 32: return gemm_rc(gemm_launch<32>(mw, ma, p, dev, dependent, st));
-    case 64: return gemm_rc(gemm_launch<64>(mw, ma, p, dev, dependent, st));
-    case 128: return gemm_rc(gemm_launch<128>(mw, ma, p, dev, dependent, st));
-    default: return gemm_rc(splits > 1 ? wide_launch<true>(mw, ma, p, dev, dependent, st) : wide_launch<false>(mw, ma, p, dev, dependent, st));
-  }
+  const int tiles = p.m_tiles * p.n_tiles, rest = plan.rest_splits > 1 ? tiles % dev.sms : 0;
+  auto launch = [&](int work0, int work, int splits, bool dep) -> cudaError_t {
+    p.work0 = work0;
+    p.work = work;
+    p.splits = splits;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    switch (nt) {
+      case 16: return gemm_launch<16>(mw, ma, p, dev, dep, st);
+      case 32: return gemm_launch<32>(mw, ma, p, dev, dep, st);
+      case 64: return gemm_launch<64>(mw, ma, p, dev, dep, st);
+      case 128: return gemm_launch<128>(mw, ma, p, dev, dep, st);
+      default: return splits > 1 ? wide_launch<true>(mw, ma, p, dev, dep, st) : wide_launch<false>(mw, ma, p, dev, dep, st);
+    }
+  };
+  cudaError_t e = launch(0, tiles - rest, plan.splits, dependent);
+  // its CTAs start as those of the full waves leave
+  if (e == cudaSuccess && rest > 0) e = launch(tiles - rest, tiles, plan.rest_splits, true);
+  return gemm_rc(e);
 }
 
 extern "C" int b200dsa_fp8_block_matmul(const void* a_e4m3, int64_t a_stride, const float* a_scale, int64_t sa_m,
