@@ -545,3 +545,46 @@ def test_calls_in_flight_on_two_streams(H):
     for i, (out, lse) in enumerate(got):
         assert torch.equal(out, alone[i % 2][0]) and torch.equal(lse, alone[i % 2][1])
     assert _status() == 0
+
+
+@pytest.mark.parametrize("H", [3, 16, 40, 128])
+def test_items_that_share_a_request_equal_calls_of_their_own(H):
+    """Many items a request (rows are not prefetched then) against one item a call (they are), bit for bit."""
+    c = attend_case(90 + H, 2, 8, H, 700, 900, 32)
+    one = (1, None)
+    out, lse = run_attend(c, workspace=one)
+    assert _status() == 0
+    if H <= 16:
+        check_few(c, out, lse, items=(0, 7, 15))
+    else:
+        check_attend(c, out, lse, items=(0, 7, 15))
+    for i in range(16):
+        alone = dict(c, q=c["q"][i:i + 1], idx=c["idx"][i:i + 1], req=c["req"][i:i + 1], qpos=c["qpos"][i:i + 1])
+        got, got_lse = run_attend(alone, workspace=one)
+        assert torch.equal(got[0], out[i]) and torch.equal(got_lse[0], lse[i])
+
+
+def test_few_heads_long_cache_and_missing_rows_among_four():
+    """Slots whose byte offset passes 32 bits; of four rows that come in one copy any may be missing, the cache's first and
+    last slot among the others."""
+    from transarch_b200 import kernels as K
+    slots_n, page = 6_600_000 // 64 * 64, 64
+    cache = torch.zeros(slots_n, 656, dtype=torch.uint8, device=DEV)
+    g = torch.Generator().manual_seed(6)
+    own = random_cache(2 * page, g)
+    cache[:page] = own[:page].to(DEV)
+    cache[slots_n - page:] = own[page:].to(DEV)
+    table = torch.tensor([[0, slots_n // page - 1]], dtype=torch.int32)
+    n = 16
+    idx = torch.stack([torch.randperm(2 * page, generator=g) for _ in range(n)]).to(torch.int32)
+    for i in range(n):                             # every pattern of missing rows among four
+        for j in range(4):
+            if i >> j & 1:
+                idx[i, j::4] = -1
+    q = torch.randn(n, 16, 576, generator=g).bfloat16()
+    out, lse = K.sparse_mla_decode_cached(q.to(DEV), cache, page, idx.to(DEV), 0.05, block_table=table.to(DEV),
+                                          row_request=torch.zeros(n, dtype=torch.int32, device=DEV))
+    assert _status() == 0
+    local = dict(cache=own, page=page, scale=0.05, table=torch.tensor([[0, 1]], dtype=torch.int32), q=q, idx=idx,
+                 req=torch.zeros(n, dtype=torch.int32), qpos=torch.full((n,), 2 * page, dtype=torch.int32), mask=None)
+    check_few(local, out, lse)

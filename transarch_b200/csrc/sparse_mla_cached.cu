@@ -38,6 +38,7 @@ __device__ __forceinline__ void st_shared_v4(uint32_t addr, const uint4& v) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w));
 }
 
+template <bool kPrefetch>
 __global__ void __launch_bounds__(kMlcThreads, 1)
 sparse_mla_cached_kernel(const MlaCachedParams p) {
   pdl_launch_dependents();
@@ -360,7 +361,7 @@ sparse_mla_cached_kernel(const MlaCachedParams p) {
     tc_fence_before();
   } else if (warp == 13) {
     // ------------------------------------------------------------------ keys
-    mlc_key_warp<kMlaTile, kMlcKeyTiles>(p, item, tile0, n_tiles, n_idx, &s_slot[0][0], key_full, key_empty, abort_flag);
+    mlc_key_warp<kMlaTile, kMlcKeyTiles, kPrefetch>(p, item, tile0, n_tiles, n_idx, &s_slot[0][0], key_full, key_empty, abort_flag);
   } else {
     // ------------------------------------------------------------------ MMA issuer (warp 12)
     // One warp issues everything, in the order S(0), S(1), PV(0), S(2), PV(1), ...: the tensor pipe runs its instructions
@@ -515,6 +516,17 @@ __global__ void __launch_bounds__(128) mla_merge_kernel(const float* __restrict_
   if (threadIdx.x == 0) lse[row] = den != 0.f ? top + logf(den) : -INFINITY;
 }
 
+template <bool kPrefetch>
+static cudaError_t mlc_launch(const MlaCachedParams& p, int device, cudaStream_t stream) {
+  static OncePerDevice once;
+  const cudaError_t e = once.run(device, [] {
+    return cudaFuncSetAttribute(sparse_mla_cached_kernel<kPrefetch>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMlaSmemBytes);
+  });
+  if (e != cudaSuccess) return e;
+  return launch_chained(sparse_mla_cached_kernel<kPrefetch>, dim3(p.n_items * p.halves * p.splits), dim3(kMlcThreads),
+                        kMlaSmemBytes, stream, p);
+}
+
 static int mlc_rc(cudaError_t e) {
   if (e == cudaSuccess) return B200DSA_OK;
   set_last_error(cudaGetErrorString(e));
@@ -537,7 +549,7 @@ extern "C" int b200dsa_sparse_mla_decode_cached_splits(int32_t n_items, int32_t 
   const int64_t ctas = static_cast<int64_t>(n_items) * (n_heads > kMlaHeadsTile ? 2 : 1);
   const int keys = few ? 2 * kMlaTile : kMlaTile;
   const int tiles = (n_idx + keys - 1) / keys + (tree ? 1 : 0);
-  const double tile_clocks = few ? 4800.0 : 3700.0;
+  const double tile_clocks = few ? 3900.0 : 3700.0;
   int best = 1;
   double least = 0;
   for (int s = 1; s <= kMlcMaxSplits && (s == 1 || s <= tiles); ++s) {
@@ -584,11 +596,6 @@ extern "C" int b200dsa_sparse_mla_decode_cached(const void* q_bf16, const void* 
   DeviceInfo dev;
   cudaError_t e = current_device_info(&dev);
   const bool few = n_heads <= kMlcFewHeads;
-  static OncePerDevice once;
-  if (e == cudaSuccess && !few)
-    e = once.run(dev.index, [] {
-      return cudaFuncSetAttribute(sparse_mla_cached_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMlaSmemBytes);
-    });
   if (e != cudaSuccess) return mlc_rc(e);
   MlaCachedParams p{};
   p.q = static_cast<const __nv_bfloat16*>(q_bf16);
@@ -618,11 +625,13 @@ extern "C" int b200dsa_sparse_mla_decode_cached(const void* q_bf16, const void* 
   p.lse = lse;
   p.part = static_cast<float*>(workspace);
   p.status = status;
-  // Up to 16 heads the codes are multiplied as they are: 148 items x 2048 keys take 52 us for 16 heads, and 77 us for 17,
+  // Up to 16 heads the codes are multiplied as they are: 148 items x 2048 keys take 49 us for 16 heads, and 77 us for 17,
   // which the kernel for 64 heads does (it takes the same time for 1 head as for 64).
-  e = few ? mla_cached_few_launch(p, dev.index, static_cast<cudaStream_t>(stream))
-          : launch_chained(sparse_mla_cached_kernel, dim3(n_items * p.halves * splits), dim3(kMlcThreads), kMlaSmemBytes,
-                           static_cast<cudaStream_t>(stream), p);
+  // Rows that several items of a request select are in L2 after the first of them; prefetches then only take load slots (2048
+  // items of one request 1788 us with, 1748 without; one item a request 71.7 with, 78.7 without).
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (few) e = mla_cached_few_launch(p, dev.index, st);
+  else e = n_items >= 4ll * n_requests ? mlc_launch<false>(p, dev.index, st) : mlc_launch<true>(p, dev.index, st);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e == cudaSuccess && splits > 1) {
     // the merge becomes resident while the attention drains (it waits for it inside)

@@ -33,9 +33,9 @@ struct MlaCachedParams {
 
 
 // One warp turns the positions of an item's keys into slots of the cache, kTile keys at a time, up to kRing tiles ahead of
-// the warps that fetch the rows, and has the rows brought into L2 meanwhile.  Tiles tile0 .. tile0 + n_tiles - 1 of the
+// the warps that fetch the rows, and with kPrefetch has the rows brought into L2 meanwhile.  Tiles tile0 .. tile0 + n_tiles - 1 of the
 // item: its selected positions, then (with a tree mask) one tile of drafted tokens.
-template <int kTile, int kRing>
+template <int kTile, int kRing, bool kPrefetch>
 __device__ __forceinline__ void mlc_key_warp(const MlaCachedParams& p, int item, int tile0, int n_tiles, int n_idx,
                                              int* s_slot, uint64_t* key_full, uint64_t* key_empty,
                                              volatile int* abort_flag) {
@@ -116,7 +116,7 @@ __device__ __forceinline__ void mlc_key_warp(const MlaCachedParams& p, int item,
     __syncwarp();
     if (lane == 0) mbar_arrive(&key_full[ring]);
     // 656 bytes lie in at most seven lines of 128; the first tiles are loaded at once
-    for (int i = 0; t >= 2 && i < kTile / 4; ++i) {
+    for (int i = 0; kPrefetch && t >= 2 && i < kTile / 4; ++i) {
       const int r = 4 * i + (lane >> 3), s = s_slot[ring * kTile + r];
       if (s >= 0 && (lane & 7) < 7)
         asm volatile("prefetch.global.L2 [%0];" ::"l"(p.cache + static_cast<int64_t>(s) * kLatentRowBytes +

@@ -18,11 +18,14 @@
 // The running maximum m[h] and the reference scale ref (a power of two) are common to the CTA; they are renewed, and O and
 // the sums rescaled, when a score exceeds m by 4.5 (base 2) or a scale exceeds ref.
 //
-// Work split: CTA = (item, split), as in the other kernel.  Roles (512 threads): warps 0-3 rows (16-byte asynchronous
-// copies straight into the operand layout), warp 4 keys, warps 5 and 6 MMAs, warps 8-15 softmax (thread = key, eight heads).
-// All waits are bounded.  148 items x 16 heads x 2048 keys: 52 us (77 us in the kernel for 64 heads), 2.5 us a tile; what
-// bounds it is the way of the rows into shared memory: 164 copies of 512 bytes a tile at 18 clocks each, and two stages,
-// since three do not fit beside P and Q.
+// Work split: CTA = (item, split), as in the other kernel.  Roles (512 threads): warps 0-3 rows (TMA gathers of four rows
+// x 128 bytes straight into the operand layout, the scales by 16-byte asynchronous copies), warp 4 keys, warps 5 and 6 MMAs,
+// warps 8-15 softmax (thread = key, eight heads).  All waits are bounded.  148 items x 16 heads x 2048 keys, every item a
+// request of its own: 49 us (78 us in the kernel for 64 heads); 592 items of 148 requests: 176 us.  A tile takes 2 us: of the
+// 7 k clocks of its chain (rows 2.2, scores 1.3, softmax 1.8, values 1.8) two stages overlap two, and a third does not fit
+// beside P and Q.  Before the gathers (every 16 bytes by an asynchronous copy, 28 bytes a clock) it took 2.5 us.  A
+// gather takes its issuing lane about 50 clocks: two issuing warps take 2 - 4 % longer, one 14 - 20 %, and a copy of each lane of
+// a warp 90 clocks.
 #include "sparse_mla_cached.cuh"
 
 namespace b200dsa {
@@ -32,6 +35,7 @@ constexpr int kFewTile = 128;
 constexpr int kFewHeads = kMlcFewHeads;
 constexpr int kFewStages = 2;
 constexpr int kFewKeyTiles = 4;
+constexpr int kFewRowWarps = 4;
 constexpr int kFewGroupBytes = kFewTile * 128;                      // 128 keys x 128 codes
 constexpr int kFewPeOff = 4 * kFewGroupBytes;                       // 128 keys x 64 bf16
 constexpr int kFewScaleOff = kFewPeOff + kFewTile * 128;            // 128 keys x 4 fp32
@@ -49,6 +53,14 @@ constexpr float kFewHeadroom = 4.5f;                                // and 16 * 
 
 __device__ __align__(16) uint8_t g_few_zero[16];
 
+// 128 bytes from byte x of the rows r.x .. r.w, zeros for a row that does not exist (-1).
+__device__ __forceinline__ void few_gather4(uint32_t dst, const CUtensorMap* m, uint64_t* bar, int x, int4 r) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, "
+      "%6}], [%7];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w),
+      "r"(smem_u32(bar))
+      : "memory");
+}
 __device__ __forceinline__ void few_ld8(uint32_t taddr, float (&v)[8]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
@@ -67,18 +79,16 @@ __device__ __forceinline__ void split_e4m3x2(float a, float b, uint32_t& hi, uin
   const float2 f = __half22float2(__half2(h));
   lo = __nv_cvt_float2_to_fp8x2(make_float2(a - f.x, b - f.y), __NV_SATFINITE, __NV_E4M3);
 }
-__device__ __forceinline__ void few_st_u8(uint32_t addr, uint32_t v) {
-  asm volatile("st.shared.u8 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
-}
 
+template <bool kPrefetch>
 __global__ void __launch_bounds__(kFewThreads, 1)
-sparse_mla_cached_few_kernel(const MlaCachedParams p) {
+sparse_mla_cached_few_kernel(const MlaCachedParams p, const __grid_constant__ CUtensorMap tmap_rows) {
   pdl_launch_dependents();
   pdl_wait_prior();
   extern __shared__ uint8_t smem_dyn[];
   __shared__ uint32_t s_tmem_base;
   __shared__ int s_abort;
-  __shared__ int s_slot[kFewKeyTiles][kFewTile];
+  __shared__ __align__(16) int s_slot[kFewKeyTiles][kFewTile];
   __shared__ uint32_t s_mask[kFewStages][4];      // validity bit per key of the stage
   __shared__ int s_renew[3];                      // somebody's key exceeds the references (tile % 3)
   __shared__ float s_top[4][kFewHeads];           // maxima of the four lane quadrants
@@ -91,7 +101,7 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p) {
   const uint32_t smem_base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
   uint8_t* smem_al = smem_dyn + (smem_base - smem_u32(smem_dyn));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem_al + kFewBarOff);
-  uint64_t* kv_full = bars;                       // [stages] 128 row threads: their copies have landed
+  uint64_t* kv_full = bars;                       // [stages] the row warps' threads, their issuing lanes and bytes
   uint64_t* kv_empty = bars + kFewStages;         // [stages] value MMAs retired
   uint64_t* s_full = bars + 2 * kFewStages;       // [2] score MMAs retired
   uint64_t* s_empty = s_full + 2;                 // [2] 256 softmax threads have read the scores
@@ -100,7 +110,7 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p) {
   uint64_t* q_full = pv_done + 1;                 // [1] 256 softmax threads: Q written
   uint64_t* meet = q_full + 1;                    // [1] rendezvous of the eight softmax warps
   uint64_t* key_full = meet + 1;                  // [kFewKeyTiles]
-  uint64_t* key_empty = key_full + kFewKeyTiles;  // [kFewKeyTiles] four row warps
+  uint64_t* key_empty = key_full + kFewKeyTiles;  // [kFewKeyTiles] the row warps
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int n_idx = p.n_idx_item ? max(0, min(p.n_idx, p.n_idx_item[item])) : p.n_idx;
@@ -113,7 +123,7 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p) {
     s_abort = 0;
     s_renew[0] = s_renew[1] = s_renew[2] = 0;
     for (int s = 0; s < kFewStages; ++s) {
-      mbar_init(&kv_full[s], 128);
+      mbar_init(&kv_full[s], 33 * kFewRowWarps);
       mbar_init(&kv_empty[s], 1);
     }
     for (int s = 0; s < 2; ++s) {
@@ -126,7 +136,7 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p) {
     mbar_init(meet, 8);
     for (int s = 0; s < kFewKeyTiles; ++s) {
       mbar_init(&key_full[s], 1);
-      mbar_init(&key_empty[s], 4);
+      mbar_init(&key_empty[s], kFewRowWarps);
     }
     mbar_fence_init();
   }
@@ -139,46 +149,51 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p) {
   tc_fence_after();
   const uint32_t tmem_base = s_tmem_base;
 
-  if (warp < 4) {
-    // ------------------------------------------------------------------ rows: warp w the rows 32w .. 32w+31 of a tile
+  if (warp < kFewRowWarps) {
+    // ------------------------------------------------------------------ rows: warp w the rows w * kPer ... of a tile
+    constexpr int kPer = kFewTile / kFewRowWarps;
+    int started = 0;
     for (int t = 0; t < n_tiles; ++t) {
       const int s = t % kFewStages, ring = t % kFewKeyTiles;
       const bool ok = mbar_wait(&key_full[ring], (t / kFewKeyTiles) & 1, abort_flag) &&
                       mbar_wait(&kv_empty[s], ((t / kFewStages) & 1) ^ 1, abort_flag);
       if (!__all_sync(0xffffffffu, ok)) break;
-      const int mine = s_slot[ring][warp * 32 + lane];
-      const unsigned vmask = __ballot_sync(0xffffffffu, mine >= 0);
       const uint32_t stage = smem_base + s * kFewStageBytes;
-      // codes: lane l copies 16 bytes l of a row, i.e. piece l % 8 of group l / 8
-      const uint32_t dst0 = stage + (lane >> 3) * kFewGroupBytes + warp * 32 * 128;
-#pragma unroll 8
-      for (int i = 0; i < 32; ++i) {
-        const int slot = __shfl_sync(0xffffffffu, mine, i);
-        const uint8_t* src = slot >= 0 ? p.cache + static_cast<int64_t>(slot) * kLatentRowBytes + lane * 16 : g_few_zero;
-        cp_async_16(dst0 + i * 128 + (((lane & 7) ^ (i & 7)) << 4), src, slot >= 0);
-      }
-      // scales (16 bytes) and position dims (8 pieces) of the rows: 288 pieces
 #pragma unroll
-      for (int u = 0; u < 9; ++u) {
-        const int c = u * 32 + lane, r = c / 9, piece = c - 9 * r;
-        const int slot = __shfl_sync(0xffffffffu, mine, r);
-        const uint8_t* src = slot >= 0 ? p.cache + static_cast<int64_t>(slot) * kLatentRowBytes + 512 + piece * 16 : g_few_zero;
-        const int row = warp * 32 + r;
-        const uint32_t dst = piece == 0 ? stage + kFewScaleOff + row * 16
-                                        : stage + kFewPeOff + row * 128 + (((piece - 1) ^ (row & 7)) << 4);
-        cp_async_16(dst, src, slot >= 0);
+      for (int u = 0; u < kPer / 32; ++u) {
+        const int row = warp * kPer + u * 32 + lane, slot = s_slot[ring][row];
+        const unsigned valid = __ballot_sync(0xffffffffu, slot >= 0);
+        if (lane == 0) s_mask[s][row >> 5] = valid;
+        const uint8_t* src = slot >= 0 ? p.cache + static_cast<int64_t>(slot) * kLatentRowBytes + 512 : g_few_zero;
+        cp_async_16(stage + kFewScaleOff + row * 16, src, slot >= 0);
       }
-      if (lane == 0) {
-        s_mask[s][warp] = vmask;
+      __syncwarp();
+      if (elect_one()) {
+        mbar_arrive_expect_tx(&kv_full[s], kPer * 640);
+        const int4* quads = reinterpret_cast<const int4*>(&s_slot[ring][warp * kPer]);
+#pragma unroll 4
+        for (int q = 0; q < kPer / 4; ++q) {
+          const int4 rows = quads[q];
+#pragma unroll
+          for (int g = 0; g < 5; ++g)
+            few_gather4(stage + g * kFewGroupBytes + (warp * (kPer / 4) + q) * 512, &tmap_rows, &kv_full[s],
+                        g < 4 ? g * 128 : 528, rows);
+        }
         mbar_arrive(&key_empty[ring]);
       }
-      __threadfence_block();
       __syncwarp();
-      cp_async_mbar_arrive(&kv_full[s]);       // this thread's arrival once all its copies above have landed
+      cp_async_mbar_arrive(&kv_full[s]);       // this thread's arrival once its copies above have landed
+      started = t + 1;
     }
     cp_async_wait_all();
+    // whatever ended the loop, the copies in flight land before the shared memory is given up
+    for (int t = max(0, started - kFewStages); t < started; ++t) {
+      const long long t0 = clock64();
+      while (!mbar_test(&kv_full[t % kFewStages], (t / kFewStages) & 1) && clock64() - t0 < kWaitLimitCycles) {
+      }
+    }
   } else if (warp == 4) {
-    mlc_key_warp<kFewTile, kFewKeyTiles>(p, item, tile0, n_tiles, n_idx, &s_slot[0][0], key_full, key_empty, abort_flag);
+    mlc_key_warp<kFewTile, kFewKeyTiles, kPrefetch>(p, item, tile0, n_tiles, n_idx, &s_slot[0][0], key_full, key_empty, abort_flag);
   } else if (warp == 5) {
     // ------------------------------------------------------------------ score MMAs
     constexpr uint32_t idesc_s = make_idesc(kFmtE4M3, kFmtE4M3, 128, 32);
@@ -189,7 +204,6 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p) {
       ok = __all_sync(0xffffffffu, mbar_wait(&kv_full[s], (t / kFewStages) & 1, abort_flag) &&
                                        mbar_wait(&s_empty[sb], ((t >> 1) & 1) ^ 1, abort_flag));
       if (!ok) break;
-      fence_proxy_async();               // the rows were copied through the generic proxy
       tc_fence_after();
       if (elect_one()) {
         const uint32_t d = tmem_base + kFewTmemS + sb * kFewSCols;
@@ -219,7 +233,6 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p) {
       ok = __all_sync(0xffffffffu, mbar_wait(&kv_full[s], (t / kFewStages) & 1, abort_flag) &&
                                        mbar_wait(p_full, t & 1, abort_flag));
       if (!ok) break;
-      fence_proxy_async();               // this warp's MMAs read the copied rows too
       tc_fence_after();
       if (elect_one()) {
         // 32 keys an MMA: four atoms of 8 keys x 128 dims, 1024 bytes apart
@@ -479,13 +492,31 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p) {
   if (tid == 0 && s_abort) atomicMax(p.status, kDevWaitTimeout);
 }
 
-cudaError_t mla_cached_few_launch(const MlaCachedParams& p, int device, cudaStream_t stream) {
+template <bool kPrefetch>
+static cudaError_t few_launch(const MlaCachedParams& p, const CUtensorMap& rows, int device, cudaStream_t stream) {
   static OncePerDevice once;
   cudaError_t e = once.run(device, [] {
-    return cudaFuncSetAttribute(sparse_mla_cached_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem);
+    return cudaFuncSetAttribute(sparse_mla_cached_few_kernel<kPrefetch>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem);
   });
   if (e != cudaSuccess) return e;
-  return launch_chained(sparse_mla_cached_few_kernel, dim3(p.n_items * p.splits), dim3(kFewThreads), kFewSmem, stream, p);
+  return launch_chained(sparse_mla_cached_few_kernel<kPrefetch>, dim3(p.n_items * p.splits), dim3(kFewThreads), kFewSmem,
+                        stream, p, rows);
+}
+
+cudaError_t mla_cached_few_launch(const MlaCachedParams& p, int device, cudaStream_t stream) {
+  PFN_encodeTiled enc = get_encode_tiled();
+  if (!enc) return cudaErrorNotSupported;
+  // the rows of all slots, in pieces of 128 bytes and the operands' swizzle
+  CUtensorMap rows;
+  const cuuint64_t dims[2] = {kLatentRowBytes, static_cast<cuuint64_t>(p.n_slots)}, pitch[1] = {kLatentRowBytes};
+  const cuuint32_t box[2] = {128, 1}, step[2] = {1, 1};
+  if (enc(&rows, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(p.cache), dims, pitch, box, step,
+          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return cudaErrorInvalidValue;
+  // Rows that several items of a request select are in L2 after the first of them: the prefetches would only take load slots
+  // (592 items of 148 requests 176 us without, 187 with; one item a request 54 without, 53 with, both before the gathers).
+  return p.n_items >= 4ll * p.n_requests ? few_launch<false>(p, rows, device, stream) : few_launch<true>(p, rows, device, stream);
 }
 
 }  // namespace b200dsa
