@@ -619,6 +619,7 @@ extern "C" int b200dsa_sparse_mla_decode_cached(const void* q_bf16, const void* 
   p.n_heads = n_heads;
   p.halves = n_heads > kMlaHeadsTile ? 2 : 1;
   p.splits = splits;
+  p.ahead = dev.sms;
   p.scale_log2 = sm_scale * 1.4426950408889634f;
   p.ctx = ctx;
   p.ctx_bf16 = ctx_bf16 != 0;

@@ -23,6 +23,7 @@ struct MlaCachedParams {
   const int64_t* tree_mask;      // nullable [n_items]
   const int32_t* tree_base;      // [n_requests] with tree_mask
   int n_items, n_heads, halves, splits;
+  int ahead;                     // CTAs that run at a time
   float scale_log2;
   void* ctx;
   int ctx_bf16;
@@ -122,6 +123,18 @@ __device__ __forceinline__ void mlc_key_warp(const MlaCachedParams& p, int item,
         asm volatile("prefetch.global.L2 [%0];" ::"l"(p.cache + static_cast<int64_t>(s) * kLatentRowBytes +
                                                      min((lane & 7) * 128, kLatentRowBytes - 1)));
     }
+  }
+  // With many items: the positions and queries of the CTA that takes this one's place, into L2 (2048 x 128 x 2048: 1750 ->
+  // 1721 us)
+  const int next = blockIdx.x + p.ahead;
+  if (!kPrefetch && next < gridDim.x) {
+    const int it = next / (p.splits * p.halves), h0 = next / p.splits % p.halves * kMlaHeadsTile;
+    const char* idx = reinterpret_cast<const char*>(p.indices + static_cast<int64_t>(it) * p.idx_stride);
+    for (int64_t b = lane * 128; b < static_cast<int64_t>(p.n_idx) * 4; b += 32 * 128)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(idx + b));
+    const char* q = reinterpret_cast<const char*>(p.q + (static_cast<int64_t>(it) * p.n_heads + h0) * kMlaD);
+    const int bytes = min(kMlaHeadsTile, p.n_heads - h0) * kMlaD * 2;
+    for (int b = lane * 128; b < bytes; b += 32 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + b));
   }
 }
 
