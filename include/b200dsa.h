@@ -685,7 +685,9 @@ int b200dsa_draft_tree_masks(const int32_t* parents, int32_t n_trees, int32_t n_
  *   An item without keys gives ctx = 0 and lse = -inf.  A key without a page or outside the cache, and an item whose
  *   request does not exist, are left out and reported (status 2).
  * splits (1..32): every item's keys are cut into that many runs, merged by a second kernel; the caller lends
- * splits * n_items * n_heads * 513 floats, which two calls in flight must not share.
+ * splits * n_items * n_heads * 513 floats, which two calls in flight must not share.  splits (-32..-2): the items whose
+ * CTAs (one, or two above 64 heads) fill whole waves of the multiprocessors stay whole and the others are cut into
+ * -splits runs, with a workspace for those: at most -splits * min(n_items, multiprocessors) * n_heads * 513 floats.
  * b200dsa_sparse_mla_decode_cached_splits is the number that fills the current device (1 = no workspace). */
 int b200dsa_sparse_mla_decode_cached_splits(int32_t n_items, int32_t n_heads, int32_t n_idx, int32_t tree);
 int b200dsa_sparse_mla_decode_cached(const void* q_bf16, const void* cache, int64_t n_slots, int32_t page_size,

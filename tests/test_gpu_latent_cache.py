@@ -588,3 +588,60 @@ def test_few_heads_long_cache_and_missing_rows_among_four():
     local = dict(cache=own, page=page, scale=0.05, table=torch.tensor([[0, 1]], dtype=torch.int32), q=q, idx=idx,
                  req=torch.zeros(n, dtype=torch.int32), qpos=torch.full((n,), 2 * page, dtype=torch.int32), mask=None)
     check_few(local, out, lse)
+
+
+@pytest.mark.parametrize("H,over,own,tree", [(16, 9, True, False), (16, 3, False, True), (8, 0, False, False),
+                                             (40, 5, True, False), (128, 3, False, False)])
+def test_items_behind_the_last_full_wave_are_cut_into_runs(H, over, own, tree):
+    """splits = -3: whole waves of items as splits = 1, the others as splits = 3, bit for bit; `own`: item i is request i."""
+    from transarch_b200 import kernels as K
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    whole = sms // 2 if H > 64 else sms
+    n = whole + over
+    c = attend_case(120 + H + over, n if own else 1, 1 if own else n, H, 400, 600, 32, drafts=7 if tree else 0)
+    if not tree:
+        c["qpos"].fill_(500)
+    if own:
+        c["req"] = None
+    limit = torch.randint(0, 401, (n,), generator=torch.Generator().manual_seed(H), dtype=torch.int32).to(DEV)
+    got = {}
+    for splits in (1, 3, -3):
+        ws = None if splits == 1 else torch.full((abs(splits) * n * H * 513,), float("nan"), device=DEV)
+        got[splits] = run_attend(c, workspace=(splits, ws), n_idx_item=limit)
+    assert _status() == 0
+    for x, a, b in zip(got[-3], got[1], got[3]):
+        assert torch.equal(x[:whole], a[:whole]) and torch.equal(x[whole:], b[whole:])
+    # a smaller call takes the same workspace, one that does not hold its runs is refused
+    splits, ws = K.sparse_mla_cached_workspace(n, H, 400, DEV, tree=tree)
+    small = {k: (v[:5] if k in ("q", "idx", "qpos", "req", "mask") and v is not None else v) for k, v in c.items()}
+    out, _ = run_attend(small, workspace=(splits, ws))
+    assert out.shape[0] == 5 and bool(torch.isfinite(out).all())
+    if over:
+        from transarch_b200._lib import B200DSAError
+        with pytest.raises(B200DSAError, match="workspace"):
+            run_attend(c, workspace=(-3, torch.empty(3 * over * H * 513 - 1, device=DEV)))
+
+
+def test_plan_of_items_behind_the_last_full_wave():
+    """192 items of 16 heads are more than one wave: planned, allocated and captured."""
+    from transarch_b200 import kernels as K
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    n = sms + 44
+    splits, ws = K.sparse_mla_cached_workspace(n, 16, 2048, DEV)
+    assert splits < -1 and ws.numel() <= -splits * n * 16 * 513
+    c = attend_case(140, 2, n // 2, 16, 2048, 2500, 64)
+    out, lse = run_attend(c)
+    held = run_attend(c, workspace=(splits, ws))
+    d = {k: (v.to(DEV) if isinstance(v, torch.Tensor) else v) for k, v in c.items()}
+    ctx, l2 = torch.zeros_like(out), torch.zeros_like(lse)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        K.sparse_mla_decode_cached(d["q"], d["cache"], 64, d["idx"], d["scale"], block_table=d["table"], row_request=d["req"],
+                                   q_pos=d["qpos"], ctx=ctx, lse=l2, workspace=(splits, ws))
+    for _ in range(2):
+        ctx.zero_()
+        graph.replay()
+        for a, b in ((held[0], out), (ctx, out), (held[1], lse), (l2, lse)):
+            assert torch.equal(a, b)
+    assert _status() == 0
+    check_few(c, out, lse, items=(0, 1, n // 2, n - 1))

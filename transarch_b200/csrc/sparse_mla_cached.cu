@@ -16,7 +16,9 @@
 // A tree is one more tile: its 64 keys are the drafted positions in order, its validity bits are the mask itself.
 //
 // Work split: CTA = (item, 64-head half, split).  Small batches cut an item's tiles into `splits` runs whose partial
-// contexts (normalised, fp32) and log-sum-exps are merged by mla_merge_kernel; large ones have splits = 1 and no merge.
+// contexts (normalised, fp32) and log-sum-exps are merged by mla_merge_kernel; large ones have splits = 1 and no merge,
+// or (splits < 0) cut only the items behind the last full wave, in a second launch: 80 x 128 x 2048 134 -> 99 us, 192 x 16 x 2048
+// 82 -> 71, 170 x 64 x 2048 139 -> 111.
 //
 // Roles (448 threads): warps 0-7 rows, warps 8-11 softmax, warp 12 MMAs, warp 13 keys: it turns positions into slots, up
 // to four tiles ahead of the rows, and has their bytes brought into L2 meanwhile.  (The row warps did that themselves at
@@ -527,6 +529,36 @@ static cudaError_t mlc_launch(const MlaCachedParams& p, int device, cudaStream_t
                         kMlaSmemBytes, stream, p);
 }
 
+// Items whose CTAs fill whole waves of the multiprocessors.
+static int whole_wave_items(int n_items, int n_heads, int sms) {
+  const int halves = n_heads > kMlaHeadsTile ? 2 : 1;
+  return static_cast<int>(static_cast<int64_t>(n_items) * halves / sms * sms / halves);
+}
+
+static cudaError_t mlc_run(const MlaCachedParams& p, bool prefetch, int device, cudaStream_t stream) {
+  if (p.n_items == 0) return cudaSuccess;
+  // Up to 16 heads the codes are multiplied as they are: 148 items x 2048 keys take 49 us for 16 heads, and 77 us for 17,
+  // which the kernel for 64 heads does (it takes the same time for 1 head as for 64).
+  cudaError_t e;
+  if (p.n_heads <= kMlcFewHeads) e = mla_cached_few_launch(p, prefetch, device, stream);
+  else e = prefetch ? mlc_launch<true>(p, device, stream) : mlc_launch<false>(p, device, stream);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess || p.splits == 1) return e;
+  // the merge becomes resident while the attention drains (it waits for it inside)
+  const int rows = p.n_items * p.n_heads;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(rows));
+  cfg.blockDim = dim3(128);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, mla_merge_kernel, static_cast<const float*>(p.part), rows, p.splits, p.ctx, p.ctx_bf16, p.lse);
+  return e == cudaSuccess ? cudaGetLastError() : e;
+}
+
 static int mlc_rc(cudaError_t e) {
   if (e == cudaSuccess) return B200DSA_OK;
   set_last_error(cudaGetErrorString(e));
@@ -561,6 +593,19 @@ extern "C" int b200dsa_sparse_mla_decode_cached_splits(int32_t n_items, int32_t 
       best = s;
     }
   }
+  // Items that would start one more, mostly empty wave can be a launch of their own, cut into runs, while those of the full
+  // waves stay whole (192 items x 16 heads on 148 SMs: 148 whole, 44 in three runs).
+  const int rest = n_items - whole_wave_items(n_items, n_heads, dev.sms);
+  for (int s = 2; rest > 0 && rest < n_items && s <= kMlcMaxSplits && s <= tiles; ++s) {
+    const int64_t rest_ctas = static_cast<int64_t>(rest) * (n_heads > kMlaHeadsTile ? 2 : 1);
+    const double cost = static_cast<double>(ctas / dev.sms) * (tiles * tile_clocks + 23000.0) +
+                        static_cast<double>((rest_ctas * s + dev.sms - 1) / dev.sms) * ((tiles + s - 1) / s * tile_clocks + 23000.0) +
+                        6000.0 + 2.0 * s * rest * n_heads + 4000.0;
+    if (cost * 1.03 < least) {
+      least = cost * 1.03;
+      best = -s;
+    }
+  }
   return best;
 }
 
@@ -577,26 +622,28 @@ extern "C" int b200dsa_sparse_mla_decode_cached(const void* q_bf16, const void* 
   if (!q_bf16 || !cache || !block_table || (!indices && n_idx > 0) || !ctx || !lse || !status || n_items < 0 ||
       n_heads < 1 || n_heads > kMlaMaxHeads || n_idx < 0 || n_idx > (1 << 30) || idx_stride < n_idx || n_slots < 1 ||
       n_slots > 0x7fffffffll || page_size < 1 || table_cols < 1 || table_stride < table_cols || n_requests < 1 ||
-      (!row_request && n_requests < n_items) || !(sm_scale > 0.f) || (tree_mask && !tree_base) || splits < 1 || splits > kMlcMaxSplits ||
-      static_cast<int64_t>(n_items) * 2 * splits > 0x7fffffffll) {
-    set_last_error("b200dsa_sparse_mla_decode_cached: bad argument (1 <= n_heads <= 128, 1 <= splits <= 32, "
+      (!row_request && n_requests < n_items) || !(sm_scale > 0.f) || (tree_mask && !tree_base) || splits < -kMlcMaxSplits ||
+      splits == 0 || splits == -1 || splits > kMlcMaxSplits || static_cast<int64_t>(n_items) * 2 * kMlcMaxSplits > 0x7fffffffll) {
+    set_last_error("b200dsa_sparse_mla_decode_cached: bad argument (1 <= n_heads <= 128, 1 <= splits <= 32 or -32 <= splits <= -2, "
                    "idx_stride >= n_idx, sm_scale > 0, a request for every item)");
     return B200DSA_EINVAL;
   }
-  const int64_t rows = static_cast<int64_t>(n_items) * n_heads;
-  if (splits > 1 && (!workspace || workspace_bytes < rows * splits * (kMlaDv + 1) * 4)) {
-    set_last_error("b200dsa_sparse_mla_decode_cached: the workspace is smaller than splits * n_items * n_heads * 513 floats");
+  DeviceInfo dev;
+  cudaError_t e = current_device_info(&dev);
+  if (e != cudaSuccess) return mlc_rc(e);
+  // splits < 0: the items of full waves whole, the others in -splits runs
+  const int whole = splits == 1 ? n_items : splits < 0 ? whole_wave_items(n_items, n_heads, dev.sms) : 0;
+  const int runs = splits < 0 ? -splits : splits;
+  const int64_t rows = static_cast<int64_t>(n_items - whole) * n_heads;
+  if (rows > 0 && (!workspace || workspace_bytes < rows * runs * (kMlaDv + 1) * 4)) {
+    set_last_error("b200dsa_sparse_mla_decode_cached: the workspace is smaller than 513 floats for every run of every head");
     return B200DSA_EINVAL;
   }
   if ((reinterpret_cast<uintptr_t>(q_bf16) & 15) || (reinterpret_cast<uintptr_t>(cache) & 15) ||
-      (reinterpret_cast<uintptr_t>(ctx) & 15) || (splits > 1 && (reinterpret_cast<uintptr_t>(workspace) & 15))) {
+      (reinterpret_cast<uintptr_t>(ctx) & 15) || (rows > 0 && (reinterpret_cast<uintptr_t>(workspace) & 15))) {
     set_last_error("b200dsa_sparse_mla_decode_cached: q, cache, ctx and workspace must be 16-byte aligned");
     return B200DSA_EALIGN;
   }
-  DeviceInfo dev;
-  cudaError_t e = current_device_info(&dev);
-  const bool few = n_heads <= kMlcFewHeads;
-  if (e != cudaSuccess) return mlc_rc(e);
   MlaCachedParams p{};
   p.q = static_cast<const __nv_bfloat16*>(q_bf16);
   p.cache = static_cast<const uint8_t*>(cache);
@@ -618,7 +665,7 @@ extern "C" int b200dsa_sparse_mla_decode_cached(const void* q_bf16, const void* 
   p.n_items = n_items;
   p.n_heads = n_heads;
   p.halves = n_heads > kMlaHeadsTile ? 2 : 1;
-  p.splits = splits;
+  p.splits = runs;
   p.ahead = dev.sms;
   p.scale_log2 = sm_scale * 1.4426950408889634f;
   p.ctx = ctx;
@@ -626,28 +673,30 @@ extern "C" int b200dsa_sparse_mla_decode_cached(const void* q_bf16, const void* 
   p.lse = lse;
   p.part = static_cast<float*>(workspace);
   p.status = status;
-  // Up to 16 heads the codes are multiplied as they are: 148 items x 2048 keys take 49 us for 16 heads, and 77 us for 17,
-  // which the kernel for 64 heads does (it takes the same time for 1 head as for 64).
   // Rows that several items of a request select are in L2 after the first of them; prefetches then only take load slots (2048
   // items of one request 1788 us with, 1748 without; one item a request 71.7 with, 78.7 without).
+  const bool prefetch = n_items < 4ll * n_requests;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (few) e = mla_cached_few_launch(p, dev.index, st);
-  else e = n_items >= 4ll * n_requests ? mlc_launch<false>(p, dev.index, st) : mlc_launch<true>(p, dev.index, st);
-  if (e == cudaSuccess) e = cudaGetLastError();
-  if (e == cudaSuccess && splits > 1) {
-    // the merge becomes resident while the attention drains (it waits for it inside)
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(rows));
-    cfg.blockDim = dim3(128);
-    cfg.stream = static_cast<cudaStream_t>(stream);
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, mla_merge_kernel, static_cast<const float*>(p.part), static_cast<int>(rows),
-                           static_cast<int>(splits), ctx, static_cast<int>(ctx_bf16 != 0), lse);
-    if (e == cudaSuccess) e = cudaGetLastError();
+  MlaCachedParams first = p;
+  first.n_items = whole;
+  first.splits = 1;
+  e = mlc_run(first, prefetch, dev.index, st);
+  if (e != cudaSuccess) return mlc_rc(e);
+  p.n_items -= whole;
+  p.q += static_cast<int64_t>(whole) * n_heads * kMlaD;
+  if (p.indices) p.indices += whole * idx_stride;
+  if (p.n_idx_item) p.n_idx_item += whole;
+  if (p.q_pos) p.q_pos += whole;
+  if (p.tree_mask) p.tree_mask += whole;
+  if (p.row_request) {
+    p.row_request += whole;
+  } else {                     // item i is request i
+    p.table += whole * table_stride;
+    p.n_requests -= whole;
+    if (p.tree_base) p.tree_base += whole;
   }
+  p.ctx = static_cast<uint8_t*>(ctx) + static_cast<int64_t>(whole) * n_heads * kMlaDv * (ctx_bf16 ? 2 : 4);
+  p.lse += static_cast<int64_t>(whole) * n_heads;
+  e = mlc_run(p, prefetch, dev.index, st);
   return mlc_rc(e);
 }

@@ -503,7 +503,7 @@ static cudaError_t few_launch(const MlaCachedParams& p, const CUtensorMap& rows,
                         stream, p, rows);
 }
 
-cudaError_t mla_cached_few_launch(const MlaCachedParams& p, int device, cudaStream_t stream) {
+cudaError_t mla_cached_few_launch(const MlaCachedParams& p, bool prefetch, int device, cudaStream_t stream) {
   PFN_encodeTiled enc = get_encode_tiled();
   if (!enc) return cudaErrorNotSupported;
   // the rows of all slots, in pieces of 128 bytes and the operands' swizzle
@@ -514,9 +514,8 @@ cudaError_t mla_cached_few_launch(const MlaCachedParams& p, int device, cudaStre
           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return cudaErrorInvalidValue;
-  // Rows that several items of a request select are in L2 after the first of them: the prefetches would only take load slots
-  // (592 items of 148 requests 176 us without, 187 with; one item a request 54 without, 53 with, both before the gathers).
-  return p.n_items >= 4ll * p.n_requests ? few_launch<false>(p, rows, device, stream) : few_launch<true>(p, rows, device, stream);
+  // 592 items of 148 requests: 176 us without prefetches, 187 with
+  return prefetch ? few_launch<true>(p, rows, device, stream) : few_launch<false>(p, rows, device, stream);
 }
 
 }  // namespace b200dsa

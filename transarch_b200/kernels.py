@@ -1138,12 +1138,25 @@ def draft_tree_masks(parents: torch.Tensor) -> torch.Tensor:
     return masks
 
 
+_sm_counts = {}
+
+
+def _cached_parts(splits: int, n_items: int, n_heads: int, index: int) -> int:
+    """Floats of workspace that `splits` needs for calls of at most n_items items on device `index`."""
+    if splits < 0:                       # only the items behind the last full wave of multiprocessors are cut into runs
+        if index not in _sm_counts:
+            _sm_counts[index] = torch.cuda.get_device_properties(index).multi_processor_count
+        n_items = min(n_items, _sm_counts[index])
+    return 0 if splits == 1 else abs(splits) * n_items * n_heads * 513
+
+
 def sparse_mla_cached_workspace(n_items: int, n_heads: int, n_idx: int, device, *, tree: bool = False):
     """(splits, workspace or None) that sparse_mla_decode_cached takes for calls of at most this size on `device`; keep
     one for each call that may be in flight at a time."""
     with torch.cuda.device(device):
         splits = _lib.load().b200dsa_sparse_mla_decode_cached_splits(n_items, n_heads, n_idx, tree)
-        ws = None if splits == 1 else torch.empty(splits * n_items * n_heads * 513, dtype=torch.float32, device=device)
+        parts = _cached_parts(splits, n_items, n_heads, torch.cuda.current_device())
+        ws = torch.empty(parts, dtype=torch.float32, device=device) if parts else None
     return splits, ws
 
 
@@ -1206,10 +1219,10 @@ def sparse_mla_decode_cached(q: torch.Tensor, cache: torch.Tensor, page_size: in
     lib = _lib.load()
     if workspace is None:
         splits = lib.b200dsa_sparse_mla_decode_cached_splits(n, H, n_idx, tree_mask is not None)
-        if splits > 1:
-            ws = torch.empty(splits * n * H * 513, dtype=torch.float32, device=q.device)
-    elif splits > 1 and (ws is None or ws.dtype != torch.float32 or not ws.is_contiguous() or
-                         ws.numel() < splits * n * H * 513):
+        if splits != 1:
+            ws = torch.empty(_cached_parts(splits, n, H, index), dtype=torch.float32, device=q.device)
+    elif splits != 1 and (ws is None or ws.dtype != torch.float32 or not ws.is_contiguous() or
+                          (splits > 1 and ws.numel() < splits * n * H * 513)):
         raise _lib.B200DSAError("the workspace is smaller than splits * n_items * n_heads * 513 floats")
     check(lib.b200dsa_sparse_mla_decode_cached(
         q.data_ptr(), cache.data_ptr(), n_slots, page_size, block_table.data_ptr(), stride, cols, R, ptr(row_request),
