@@ -628,9 +628,9 @@ extern "C" int b200dsa_sparse_mla_decode_cached(const void* q_bf16, const void* 
                    "idx_stride >= n_idx, sm_scale > 0, a request for every item)");
     return B200DSA_EINVAL;
   }
-  DeviceInfo dev;
-  cudaError_t e = current_device_info(&dev);
-  if (e != cudaSuccess) return mlc_rc(e);
+  DeviceInfo dev{};
+  cudaError_t e = cudaSuccess;
+  if (splits < 0 && (e = current_device_info(&dev)) != cudaSuccess) return mlc_rc(e);
   // splits < 0: the items of full waves whole, the others in -splits runs
   const int whole = splits == 1 ? n_items : splits < 0 ? whole_wave_items(n_items, n_heads, dev.sms) : 0;
   const int runs = splits < 0 ? -splits : splits;
@@ -644,6 +644,7 @@ extern "C" int b200dsa_sparse_mla_decode_cached(const void* q_bf16, const void* 
     set_last_error("b200dsa_sparse_mla_decode_cached: q, cache, ctx and workspace must be 16-byte aligned");
     return B200DSA_EALIGN;
   }
+  if (splits > 0 && (e = current_device_info(&dev)) != cudaSuccess) return mlc_rc(e);
   MlaCachedParams p{};
   p.q = static_cast<const __nv_bfloat16*>(q_bf16);
   p.cache = static_cast<const uint8_t*>(cache);
