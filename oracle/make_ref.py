@@ -47,8 +47,8 @@ FILES = [
 
 
 def make_ref(reference_root: str = DEFAULT_ROOT) -> bool:
-    """Copy the files; returns False (and leaves oracle/_ref/ as it is) when the checkout is absent."""
-    if not os.path.isdir(reference_root):
+    """Copy the files; returns False (and leaves oracle/_ref/ as it is) when the checkout is absent or empty."""
+    if not os.path.isfile(os.path.join(reference_root, FILES[0][0])):
         return False
     for src, dst in FILES:
         s = os.path.join(reference_root, src)
