@@ -1,0 +1,86 @@
+"""Attention over the quantised latent cache where probabilities and scales span many powers of two: one key that holds
+nearly all of a head's probability over a broad tail (an attention sink), groups of dims whose scales lie far apart.
+
+Bounds: check_attend's (a probability is off by at most a bf16 half step, 2^-8 of itself, however small it is), and for
+the queries, which up to 16 heads are two e4m3 numbers, 2^-18 of a row's largest latent value."""
+import pytest
+import torch
+
+from oracle import latent_oracle as L
+from tests.test_gpu_latent_cache import BF16, DEV, F32, _status, run_attend
+
+pytestmark = pytest.mark.gpu
+QUERY = 2.0 ** -18
+
+
+def check_range(c, ctx, lse, items, query=QUERY):
+    """Every item of `items` against the 64-bit definition."""
+    for i in items:
+        slots = L.item_keys(c["idx"][i], c["table"][int(c["req"][i])], c["page"], int(c["qpos"][i]))
+        rows, q = L.cache_rows(c["cache"], slots), c["q"][i].double()
+        ref, ref_lse, mass, qk = L.attend(q, rows, c["scale"])
+        k = slots.numel()
+        q_off = query * q[:, :512].abs().amax(1) * rows[:, :512].abs().sum(1).max() * c["scale"] * (q.shape[0] <= 16)
+        d = (576 * F32 * qk + q_off).view(-1, 1) + 1e-6           # error of a score; exp of it is relative
+        step = BF16 if ctx.dtype == torch.bfloat16 else F32
+        bound = (BF16 + 2 * d + k * F32) * mass + step * ref.abs() + 1e-30
+        got = ctx[i].double().cpu()
+        assert bool(((got - ref).abs() <= bound).all()), (i, float(((got - ref).abs() / bound).max()))
+        lim = d.view(-1) + k * F32 + 8 * F32 * ref_lse.abs() + 2e-7
+        assert bool(((lse[i].double().cpu() - ref_lse).abs() <= lim).all())
+
+
+def range_case(seed, H, nats, at, k=2048, items=1, scales=(0, 0, 0, 0)):
+    """k keys whose codes share a mean, their scores decided by the first position dim: key number `at` of the list lies
+    `nats` above the others, which are within one of each other.  scales: powers of two of the four groups."""
+    g = torch.Generator().manual_seed(seed)
+    page = 64
+    pages = (k + page - 1) // page
+    cache = torch.zeros(pages * page, 656, dtype=torch.uint8)
+    codes = (torch.randn(k, 512, generator=g) * 40 + 90).clamp(-448, 448)
+    cache[:k, :512] = codes.to(torch.float8_e4m3fn).view(torch.uint8)
+    cache[:k, 512:528] = torch.exp2(torch.tensor(scales).float() - 7).repeat(k, 1).view(torch.uint8)
+    pe = torch.zeros(k, 64)
+    pe[:, 0] = torch.rand(k, generator=g)
+    order = torch.randperm(k, generator=g)
+    pe[order[at], 0] = nats + 0.5
+    cache[:k, 528:] = pe.bfloat16().view(torch.uint8)
+    q = 2.0 ** -6 * torch.randn(items, H, 576, generator=g)
+    q[:, :, 512:] = 0
+    q[:, :, 512] = 16                                              # times 1/16: nats
+    return {"cache": cache, "page": page, "scale": 1 / 16, "table": torch.arange(pages, dtype=torch.int32).view(1, -1),
+            "q": q.bfloat16(), "req": torch.zeros(items, dtype=torch.int32), "idx": order.to(torch.int32).repeat(items, 1),
+            "qpos": torch.full((items,), k, dtype=torch.int32), "lens": torch.tensor([k]), "mask": None}
+
+
+@pytest.mark.parametrize("H", [1, 8, 16, 17])
+@pytest.mark.parametrize("nats", [6.0, 8.0, 9.5, 10.0, 12.0, 15.0])
+def test_one_key_over_a_broad_tail(H, nats):
+    """In the first and in the last tile of the list, one CTA an item and several; 17 heads take the other kernel."""
+    for at in (3, 2045):
+        c = range_case(int(nats * 2) + H + at, H, nats, at)
+        for splits in (1, 5):
+            ws = (splits, torch.empty(splits * H * 513, device=DEV) if splits > 1 else None)
+            out, lse = run_attend(c, ctx=torch.empty(1, H, 512, device=DEV), workspace=ws)
+            check_range(c, out, lse, [0])
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("scales", [(0, -6, -8, -14), (-8, 0, 0, -6), (3, -3, -11, 0)])
+@pytest.mark.parametrize("H", [1, 8, 16])
+def test_groups_of_uneven_scales(H, scales):
+    """A group keeps its precision whatever the scales of the others."""
+    for nats, at in ((0.0, 0), (9.5, 1000)):
+        c = range_case(31 + H, H, nats, at, k=1500, scales=scales)
+        out, lse = run_attend(c, ctx=torch.empty(1, H, 512, device=DEV), workspace=(1, None))
+        check_range(c, out, lse, [0])
+    assert _status() == 0
+
+
+def test_tail_in_items_behind_the_last_full_wave():
+    """Whole items and items cut into runs in one call, the default result type."""
+    n = torch.cuda.get_device_properties(0).multi_processor_count + 3
+    c = range_case(77, 16, 10.0, 600, k=700, items=n)
+    out, lse = run_attend(c, workspace=(-3, torch.empty(3 * 3 * 16 * 513, device=DEV)))
+    assert _status() == 0
+    check_range(c, out, lse, [0, 1, n - 4, n - 3, n - 1])

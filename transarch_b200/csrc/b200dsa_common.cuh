@@ -172,7 +172,8 @@ __device__ __forceinline__ void mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uin
 // Instruction descriptor (32 bit): dense, fp32 accumulate, both operands K-major unless flagged.
 //   [4,6) D format (1 = f32)   [7,10) A format   [10,13) B format
 //   [15] A MN-major   [16] B MN-major   [17,23) N>>3   [24,29) M>>4
-constexpr uint32_t kFmtE4M3 = 0;  // kind::f8f6f4
+constexpr uint32_t kFmtE4M3 = 0;  // kind::f8f6f4; its operands' formats may differ
+constexpr uint32_t kFmtE5M2 = 1;  // kind::f8f6f4
 constexpr uint32_t kFmtBF16 = 1;  // kind::f16
 __host__ __device__ constexpr uint32_t make_idesc(uint32_t fmt_a, uint32_t fmt_b, uint32_t M, uint32_t N,
                                                   uint32_t a_mn_major = 0, uint32_t b_mn_major = 0) {

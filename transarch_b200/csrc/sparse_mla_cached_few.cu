@@ -7,13 +7,18 @@
 //   S^T_g [128 keys x 32]  = K_g [128 x 128 dims, e4m3] * (Q_hi | Q_lo)_g      for each group g of 128 dims
 //   R^T   [128 keys x 16]  = K_pe [128 x 64, bf16] * Q_pe
 //   s[key, h] = q_scale[h] * sum_g scale_g[key] * (S_hi + S_lo) + R            one thread a key: its scales are its own
-//   p = 2^(s - m[h]),   P_g = 16 p * scale_g / ref as hi + lo                for each group, because the scales of V differ by group
-//   O^T_g [128 dims x 32] += V_g^T [128 dims x 128 keys, the same bytes read MN-major] * (P_hi | P_lo)_g
+//   p = 2^(s - m[h]),   P_g = 2^10 p * scale_g / ref in three terms          for each group, because the scales of V differ by group
+//   O^T_g [128 dims x 48] += V_g^T [128 dims x 128 keys, the same bytes read MN-major] * (P_0 | P_1 | P_2)_g
 //
-// An 8-bit number has four significant bits, a bf16 number eight: q over a power of two and p are split into two e4m3
-// numbers, hi = e4m3(x) and lo = e4m3(x - hi), so that the products carry bf16's precision down to 2^-17 of the largest
-// value; hi and lo stand side by side in N and are added in fp32.  The position dims stay bf16.  A tile of 128 keys
-// takes 36 MMAs of at most 32 columns, where two tiles of the other kernel take 88 and 128 widened rows.
+// q over a power of two that brings a row's largest latent value below 448 is hi = e4m3(q) and lo = e4m3(q - hi): eight
+// bits, as bf16 has, and off by at most 2^-18 of the largest value.  Probabilities need more range: thousands of keys
+// that hold 2^-17 of the largest one's each are a share of the result.  P is t0 + t1 / 16 + t2 / 256 in e5m2,
+//   t0 = e5m2(P),  t1 = e5m2(16 (P - t0)),  t2 = e5m2(16 (16 (P - t0) - t1)),
+// each rounding off by 2^-3 of what it rounds: three leave 2^-9 of P, half of a bf16 rounding's 2^-8, as long as t2 is a normal
+// number, and never more than 2^-25 (half of e5m2's smallest step, 2^-17, over 256).  P stays below 2^15, so that a rest, at
+// most 2^11, times 16 does too.  (Two e4m3 terms of one unit lost everything below 2^-14 of the largest probability.)  The terms stand
+// side by side in N and are added in fp32.  The position dims stay bf16.  A tile of 128 keys takes 36 MMAs of at
+// most 48 columns, where two tiles of the other kernel take 88 and 128 widened rows.
 //
 // The running maximum m[h] and the reference scale ref (a power of two) are common to the CTA; they are renewed, and O and
 // the sums rescaled, when a score exceeds m by 4.5 (base 2) or a scale exceeds ref.
@@ -41,15 +46,20 @@ constexpr int kFewPeOff = 4 * kFewGroupBytes;                       // 128 keys 
 constexpr int kFewScaleOff = kFewPeOff + kFewTile * 128;            // 128 keys x 4 fp32
 constexpr int kFewStageBytes = kFewScaleOff + kFewTile * 16;
 static_assert(kFewStageBytes % 1024 == 0, "stages start on swizzle atoms");
-constexpr int kFewPOff = kFewStages * kFewStageBytes;               // 4 groups x 32 rows (hi, lo) x 128 keys
-constexpr int kFewQOff = kFewPOff + 4 * 32 * 128;                   // 4 groups x 32 rows (hi, lo) x 128 dims
+constexpr int kFewTerms = 3;                                        // e5m2 terms of a probability
+constexpr int kFewPOctet = kFewTerms * 128;                         // 8 keys x 16 heads a term
+constexpr int kFewPGroup = kFewTile / 8 * kFewPOctet;
+constexpr int kFewPOff = kFewStages * kFewStageBytes;               // 4 groups x 16 octets of keys
+constexpr int kFewQOff = kFewPOff + 4 * kFewPGroup;                 // 4 groups x 32 rows (hi, lo) x 128 dims
 constexpr int kFewQpeOff = kFewQOff + 4 * 32 * 128;                 // 16 rows x 64 bf16
 constexpr int kFewBarOff = kFewQpeOff + 16 * 128;
 constexpr int kFewSmem = kFewBarOff + 256 + 1024;
-constexpr uint32_t kFewTmemS = 128;                                 // O in columns 0..127, two score buffers of 144 behind
+constexpr uint32_t kFewOCols = kFewTerms * 16;                      // O of a group
+constexpr uint32_t kFewTmemS = 4 * kFewOCols;                       // two score buffers of 144 columns behind O
 constexpr uint32_t kFewSCols = 144;                                 // 4 groups x (16 hi + 16 lo), 16 position products
-constexpr float kFewLift = 16.0f;                                   // P = 16 p: probabilities down to 2^-13 keep a digit,
-constexpr float kFewHeadroom = 4.5f;                                // and 16 * 2^4.5 = 362 is the largest P (e4m3 ends at 448)
+static_assert(kFewTmemS + 2 * kFewSCols <= 512, "O and two score buffers");
+constexpr float kFewLift = 1024.0f;                                 // P = 2^10 p scale / ref,
+constexpr float kFewHeadroom = 4.5f;                                // at most 2^14.5
 
 __device__ __align__(16) uint8_t g_few_zero[16];
 
@@ -78,6 +88,15 @@ __device__ __forceinline__ void split_e4m3x2(float a, float b, uint32_t& hi, uin
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(hi), __NV_E4M3);
   const float2 f = __half22float2(__half2(h));
   lo = __nv_cvt_float2_to_fp8x2(make_float2(a - f.x, b - f.y), __NV_SATFINITE, __NV_E4M3);
+}
+// The next e5m2 term of a and b; they become 16 times what it leaves.
+__device__ __forceinline__ uint32_t term_e5m2x2(float& a, float& b) {
+  const uint32_t t = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E5M2);
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(t), __NV_E5M2);
+  const float2 f = __half22float2(__half2(h));
+  a = (a - f.x) * 16.0f;
+  b = (b - f.y) * 16.0f;
+  return t;
 }
 
 template <bool kPrefetch>
@@ -226,7 +245,7 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p, const __grid_constant__ CU
   } else if (warp == 6) {
     // ------------------------------------------------------------------ value MMAs.  A warp of their own: behind S(t+1) in
     // one warp's order they would wait for the rows of tile t+1, which wait for the stage that these MMAs free.
-    constexpr uint32_t idesc_pv = make_idesc(kFmtE4M3, kFmtE4M3, 128, 32, 1, 1);     // both read MN-major: dims x keys x heads
+    constexpr uint32_t idesc_pv = make_idesc(kFmtE4M3, kFmtE5M2, 128, kFewOCols, 1, 1);   // both read MN-major: dims x keys x heads
     bool ok = true;
     for (int t = 0; ok && t < n_tiles; ++t) {
       const int s = t % kFewStages;
@@ -237,14 +256,14 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p, const __grid_constant__ CU
       if (elect_one()) {
         // 32 keys an MMA: four atoms of 8 keys x 128 dims, 1024 bytes apart
         const uint64_t v0 = make_desc_mn_sw128(smem_base + s * kFewStageBytes, kFewGroupBytes, 1024);
-        // P without swizzle: 128 bytes between core matrices along the heads, 256 along the keys
-        const uint64_t p0 = make_desc_k_noswz(smem_base + kFewPOff, 256, 128);
+        // P without swizzle: 128 bytes between core matrices along the heads and terms, kFewPOctet along the keys
+        const uint64_t p0 = make_desc_k_noswz(smem_base + kFewPOff, kFewPOctet, 128);
 #pragma unroll
         for (int g = 0; g < 4; ++g)
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
-            mma_f8f6f4_ss(tmem_base + g * 32, v0 + ((g * kFewGroupBytes + kk * 4096) >> 4), p0 + ((g * 4096 + kk * 1024) >> 4),
-                          idesc_pv, (t | kk) != 0);
+            mma_f8f6f4_ss(tmem_base + g * kFewOCols, v0 + ((g * kFewGroupBytes + kk * 4096) >> 4),
+                          p0 + ((g * kFewPGroup + kk * 4 * kFewPOctet) >> 4), idesc_pv, (t | kk) != 0);
         tc_commit(&kv_empty[s]);
         tc_commit(pv_done);
       }
@@ -397,7 +416,7 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p, const __grid_constant__ CU
             ok = __all_sync(0xffffffffu, mbar_wait(pv_done, (t - 1) & 1, abort_flag));
             tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < 8; ++c) {                   // group c / 2, hi or lo
+            for (int c = 0; c < 4 * kFewTerms; ++c) {       // the terms of every group
               float o[8];
               const uint32_t at = tmem_base + lane_addr + c * 16 + hb;
               few_ld8(at, o);
@@ -412,7 +431,7 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p, const __grid_constant__ CU
         } else if (t > 0) {
           ok = __all_sync(0xffffffffu, mbar_wait(pv_done, (t - 1) & 1, abort_flag));    // P is free
         }
-        // P of group g, MN-major: core matrices of 8 keys x 16 bytes, hi and lo of the 16 heads side by side.  (Stored
+        // P of group g, MN-major: core matrices of 8 keys x 16 bytes, the terms of the 16 heads side by side.  (Stored
         // K-major, one byte a store, it took 64 stores a thread.)
         float pr[8];
 #pragma unroll
@@ -422,17 +441,21 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p, const __grid_constant__ CU
           l[j] += e;
           pr[j] = e * kFewLift;
         }
-        const uint32_t row = smem_base + kFewPOff + (key >> 3) * 256 + (key & 7) * 16 + hb;
+        const uint32_t row = smem_base + kFewPOff + (key >> 3) * kFewPOctet + (key & 7) * 16 + hb;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const float w = valid ? sc[g] * inv_ref : 0.f;
-          uint32_t h2[4], l2[4];
+          float x[8];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) split_e4m3x2(pr[2 * j] * w, pr[2 * j + 1] * w, h2[j], l2[j]);
-          asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(row + g * 4096), "r"(h2[0] | h2[1] << 16),
-                       "r"(h2[2] | h2[3] << 16) : "memory");
-          asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(row + g * 4096 + 128), "r"(l2[0] | l2[1] << 16),
-                       "r"(l2[2] | l2[3] << 16) : "memory");
+          for (int j = 0; j < 8; ++j) x[j] = pr[j] * w;
+#pragma unroll
+          for (int c = 0; c < kFewTerms; ++c) {
+            uint32_t t2[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) t2[j] = term_e5m2x2(x[2 * j], x[2 * j + 1]);
+            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(row + g * kFewPGroup + c * 128), "r"(t2[0] | t2[1] << 16),
+                         "r"(t2[2] | t2[3] << 16) : "memory");
+          }
         }
         fence_proxy_async();
         mbar_arrive(p_full);
@@ -466,17 +489,18 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p, const __grid_constant__ CU
       }
 #pragma unroll 1
       for (int g = 0; g < 4; ++g) {
-        float a[8], b[8];
+        float a[8], b[8], c[8];
         if (n_tiles > 0) {
-          few_ld8(tmem_base + lane_addr + g * 32 + hb, a);
-          few_ld8(tmem_base + lane_addr + g * 32 + 16 + hb, b);
+          few_ld8(tmem_base + lane_addr + g * kFewOCols + hb, a);
+          few_ld8(tmem_base + lane_addr + g * kFewOCols + 16 + hb, b);
+          few_ld8(tmem_base + lane_addr + g * kFewOCols + 32 + hb, c);
           tc_wait_ld();
         }
         const int dim = g * 128 + key;                      // the lane is a dim of the group here
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           if (hb + j >= p.n_heads) continue;
-          const float v = k[j] != 0.f ? (a[j] + b[j]) * k[j] : 0.f;
+          const float v = k[j] != 0.f ? fmaf(fmaf(c[j], 1.0f / 16, b[j]), 1.0f / 16, a[j]) * k[j] : 0.f;
           if (p.splits > 1) p.part[(split * parts + row0 + j) * kMlaDv + dim] = v;
           else if (p.ctx_bf16) static_cast<__nv_bfloat16*>(p.ctx)[(row0 + j) * kMlaDv + dim] = __float2bfloat16_rn(v);
           else static_cast<float*>(p.ctx)[(row0 + j) * kMlaDv + dim] = v;
