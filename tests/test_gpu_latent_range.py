@@ -84,3 +84,60 @@ def test_tail_in_items_behind_the_last_full_wave():
     out, lse = run_attend(c, workspace=(-3, torch.empty(3 * 3 * 16 * 513, device=DEV)))
     assert _status() == 0
     check_range(c, out, lse, [0, 1, n - 4, n - 3, n - 1])
+
+
+@pytest.mark.parametrize("ratio,nats", [(8, 12.0), (14, 12.0), (14, 30.0), (30, 30.0), (40, 60.0)])
+@pytest.mark.parametrize("H", [1, 16])
+def test_a_key_of_large_scales_and_no_weight(H, ratio, nats):
+    """A key whose scales are 2^ratio times the others' but whose probability is e^-nats of theirs: its latent dims and the
+    queries' do not meet, so that its score is the position dims' alone."""
+    for at in (0, 700, 1499):
+        c = range_case(90 + H + at, H, 2.0, (at + 5) % 1500, k=1500)
+        lone = int(c["idx"][0, at])
+        row = c["cache"][lone]
+        row[512:528] = torch.full((4,), 2.0 ** (ratio - 7)).view(torch.uint8)
+        row[:512:2] = 0                                           # the odd latent dims hold its values,
+        c["q"][:, :, 1:512:2] = 0                                 # the even ones the queries'
+        row[528:] = 0
+        row[528:530] = torch.tensor([-nats], dtype=torch.bfloat16).view(torch.uint8)
+        for splits in (1, 4):
+            ws = (splits, torch.empty(splits * H * 513, device=DEV) if splits > 1 else None)
+            out, lse = run_attend(c, ctx=torch.empty(1, H, 512, device=DEV), workspace=ws)
+            check_range(c, out, lse, [0], query=0)
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("H", [3, 16])
+def test_scores_and_scales_that_grow_in_turn(H):
+    """Tile by tile the score, or one group's scale by any factor, takes the lead: references of heads and groups are renewed
+    at different times; then the same keys in falling order."""
+    g = torch.Generator().manual_seed(H)
+    k = 1280
+    c = range_case(5 + H, H, 0.0, 0, k=k)
+    tile = torch.arange(k) // 128
+    up = torch.stack([tile * 3 % 7 - 9, tile - 12, -2 * tile, (tile % 2) * 9 - 14], 1).float()
+    c["cache"][:k, 512:528] = torch.exp2(up).view(torch.uint8)
+    pe = torch.zeros(k, 64)
+    pe[:, 0] = tile * 1.5 + torch.rand(k, generator=g)
+    pe[:, 1] = -tile.float()                                      # for the heads that look there scores fall
+    c["cache"][:k, 528:] = pe.bfloat16().view(torch.uint8)
+    c["q"][:, 1::2, 512], c["q"][:, 1::2, 513] = 0, 16
+    c["qpos"][:] = k
+    for order in (torch.arange(k), torch.arange(k).flip(0)):
+        c["idx"] = order.to(torch.int32).view(1, -1)
+        out, lse = run_attend(c, ctx=torch.empty(1, H, 512, device=DEV), workspace=(1, None))
+        check_range(c, out, lse, [0])
+    assert _status() == 0
+
+
+def test_scales_of_zero_and_of_the_smallest_numbers():
+    """Rows of zeros (a cache that nobody wrote), a group of tiny scales beside ordinary ones."""
+    c = range_case(8, 16, 3.0, 40, k=300)
+    c["cache"][:150] = 0
+    c["cache"][200:, 512:516] = torch.tensor([2.0 ** -126]).view(torch.uint8)
+    out, lse = run_attend(c, ctx=torch.empty(1, 16, 512, device=DEV), workspace=(1, None))
+    check_range(c, out, lse, [0])
+    c["cache"][:300] = 0                                          # nothing but zeros: scores 0, the mean of zeros
+    out, lse = run_attend(c)
+    assert _status() == 0 and bool((out == 0).all())
+    assert bool(((lse.cpu() - torch.log(torch.tensor(300.0))).abs() < 1e-5).all())

@@ -7,7 +7,7 @@
 //   S^T_g [128 keys x 32]  = K_g [128 x 128 dims, e4m3] * (Q_hi | Q_lo)_g      for each group g of 128 dims
 //   R^T   [128 keys x 16]  = K_pe [128 x 64, bf16] * Q_pe
 //   s[key, h] = q_scale[h] * sum_g scale_g[key] * (S_hi + S_lo) + R            one thread a key: its scales are its own
-//   p = 2^(s - m[h]),   P_g = 2^10 p * scale_g / ref in three terms          for each group, because the scales of V differ by group
+//   p = 2^(s - m[h]),   P_g = 2^10 p * scale_g / 2^(u_g[h] - m[h]) in three terms       the scales of V differ by group
 //   O^T_g [128 dims x 48] += V_g^T [128 dims x 128 keys, the same bytes read MN-major] * (P_0 | P_1 | P_2)_g
 //
 // q over a power of two that brings a row's largest latent value below 448 is hi = e4m3(q) and lo = e4m3(q - hi): eight
@@ -20,8 +20,10 @@
 // side by side in N and are added in fp32.  The position dims stay bf16.  A tile of 128 keys takes 36 MMAs of at
 // most 48 columns, where two tiles of the other kernel take 88 and 128 widened rows.
 //
-// The running maximum m[h] and the reference scale ref (a power of two) are common to the CTA; they are renewed, and O and
-// the sums rescaled, when a score exceeds m by 4.5 (base 2) or a scale exceeds ref.
+// Each head has a running maximum m[h] of the scores, each head and group one u_g[h] of s + log2(scale_g): what a key adds
+// to the group's values, so that a key of large scales but no weight does not push the others out of the terms' range.  Both
+// are whole numbers (rescaling is exact) and common to the CTA; they are renewed, and O and the sums rescaled, when a score exceeds
+// m by 4.5 (base 2) or a P_g 2^15.
 //
 // Work split: CTA = (item, split), as in the other kernel.  Roles (512 threads): warps 0-3 rows (TMA gathers of four rows
 // x 128 bytes straight into the operand layout, the scales by 16-byte asynchronous copies), warp 4 keys, warps 5 and 6 MMAs,
@@ -58,8 +60,10 @@ constexpr uint32_t kFewOCols = kFewTerms * 16;                      // O of a gr
 constexpr uint32_t kFewTmemS = 4 * kFewOCols;                       // two score buffers of 144 columns behind O
 constexpr uint32_t kFewSCols = 144;                                 // 4 groups x (16 hi + 16 lo), 16 position products
 static_assert(kFewTmemS + 2 * kFewSCols <= 512, "O and two score buffers");
-constexpr float kFewLift = 1024.0f;                                 // P = 2^10 p scale / ref,
-constexpr float kFewHeadroom = 4.5f;                                // at most 2^14.5
+constexpr float kFewLift = 10.0f;                                   // log2 of the largest P after a renewal
+constexpr float kFewMaxP = 32768.0f;                                // and P before the next one
+constexpr float kFewHeadroom = 4.5f;
+constexpr float kFewMinScale = -100.0f;                             // u_g - m: groups of scales below 2^-100 lose range
 
 __device__ __align__(16) uint8_t g_few_zero[16];
 
@@ -99,6 +103,31 @@ __device__ __forceinline__ uint32_t term_e5m2x2(float& a, float& b) {
   return t;
 }
 
+// 2^n for a whole n up to 127; zero below the normal numbers.
+__device__ __forceinline__ float pow2_of(float n) {
+  return n < -126.f ? 0.f : __int_as_float((static_cast<int>(n) + 127) << 23);
+}
+
+// The largest of each of N values over the warp: lane L ends up with that of value L / (32 / N) in v[0].
+template <int N>
+__device__ __forceinline__ void warp_max_spread(float (&v)[N]) {
+#pragma unroll
+  for (int o = 16, n = N; o > 0; o >>= 1) {
+    const bool up = threadIdx.x & o;
+    if (n > 1) {
+      n /= 2;
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i)
+        if (i < n) {
+          const float keep = up ? v[i + n] : v[i], give = up ? v[i] : v[i + n];
+          v[i] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, give, o));
+        }
+    } else {
+      v[0] = fmaxf(v[0], __shfl_xor_sync(0xffffffffu, v[0], o));
+    }
+  }
+}
+
 template <bool kPrefetch>
 __global__ void __launch_bounds__(kFewThreads, 1)
 sparse_mla_cached_few_kernel(const MlaCachedParams p, const __grid_constant__ CUtensorMap tmap_rows) {
@@ -110,8 +139,12 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p, const __grid_constant__ CU
   __shared__ __align__(16) int s_slot[kFewKeyTiles][kFewTile];
   __shared__ uint32_t s_mask[kFewStages][4];      // validity bit per key of the stage
   __shared__ int s_renew[3];                      // somebody's key exceeds the references (tile % 3)
-  __shared__ float s_top[4][kFewHeads];           // maxima of the four lane quadrants
-  __shared__ float s_ref[4];                      // largest scales of the four quadrants
+  __shared__ uint32_t s_top[kFewHeads];           // largest score so far, in the order of unsigned numbers
+  __shared__ uint32_t s_vtop[4][kFewHeads];       // largest s + log2(scale_g) so far, likewise
+  __shared__ float s_m[kFewHeads];                // m[h] and, of every group, u_g[h], 2^(10 + m - u_g) and the factor that a
+  __shared__ float s_u[4][kFewHeads];             // renewal, or the output, applies to O
+  __shared__ __align__(16) float s_lift[4][kFewHeads];
+  __shared__ __align__(16) float s_shrink[4][kFewHeads];
   __shared__ float s_sum[4][kFewHeads];
   __shared__ float s_qscale[kFewHeads];
 
@@ -138,6 +171,13 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p, const __grid_constant__ CU
   const int n_tiles = static_cast<int>(static_cast<int64_t>(all_tiles) * (split + 1) / p.splits) - tile0;
   volatile int* abort_flag = &s_abort;
 
+  if (tid < 4 * kFewHeads) {
+    if (tid < kFewHeads) s_top[tid] = float_to_ordered(-INFINITY);
+    s_vtop[tid / kFewHeads][tid % kFewHeads] = float_to_ordered(-INFINITY);
+    s_u[tid / kFewHeads][tid % kFewHeads] = -INFINITY;
+    s_m[tid % kFewHeads] = -INFINITY;
+    s_lift[tid / kFewHeads][tid % kFewHeads] = 0.f;
+  }
   if (tid == 0) {
     s_abort = 0;
     s_renew[0] = s_renew[1] = s_renew[2] = 0;
@@ -339,7 +379,6 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p, const __grid_constant__ CU
       m[j] = -INFINITY;
       l[j] = 0.f;
     }
-    float ref = 0.f, inv_ref = 0.f;                        // reference scale (a power of two, 0 before the first key)
     for (int t = 0; ok && t < n_tiles; ++t) {
       const int sb = t & 1, st = t % kFewStages;
       ok = __all_sync(0xffffffffu, mbar_wait(&s_full[sb], (t >> 1) & 1, abort_flag) &&
@@ -371,10 +410,25 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p, const __grid_constant__ CU
         }
         tc_fence_before();
         mbar_arrive(&s_empty[sb]);
-        // the scale that a value of this key may be multiplied by, as a power of two
-        float big = max_nan(max_nan(fabsf(sc[0]), fabsf(sc[1])), max_nan(fabsf(sc[2]), fabsf(sc[3])));
-        if (!valid) big = 0.f;
-        bool over = !(big <= ref);
+        float e[8], x[4][8];
+        auto probabilities = [&]() {                        // and P of every group; a missing key has p = 0 and scales of 0
+#pragma unroll
+          for (int j = 0; j < 8; ++j) e[j] = fast_exp2(s[j] - (m[j] == -INFINITY ? 0.f : m[j]));
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const float4 a = *reinterpret_cast<const float4*>(&s_lift[g][hb]), b = *reinterpret_cast<const float4*>(&s_lift[g][hb + 4]);
+            const float f[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[g][j] = e[j] * sc[g] * f[j];
+          }
+        };
+        probabilities();
+        float big = 0.f;                                    // a NaN needs no other reference
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(x[g][j]));
+        bool over = big > kFewMaxP;
 #pragma unroll
         for (int j = 0; j < 8; ++j) over = over || s[j] > m[j] + kFewHeadroom;
         if (__any_sync(0xffffffffu, over) && lane == 0) *reinterpret_cast<volatile int*>(&s_renew[t % 3]) = 1;
@@ -382,36 +436,41 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p, const __grid_constant__ CU
         if (!ok) break;
         if (tid == 256) s_renew[(t + 2) % 3] = 0;           // read by everyone before this barrier, set after the next
         if (*reinterpret_cast<volatile int*>(&s_renew[t % 3])) {
-          // new references: the largest score of every head and the largest scale among the tile's 128 keys
-          float top[8];
+          // New references from the tile's 128 keys: lane 8 g + j of a warp ends up with the largest value of group g and head j.
+          float top[32];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) top[j] = s[j];
-          for (int o = 16; o > 0; o >>= 1) {
+          for (int g = 0; g < 4; ++g) {
+            const float size = log2f(fabsf(sc[g]));
 #pragma unroll
-            for (int j = 0; j < 8; ++j) top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], o));
-            big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, o));
+            for (int j = 0; j < 8; ++j) top[g * 8 + j] = s[j] + size;
           }
-          if (lane == 0) {
+          warp_max_spread(top);
+          atomicMax(&s_vtop[lane >> 3][hb + (lane & 7)], float_to_ordered(top[0]));
+          float best[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s_top[wq][hb + j] = top[j];
-            if (hb == 0) s_ref[wq] = big;
+          for (int j = 0; j < 8; ++j) best[j] = s[j];
+          warp_max_spread(best);
+          if ((lane & 3) == 0) atomicMax(&s_top[hb + (lane >> 2)], float_to_ordered(best[0]));
+          ok = rendezvous();
+          if (!ok) break;
+          if (tid < 256 + 4 * kFewHeads) {
+            const int h = tid % kFewHeads, g = (tid - 256) / kFewHeads;
+            const float nm = ceilf(ordered_to_float(s_top[h]));
+            const float nu = fmaxf(ceilf(ordered_to_float(s_vtop[g][h])), nm + kFewMinScale), u = s_u[g][h];
+            s_shrink[g][h] = pow2_of(u - nu);
+            s_lift[g][h] = nm == -INFINITY ? 0.f : pow2_of(nm - nu + kFewLift);
+            s_u[g][h] = nu;
+            if (g == 0) s_m[h] = nm;
           }
           ok = rendezvous();
           if (!ok) break;
-          float f[8];
-          const float all = max_nan(max_nan(s_ref[0], s_ref[1]), max_nan(s_ref[2], s_ref[3]));
-          const float new_ref = all <= ref ? ref : pow2_at_least(all);
-          const float shrink = ref > 0.f ? ref / new_ref : 0.f;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const float n = fmaxf(m[j], fmaxf(fmaxf(s_top[0][hb + j], s_top[1][hb + j]), fmaxf(s_top[2][hb + j], s_top[3][hb + j])));
-            f[j] = m[j] == -INFINITY ? 0.f : exp2f(m[j] - n);
+            const float n = s_m[hb + j];
+            l[j] *= pow2_of(m[j] - n);
             m[j] = n;
-            l[j] *= f[j];
-            f[j] *= shrink;
           }
-          ref = new_ref;
-          inv_ref = ref > 0.f ? 1.0f / ref : 0.f;
+          probabilities();
           if (t > 0) {
             ok = __all_sync(0xffffffffu, mbar_wait(pv_done, (t - 1) & 1, abort_flag));
             tc_fence_after();
@@ -419,6 +478,7 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p, const __grid_constant__ CU
             for (int c = 0; c < 4 * kFewTerms; ++c) {       // the terms of every group
               float o[8];
               const uint32_t at = tmem_base + lane_addr + c * 16 + hb;
+              const float* f = &s_shrink[c / kFewTerms][hb];
               few_ld8(at, o);
               tc_wait_ld();
 #pragma unroll
@@ -433,26 +493,16 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p, const __grid_constant__ CU
         }
         // P of group g, MN-major: core matrices of 8 keys x 16 bytes, the terms of the 16 heads side by side.  (Stored
         // K-major, one byte a store, it took 64 stores a thread.)
-        float pr[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float neg = m[j] == -INFINITY ? 0.f : -m[j];
-          const float e = fast_exp2(s[j] + neg);
-          l[j] += e;
-          pr[j] = e * kFewLift;
-        }
+        for (int j = 0; j < 8; ++j) l[j] += e[j];
         const uint32_t row = smem_base + kFewPOff + (key >> 3) * kFewPOctet + (key & 7) * 16 + hb;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const float w = valid ? sc[g] * inv_ref : 0.f;
-          float x[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = pr[j] * w;
 #pragma unroll
           for (int c = 0; c < kFewTerms; ++c) {
             uint32_t t2[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) t2[j] = term_e5m2x2(x[2 * j], x[2 * j + 1]);
+            for (int j = 0; j < 4; ++j) t2[j] = term_e5m2x2(x[g][2 * j], x[g][2 * j + 1]);
             asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(row + g * kFewPGroup + c * 128), "r"(t2[0] | t2[1] << 16),
                          "r"(t2[2] | t2[3] << 16) : "memory");
           }
@@ -472,21 +522,21 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p, const __grid_constant__ CU
 #pragma unroll
       for (int j = 0; j < 8; ++j) s_sum[wq][hb + j] = l[j];
     }
+    const int64_t parts = static_cast<int64_t>(p.n_items) * p.n_heads, row0 = static_cast<int64_t>(item) * p.n_heads;
+    if (ok) ok = rendezvous();
+    if (ok && tid < 256 + 4 * kFewHeads) {
+      // the factor of a head's O: what its P was multiplied by is taken out, and the sum
+      const int h = tid % kFewHeads, g = (tid - 256) / kFewHeads;
+      const float sum = s_sum[0][h] + s_sum[1][h] + s_sum[2][h] + s_sum[3][h];
+      const bool any = n_tiles > 0 && sum != 0.f;           // a NaN sum stays NaN in the result
+      s_shrink[g][h] = any ? pow2_of(s_u[g][h] - s_m[h] - kFewLift) / sum : 0.f;
+      if (g == 0 && h < p.n_heads) {
+        float* lse = p.splits == 1 ? p.lse + row0 + h : p.part + p.splits * parts * kMlaDv + split * parts + row0 + h;
+        *lse = any ? (s_m[h] + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+      }
+    }
     if (ok) ok = rendezvous();
     if (ok) {
-      const int64_t parts = static_cast<int64_t>(p.n_items) * p.n_heads;
-      const int64_t row0 = static_cast<int64_t>(item) * p.n_heads + hb;
-      float k[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float sum = s_sum[0][hb + j] + s_sum[1][hb + j] + s_sum[2][hb + j] + s_sum[3][hb + j];
-        const bool any = n_tiles > 0 && sum != 0.f;         // a NaN sum stays NaN in the result
-        k[j] = any ? ref * (1.0f / kFewLift) / sum : 0.f;
-        if (key == 0 && hb + j < p.n_heads) {
-          float* lse = p.splits == 1 ? p.lse + row0 + j : p.part + p.splits * parts * kMlaDv + split * parts + row0 + j;
-          *lse = any ? (m[j] + log2f(sum)) * 0.6931471805599453f : -INFINITY;
-        }
-      }
 #pragma unroll 1
       for (int g = 0; g < 4; ++g) {
         float a[8], b[8], c[8];
@@ -497,13 +547,16 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p, const __grid_constant__ CU
           tc_wait_ld();
         }
         const int dim = g * 128 + key;                      // the lane is a dim of the group here
+        float unit[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) unit[j] = s_shrink[g][hb + j];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           if (hb + j >= p.n_heads) continue;
-          const float v = k[j] != 0.f ? fmaf(fmaf(c[j], 1.0f / 16, b[j]), 1.0f / 16, a[j]) * k[j] : 0.f;
-          if (p.splits > 1) p.part[(split * parts + row0 + j) * kMlaDv + dim] = v;
-          else if (p.ctx_bf16) static_cast<__nv_bfloat16*>(p.ctx)[(row0 + j) * kMlaDv + dim] = __float2bfloat16_rn(v);
-          else static_cast<float*>(p.ctx)[(row0 + j) * kMlaDv + dim] = v;
+          const float v = unit[j] != 0.f ? fmaf(fmaf(c[j], 1.0f / 16, b[j]), 1.0f / 16, a[j]) * unit[j] : 0.f;
+          if (p.splits > 1) p.part[(split * parts + row0 + hb + j) * kMlaDv + dim] = v;
+          else if (p.ctx_bf16) static_cast<__nv_bfloat16*>(p.ctx)[(row0 + hb + j) * kMlaDv + dim] = __float2bfloat16_rn(v);
+          else static_cast<float*>(p.ctx)[(row0 + hb + j) * kMlaDv + dim] = v;
         }
         __syncwarp();
       }
