@@ -2,7 +2,8 @@
 nearly all of a head's probability over a broad tail (an attention sink), groups of dims whose scales lie far apart.
 
 Bounds: check_attend's (a probability is off by at most a bf16 half step, 2^-8 of itself, however small it is), and for
-the queries, which up to 16 heads are two e4m3 numbers, 2^-18 of a row's largest latent value."""
+the queries, which up to 16 heads are two e4m3 numbers, the second lifted by 16, 2^-21 of a row's largest latent value
+(half of e4m3's smallest step, 2^-10, over 16, of values whose largest is between 224 and 448)."""
 import pytest
 import torch
 
@@ -10,7 +11,7 @@ from oracle import latent_oracle as L
 from tests.test_gpu_latent_cache import BF16, DEV, F32, _status, run_attend
 
 pytestmark = pytest.mark.gpu
-QUERY = 2.0 ** -18
+QUERY = 2.0 ** -21
 
 
 def check_range(c, ctx, lse, items, query=QUERY):
@@ -141,3 +142,18 @@ def test_scales_of_zero_and_of_the_smallest_numbers():
     out, lse = run_attend(c)
     assert _status() == 0 and bool((out == 0).all())
     assert bool(((lse.cpu() - torch.log(torch.tensor(300.0))).abs() < 1e-5).all())
+
+
+@pytest.mark.parametrize("H", [1, 16, 17])
+@pytest.mark.parametrize("top", [64.0, 4096.0])
+def test_queries_with_one_large_dim(H, top):
+    """A query dim far above the others that meets nothing in the cache takes no precision from them: values of 1.75 * 2^-18 of
+    it, which two terms hold exactly (the row's power of two makes 256 and 1.75 * 2^-10 of them, and the second term, 16 times
+    that, is a normal number)."""
+    c = range_case(3 + H, H, 2.0, 9, k=600)
+    c["q"][:, :, :512] = 1.75 * 2.0 ** -18 * top
+    c["q"][:, :, 5:512:128] = top
+    c["cache"][:, 5:512:128] = 0
+    out, lse = run_attend(c, ctx=torch.empty(1, H, 512, device=DEV), workspace=(1, None))
+    check_range(c, out, lse, [0], query=0)
+    assert _status() == 0

@@ -6,12 +6,13 @@
 //
 //   S^T_g [128 keys x 32]  = K_g [128 x 128 dims, e4m3] * (Q_hi | Q_lo)_g      for each group g of 128 dims
 //   R^T   [128 keys x 16]  = K_pe [128 x 64, bf16] * Q_pe
-//   s[key, h] = q_scale[h] * sum_g scale_g[key] * (S_hi + S_lo) + R            one thread a key: its scales are its own
+//   s[key, h] = q_scale[h] * sum_g scale_g[key] * (S_hi + S_lo / 16) + R       one thread a key: its scales are its own
 //   p = 2^(s - m[h]),   P_g = 2^10 p * scale_g / 2^(u_g[h] - m[h]) in three terms       the scales of V differ by group
 //   O^T_g [128 dims x 48] += V_g^T [128 dims x 128 keys, the same bytes read MN-major] * (P_0 | P_1 | P_2)_g
 //
-// q over a power of two that brings a row's largest latent value below 448 is hi = e4m3(q) and lo = e4m3(q - hi): eight
-// bits, as bf16 has, and off by at most 2^-18 of the largest value.  Probabilities need more range: thousands of keys
+// q over a power of two that brings a row's largest latent value to 224 .. 448 is hi = e4m3(q) and lo = e4m3(16 (q - hi)):
+// eight bits, as bf16 has, and off by at most 2^-14 (half of e4m3's smallest step, 2^-10, over 16), 2^-21 of the largest value.  (A rest
+// is at most 16, so that 16 of it fit; unlifted, one large dim took the other dims' lower bits.)  Probabilities need more range: thousands of keys
 // that hold 2^-17 of the largest one's each are a share of the result.  P is t0 + t1 / 16 + t2 / 256 in e5m2,
 //   t0 = e5m2(P),  t1 = e5m2(16 (P - t0)),  t2 = e5m2(16 (16 (P - t0) - t1)),
 // each rounding off by 2^-3 of what it rounds: three leave 2^-9 of P, half of a bf16 rounding's 2^-8, as long as t2 is a normal
@@ -86,12 +87,12 @@ __device__ __forceinline__ void few_st8(uint32_t taddr, const float (&v)[8]) {
                "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
                : "memory");
 }
-// a and b as e4m3 hi and lo codes: (hi a, hi b) and (lo a, lo b)
+// a and b as e4m3 codes (hi a, hi b) and, of 16 times what those leave, (lo a, lo b)
 __device__ __forceinline__ void split_e4m3x2(float a, float b, uint32_t& hi, uint32_t& lo) {
   hi = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(hi), __NV_E4M3);
   const float2 f = __half22float2(__half2(h));
-  lo = __nv_cvt_float2_to_fp8x2(make_float2(a - f.x, b - f.y), __NV_SATFINITE, __NV_E4M3);
+  lo = __nv_cvt_float2_to_fp8x2(make_float2((a - f.x) * 16.0f, (b - f.y) * 16.0f), __NV_SATFINITE, __NV_E4M3);
 }
 // The next e5m2 term of a and b; they become 16 times what it leaves.
 __device__ __forceinline__ uint32_t term_e5m2x2(float& a, float& b) {
@@ -405,7 +406,7 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p, const __grid_constant__ CU
         for (int j = 0; j < 8; ++j) {
           float a = 0.f;
 #pragma unroll
-          for (int g = 0; g < 4; ++g) a = fmaf(sc[g], hi[g][j] + lo[g][j], a);
+          for (int g = 0; g < 4; ++g) a = fmaf(sc[g], fmaf(lo[g][j], 1.0f / 16, hi[g][j]), a);
           s[j] = valid ? fmaf(a, qs[j], r[j] * p.scale_log2) : -INFINITY;
         }
         tc_fence_before();
