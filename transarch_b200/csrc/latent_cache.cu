@@ -205,6 +205,8 @@ __global__ void __launch_bounds__(32 * kRowWarps) latent_read_kernel(const Laten
 // (j itself included).  A parent comes before its children, so a walk takes at most 64 steps.
 __global__ void __launch_bounds__(64) draft_tree_masks_kernel(const int32_t* __restrict__ parents, int n_nodes,
                                                               int64_t* __restrict__ masks, int32_t* status) {
+  pdl_launch_dependents();
+  pdl_wait_prior();
   __shared__ int32_t s_parent[64];
   const int64_t base = static_cast<int64_t>(blockIdx.x) * n_nodes;
   const int j = threadIdx.x;
