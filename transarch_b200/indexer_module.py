@@ -32,6 +32,27 @@ def _version(t: torch.Tensor) -> int:
     return -1 if t.is_inference() else t._version
 
 
+class _Quantised:
+    """The 8-bit copy of a weight, with what tells whether the weight is still the one that it was made of."""
+
+    def __init__(self, weight: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor):
+        self.weight, self.codes, self.scale = weight, codes, scale
+        self.dtype = weight.dtype
+        self.version: Optional[int] = _version(weight)          # None: stale for good
+
+    def of(self, weight: torch.Tensor) -> bool:
+        return weight is self.weight and _version(weight) == self.version and weight.dtype == self.dtype and \
+            weight.device == self.codes.device
+
+    # A copied or reloaded module has weights of its own, whose counters start anew.
+    def __getstate__(self):
+        return {**self.__dict__, "version": self.of(self.weight)}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self.version = _version(self.weight) if state["version"] else None
+
+
 class LightningIndexer(nn.Module):
     def __init__(self, hidden_size: int, n_heads: int = 8, head_dim: int = 128, rope_dim: int = 64,
                  q_input_dim: Optional[int] = None, dtype: torch.dtype = torch.bfloat16):
@@ -47,30 +68,30 @@ class LightningIndexer(nn.Module):
         self.wk = nn.Linear(hidden_size, head_dim, bias=False, dtype=dtype)
         self.k_norm = nn.LayerNorm(head_dim, dtype=dtype)
         self.w_proj = nn.Linear(hidden_size, n_heads, bias=False, dtype=dtype)
-        self._fp8 = {}            # quantise_projections(): name -> (codes, scales, the weight, its version and dtype)
+        self._fp8 = {}            # quantise_projections(): name -> _Quantised
         self._fp8_fmt: Optional[str] = None
 
     @torch.no_grad()
     def quantise_projections(self, scale_fmt: Optional[str] = None) -> None:
         """Keep 8-bit copies of wq and wk (one scale for a block of 128 x 128) for forward_quantised; the activations are
         quantised on the way, with `scale_fmt` scales for 128 values of a row.  The parameters stay as they are; once
-        they change, or move, forward_quantised refuses to run until this has been called again.  (Writes through `.data`
+        they change, or move, forward_quantised refuses to run until this has been called again.  A copied or reloaded module
+        takes them along.  (Writes through `.data`
         or to parameters made under inference_mode carry no version: after those, call this again yourself.)"""
         held = {}
         for name, lin in (("wq", self.wq), ("wk", self.wk)):
             codes, scale = K.fp8_quantise_blocks(lin.weight.detach(), scale_fmt=scale_fmt)
-            held[name] = (codes, scale, lin.weight, _version(lin.weight), lin.weight.dtype)
+            held[name] = _Quantised(lin.weight, codes, scale)
         self._fp8, self._fp8_fmt = held, scale_fmt
 
     def _project(self, name: str, x: torch.Tensor) -> torch.Tensor:
         lin = getattr(self, name)
         if name not in self._fp8:
             return lin(x)
-        codes, scale, weight, version, dtype = self._fp8[name]
-        if lin.weight is not weight or _version(weight) != version or weight.dtype != dtype or \
-                weight.device != codes.device:
+        held = self._fp8[name]
+        if not held.of(lin.weight):
             raise B200DSAError(f"{name} has changed since quantise_projections(): call it again")
-        return K.fp8_block_linear(x, codes, scale, scale_fmt=self._fp8_fmt, out_dtype=x.dtype)
+        return K.fp8_block_linear(x, held.codes, held.scale, scale_fmt=self._fp8_fmt, out_dtype=x.dtype)
 
     @torch.no_grad()
     def forward(self, hidden_states, q_input, cos, sin):
