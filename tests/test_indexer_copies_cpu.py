@@ -56,3 +56,25 @@ def test_a_stale_copy_stays_stale(mod, duplicate):
         mod.wk.weight.mul_(2.0)
     with pytest.raises(B200DSAError, match="wk has changed"):
         duplicate(mod)._project("wk", X)
+
+
+def test_a_weight_whose_data_was_replaced_is_refused(mod):
+    """To another type and back: the counter does not move, the values do."""
+    mod.half().float()
+    with pytest.raises(B200DSAError, match="wq has changed"):
+        mod._project("wq", X)
+    mod.quantise_projections()
+    mod.wq.half()
+    mod.wq.float()
+    with pytest.raises(B200DSAError, match="wq has changed"):
+        mod._project("wq", X)
+    mod._project("wk", X)
+    mod.wk.weight.data = mod.wk.weight.data * 2
+    with pytest.raises(B200DSAError, match="wk has changed"):
+        mod._project("wk", X)
+    mod.quantise_projections()
+    mod.float()                                                   # nothing to do: nothing is replaced
+    assert torch.equal(copy.deepcopy(mod)._project("wk", X), mod._project("wk", X))
+    torch.nn.utils.vector_to_parameters(torch.nn.utils.parameters_to_vector(mod.wq.parameters()) + 1, mod.wq.parameters())
+    with pytest.raises(B200DSAError, match="wq has changed"):
+        copy.deepcopy(mod)._project("wq", X)

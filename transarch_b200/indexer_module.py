@@ -37,20 +37,23 @@ class _Quantised:
 
     def __init__(self, weight: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor):
         self.weight, self.codes, self.scale = weight, codes, scale
-        self.dtype = weight.dtype
         self.version: Optional[int] = _version(weight)          # None: stale for good
+        # The memory that the weight had.  Held, so that no other tensor can come to lie there: `.to()`, `.half()` and
+        # assignments to `.data` move the weight without a trace in its counter.
+        self.memory = weight.detach()
 
     def of(self, weight: torch.Tensor) -> bool:
-        return weight is self.weight and _version(weight) == self.version and weight.dtype == self.dtype and \
-            weight.device == self.codes.device
+        return weight is self.weight and _version(weight) == self.version and weight.dtype == self.memory.dtype and \
+            weight.device == self.codes.device and weight.data_ptr() == self.memory.data_ptr()
 
     # A copied or reloaded module has weights of its own, whose counters start anew.
     def __getstate__(self):
-        return {**self.__dict__, "version": self.of(self.weight)}
+        return {**self.__dict__, "version": self.of(self.weight), "memory": None}
 
     def __setstate__(self, state):
         self.__dict__.update(state)
         self.version = _version(self.weight) if state["version"] else None
+        self.memory = self.weight.detach()
 
 
 class LightningIndexer(nn.Module):
@@ -75,9 +78,9 @@ class LightningIndexer(nn.Module):
     def quantise_projections(self, scale_fmt: Optional[str] = None) -> None:
         """Keep 8-bit copies of wq and wk (one scale for a block of 128 x 128) for forward_quantised; the activations are
         quantised on the way, with `scale_fmt` scales for 128 values of a row.  The parameters stay as they are; once
-        they change, or move, forward_quantised refuses to run until this has been called again.  A copied or reloaded module
-        takes them along.  (Writes through `.data`
-        or to parameters made under inference_mode carry no version: after those, call this again yourself.)"""
+        they change, or move, forward_quantised refuses to run until this has been called again.  A copied or reloaded
+        module takes the copies along.  (In-place writes to `.data` or to parameters made under inference_mode leave no
+        trace: after those, call this again yourself.)"""
         held = {}
         for name, lin in (("wq", self.wq), ("wk", self.wk)):
             codes, scale = K.fp8_quantise_blocks(lin.weight.detach(), scale_fmt=scale_fmt)
