@@ -78,3 +78,16 @@ def test_a_weight_whose_data_was_replaced_is_refused(mod):
     torch.nn.utils.vector_to_parameters(torch.nn.utils.parameters_to_vector(mod.wq.parameters()) + 1, mod.wq.parameters())
     with pytest.raises(B200DSAError, match="wq has changed"):
         copy.deepcopy(mod)._project("wq", X)
+
+
+@pytest.mark.parametrize("make", [
+    lambda x: x.t().contiguous().t(),                             # columns apart
+    lambda x: x[:1].expand(3, 32),                                # one row for all tokens
+    lambda x: x.view(3, 1, 32),
+    lambda x: x.view(3, 2, 16).transpose(1, 2).reshape(3, 32).view(1, 3, 32)[0],
+    lambda x: x[:0], lambda x: x[:0].view(0, 1, 32)])
+def test_projections_take_what_a_linear_takes(mod, make):
+    x = make(X)
+    got, want = mod._project("wq", x), mod.wq(x)
+    mass = x.abs() @ mod.wq.weight.abs().t()                      # two fp32 sums of 32 products
+    assert got.shape == want.shape and bool(((got - want).abs() <= 2 * 32 * 2.0 ** -24 * mass).all())

@@ -94,7 +94,12 @@ class LightningIndexer(nn.Module):
         held = self._fp8[name]
         if not held.of(lin.weight):
             raise B200DSAError(f"{name} has changed since quantise_projections(): call it again")
-        return K.fp8_block_linear(x, held.codes, held.scale, scale_fmt=self._fp8_fmt, out_dtype=x.dtype)
+        # any leading dims and strides, as for the Linear; the kernel wants rows that lie apart with unit column stride
+        rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+        if rows.stride(1) != 1 or (rows.shape[0] > 1 and rows.stride(0) < rows.shape[1]):
+            rows = rows.contiguous()
+        y = K.fp8_block_linear(rows, held.codes, held.scale, scale_fmt=self._fp8_fmt, out_dtype=x.dtype)
+        return y if x.dim() == 2 else y.view(*x.shape[:-1], y.shape[1])
 
     @torch.no_grad()
     def forward(self, hidden_states, q_input, cos, sin):
