@@ -540,7 +540,7 @@ static cudaError_t mlc_run(const MlaCachedParams& p, bool prefetch, int device, 
   // Up to 16 heads the codes are multiplied as they are: 148 items x 2048 keys take 49 us for 16 heads, and 77 us for 17,
   // which the kernel for 64 heads does (it takes the same time for 1 head as for 64).
   cudaError_t e;
-  if (p.n_heads <= kMlcFewHeads) e = mla_cached_few_launch(p, prefetch, device, stream);
+  if (p.n_heads <= kMlcFewHeads) e = mla_cached_few_launch(p, device, stream);
   else e = prefetch ? mlc_launch<true>(p, device, stream) : mlc_launch<false>(p, device, stream);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess || p.splits == 1) return e;

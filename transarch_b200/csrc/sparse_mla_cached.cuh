@@ -140,6 +140,6 @@ __device__ __forceinline__ void mlc_key_warp(const MlaCachedParams& p, int item,
 
 // Up to kMlcFewHeads heads: the kernel that multiplies the codes as they are (sparse_mla_cached_few.cu).
 constexpr int kMlcFewHeads = 16;
-cudaError_t mla_cached_few_launch(const MlaCachedParams& p, bool prefetch, int device, cudaStream_t stream);
+cudaError_t mla_cached_few_launch(const MlaCachedParams& p, int device, cudaStream_t stream);
 
 }  // namespace b200dsa

@@ -33,7 +33,8 @@
 // 7 k clocks of its chain (rows 2.2, scores 1.3, softmax 1.8, values 1.8) two stages overlap two, and a third does not fit
 // beside P and Q.  Before the gathers (every 16 bytes by an asynchronous copy, 28 bytes a clock) it took 2.5 us.  A
 // gather takes its issuing lane about 50 clocks: two issuing warps take 2 - 4 % longer, one 14 - 20 %, and a copy of each lane of
-// a warp 90 clocks.
+// a warp 90 clocks.  The key warp prefetches no rows: two tiles of copies in flight cover the latency, and its 896 lines a tile take
+// longer than the tile (148 items of as many requests 59.9 us with prefetches, 53.7 without; 64 items x 3 73.1 and 67.7).
 #include "sparse_mla_cached.cuh"
 
 namespace b200dsa {
@@ -129,7 +130,6 @@ __device__ __forceinline__ void warp_max_spread(float (&v)[N]) {
   }
 }
 
-template <bool kPrefetch>
 __global__ void __launch_bounds__(kFewThreads, 1)
 sparse_mla_cached_few_kernel(const MlaCachedParams p, const __grid_constant__ CUtensorMap tmap_rows) {
   pdl_launch_dependents();
@@ -253,7 +253,7 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p, const __grid_constant__ CU
       }
     }
   } else if (warp == 4) {
-    mlc_key_warp<kFewTile, kFewKeyTiles, kPrefetch>(p, item, tile0, n_tiles, n_idx, &s_slot[0][0], key_full, key_empty, abort_flag);
+    mlc_key_warp<kFewTile, kFewKeyTiles, false>(p, item, tile0, n_tiles, n_idx, &s_slot[0][0], key_full, key_empty, abort_flag);
   } else if (warp == 5) {
     // ------------------------------------------------------------------ score MMAs
     constexpr uint32_t idesc_s = make_idesc(kFmtE4M3, kFmtE4M3, 128, 32);
@@ -570,18 +570,7 @@ sparse_mla_cached_few_kernel(const MlaCachedParams p, const __grid_constant__ CU
   if (tid == 0 && s_abort) atomicMax(p.status, kDevWaitTimeout);
 }
 
-template <bool kPrefetch>
-static cudaError_t few_launch(const MlaCachedParams& p, const CUtensorMap& rows, int device, cudaStream_t stream) {
-  static OncePerDevice once;
-  cudaError_t e = once.run(device, [] {
-    return cudaFuncSetAttribute(sparse_mla_cached_few_kernel<kPrefetch>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem);
-  });
-  if (e != cudaSuccess) return e;
-  return launch_chained(sparse_mla_cached_few_kernel<kPrefetch>, dim3(p.n_items * p.splits), dim3(kFewThreads), kFewSmem,
-                        stream, p, rows);
-}
-
-cudaError_t mla_cached_few_launch(const MlaCachedParams& p, bool prefetch, int device, cudaStream_t stream) {
+cudaError_t mla_cached_few_launch(const MlaCachedParams& p, int device, cudaStream_t stream) {
   PFN_encodeTiled enc = get_encode_tiled();
   if (!enc) return cudaErrorNotSupported;
   // the rows of all slots, in pieces of 128 bytes and the operands' swizzle
@@ -592,8 +581,12 @@ cudaError_t mla_cached_few_launch(const MlaCachedParams& p, bool prefetch, int d
           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return cudaErrorInvalidValue;
-  // 592 items of 148 requests: 176 us without prefetches, 187 with
-  return prefetch ? few_launch<true>(p, rows, device, stream) : few_launch<false>(p, rows, device, stream);
+  static OncePerDevice once;
+  const cudaError_t e = once.run(device, [] {
+    return cudaFuncSetAttribute(sparse_mla_cached_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem);
+  });
+  if (e != cudaSuccess) return e;
+  return launch_chained(sparse_mla_cached_few_kernel, dim3(p.n_items * p.splits), dim3(kFewThreads), kFewSmem, stream, p, rows);
 }
 
 }  // namespace b200dsa
