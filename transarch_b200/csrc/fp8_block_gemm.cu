@@ -15,8 +15,8 @@
 // Many tokens: 128 tokens are M and 256 weight rows N.  A thread owns one token, so that the scale of a block is one
 // register and the shared-memory port carries nothing but the operands (48 KB in by TMA and 48 KB out to the MMAs a block).
 //
-// Measured: 4096 x 7168 x 7168 in 192 us (2.2 PFLOP/s; 920 clocks a block where its MMAs take 512: the tensor pipe waits
-// for the accumulating warps); 16 x 18944 x 7168 in 27 us (5.1 TB/s of weights);
+// Measured: 4096 x 7168 x 7168 in 189 - 226 us by box (1.9 - 2.2 PFLOP/s; 920 clocks a block where its MMAs take 512: the tensor pipe
+// waits for the accumulating warps); 16 x 18944 x 7168 in 27 us (5.1 TB/s of weights);
 // 64 x 8192 x 1536 in 8 us, of which the blocks are 3.
 //
 // Narrow kernel, 352 threads: warp 0 TMA loads, warp 1 MMAs, warp 2 scales, warps 3-10 accumulate (two a TMEM lane
@@ -902,9 +902,9 @@ static int gemm_rc(cudaError_t e) {
 // estimated time.  Measured clocks of a block: narrow 830 (16 tokens) .. 1000 (128), bound by the weights from HBM or
 // by the accumulating warps; wide 930.  A wave costs 600 more, a split its barriers and the exchange of the partial sums.
 // Tiles that would start one more, mostly empty wave can be a launch of their own, their K split over clusters:
-// 256 x 19200 x 7168 69 -> 50 us, 2048 x 4736 x 7168 75 -> 67, 16 x 19200 x 7168 51 -> 35, 4096 x 7168 x 7168 (six waves
-// and 8 tiles) 194.5 -> 192.  An estimated gain below 7 % was none: 8192 x 7168 x 7168 370 -> 377, 64 x 19200 x 1536 13.4 ->
-// 14.0 (after many full waves the tensor pipes are at the power limit, and an idle last wave is paid back in clocks).
+// without and with it on one box 256 x 19200 x 7168 73 -> 58 us, 2048 x 4736 x 7168 92 -> 76 - 81, 16 x 19200 x 7168 46 -> 33.5,
+// 64 x 24576 x 7168 47 -> 44 (faster boxes: 46, 70 and 33 us for the first three, with it).  An estimated gain below 7 % was none:
+// 8192 x 7168 x 7168 370 -> 377, 64 x 19200 x 1536 13.4 -> 14.0 (after many full waves the tensor pipes are at the power limit, and an idle last wave is paid back in clocks).
 struct GemmPlan {
   int nt;             // tokens of a tile; 0 = the kernel for many tokens
   int splits;

@@ -13,8 +13,10 @@
 // attention over the cache and the rows read back see the same numbers.
 //
 // One warp per row.  Lane l holds dims 8l..8l+7 of either half of the latent dims (group = half * 2 + l / 16) and the
-// rotation pair l, so that every load and store of the warp is one contiguous run of 256 or 512 bytes.  Reading is bound by
-// memory (69 666 rows in 24.6 us, 5.1 TB/s); writing 4096 tokens and reading them back takes 6.1 us, two launches.
+// rotation pair l, so that every load and store of the warp is one contiguous run of 256 or 512 bytes.  Reading 72 384 rows
+// takes 24.6 us (5.3 TB/s of bytes read and written; what it writes stays in L2, issue slots are 59 % busy), a million rows run at
+// 6.1 TB/s, near the memory's rate.  Writing 4096 tokens and reading them back takes 6.1 us, two launches; writing 65 536 takes 50 us
+// (3.0 TB/s): a row's loads wait for that of its slot.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 

@@ -18,7 +18,7 @@
 // Work split: CTA = (item, 64-head half, split).  Small batches cut an item's tiles into `splits` runs whose partial
 // contexts (normalised, fp32) and log-sum-exps are merged by mla_merge_kernel; large ones have splits = 1 and no merge,
 // or (splits < 0) cut only the items behind the last full wave, in a second launch: 80 x 128 x 2048 134 -> 99 us, 192 x 16 x 2048
-// 82 -> 71, 170 x 64 x 2048 139 -> 111.
+// 90 - 94 -> 76 - 81, 170 x 64 x 2048 139 -> 111.
 //
 // Roles (448 threads): warps 0-7 rows, warps 8-11 softmax, warp 12 MMAs, warp 13 keys: it turns positions into slots, up
 // to four tiles ahead of the rows, and has their bytes brought into L2 meanwhile.  (The row warps did that themselves at
@@ -537,7 +537,7 @@ static int whole_wave_items(int n_items, int n_heads, int sms) {
 
 static cudaError_t mlc_run(const MlaCachedParams& p, bool prefetch, int device, cudaStream_t stream) {
   if (p.n_items == 0) return cudaSuccess;
-  // Up to 16 heads the codes are multiplied as they are: 148 items x 2048 keys take 49 us for 16 heads, and 77 us for 17,
+  // Up to 16 heads the codes are multiplied as they are: 148 items x 2048 keys take 54 us for 16 heads, and 76 us for 17,
   // which the kernel for 64 heads does (it takes the same time for 1 head as for 64).
   cudaError_t e;
   if (p.n_heads <= kMlcFewHeads) e = mla_cached_few_launch(p, device, stream);
@@ -675,7 +675,9 @@ extern "C" int b200dsa_sparse_mla_decode_cached(const void* q_bf16, const void* 
   p.part = static_cast<float*>(workspace);
   p.status = status;
   // Rows that several items of a request select are in L2 after the first of them; prefetches then only take load slots (2048
-  // items of one request 1788 us with, 1748 without; one item a request 71.7 with, 78.7 without).
+  // items of one request 1788 us with, 1748 without; one item a request 71.7 with, 78.7 without).  The rows of the block table stand for
+  // the requests, which with row_request only the device knows: a table much larger than the call's requests keeps the prefetches.
+  // (The kernel for few heads has none.)
   const bool prefetch = n_items < 4ll * n_requests;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   MlaCachedParams first = p;

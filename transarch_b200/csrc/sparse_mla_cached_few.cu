@@ -29,9 +29,9 @@
 // Work split: CTA = (item, split), as in the other kernel.  Roles (512 threads): warps 0-3 rows (TMA gathers of four rows
 // x 128 bytes straight into the operand layout, the scales by 16-byte asynchronous copies), warp 4 keys, warps 5 and 6 MMAs,
 // warps 8-15 softmax (thread = key, eight heads).  All waits are bounded.  148 items x 16 heads x 2048 keys, every item a
-// request of its own: 49 us (78 us in the kernel for 64 heads); 592 items of 148 requests: 176 us.  A tile takes 2 us: of the
-// 7 k clocks of its chain (rows 2.2, scores 1.3, softmax 1.8, values 1.8) two stages overlap two, and a third does not fit
-// beside P and Q.  Before the gathers (every 16 bytes by an asynchronous copy, 28 bytes a clock) it took 2.5 us.  A
+// request of its own: 53 - 54 us (76 us for 17 heads in the other kernel); 592 items of 148 requests: 196 us.  A tile takes 2.1 us: of
+// the 7.6 k clocks of its chain (rows 2.5, scores 1.3, softmax 2.2, values 1.4) two stages overlap two, and a third does not fit
+// beside P and Q.  (With probabilities of two e4m3 terms and one reference, which were wrong, 49.4 and 174 us.)  A
 // gather takes its issuing lane about 50 clocks: two issuing warps take 2 - 4 % longer, one 14 - 20 %, and a copy of each lane of
 // a warp 90 clocks.  The key warp prefetches no rows: two tiles of copies in flight cover the latency, and its 896 lines a tile take
 // longer than the tile (148 items of as many requests 59.9 us with prefetches, 53.7 without; 64 items x 3 73.1 and 67.7).
