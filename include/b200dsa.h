@@ -682,6 +682,9 @@ int b200dsa_draft_tree_masks(const int32_t* parents, int32_t n_trees, int32_t n_
  *   cache / block_table / page_size as above (block_table [n_requests, table_stride], table_cols entries used);
  *   row_request int32 [n_items], NULL = item i is request i;  indices int32 [n_items, idx_stride], -1 = none;
  *   n_idx_item, q_pos optional;  ctx [n_items, n_heads, 512] bf16 or fp32;  lse fp32 [n_items, n_heads].
+ *   Scores, sums and accumulators are fp32.  Probabilities enter the value products in bf16 (off by 2^-8 of themselves), up to 16
+ *   heads as three e5m2 terms (2^-9 of themselves down to 2^-34 of the largest); there the latent queries are two e4m3 terms
+ *   (off by at most 2^-21 of a row's largest latent value), above 16 heads the bf16 values themselves.
  *   An item without keys gives ctx = 0 and lse = -inf.  A key without a page or outside the cache, and an item whose
  *   request does not exist, are left out and reported (status 2).
  * splits (1..32): every item's keys are cut into that many runs, merged by a second kernel; the caller lends

@@ -157,3 +157,31 @@ def test_queries_with_one_large_dim(H, top):
     out, lse = run_attend(c, ctx=torch.empty(1, H, 512, device=DEV), workspace=(1, None))
     check_range(c, out, lse, [0], query=0)
     assert _status() == 0
+
+
+@pytest.mark.parametrize("H", [2, 16])
+def test_plain_scales_over_a_broad_tail(H):
+    """Scales that are no powers of two: up to 16 heads no row is widened, so nothing more is rounded."""
+    g = torch.Generator().manual_seed(50 + H)
+    for nats, at in ((10.0, 3), (12.0, 1020)):
+        c = range_case(60 + H, H, nats, at, k=1024, scales=(0, -3, 2, -9))
+        sc = c["cache"][:, 512:528].contiguous().view(torch.float32) * (1 + torch.rand(1024, 4, generator=g))
+        c["cache"][:, 512:528] = sc.view(torch.uint8)
+        out, lse = run_attend(c, ctx=torch.empty(1, H, 512, device=DEV), workspace=(1, None))
+        check_range(c, out, lse, [0])
+    assert _status() == 0
+
+
+def test_a_committed_key_over_a_tree_and_a_drafted_one_over_the_selection():
+    """The drafted tokens are one more tile: a key that dominates from either side of it."""
+    for at in (10, 600):                                          # 600: the first drafted position
+        c = range_case(70 + at, 16, 11.0, 0, k=608)
+        pe = torch.rand(608, 1, generator=torch.Generator().manual_seed(at))
+        pe[at] = 11.5
+        c["cache"][:608, 528:530] = pe.bfloat16().view(torch.uint8)
+        sel = torch.arange(600).flip(0).to(torch.int32).view(1, -1)
+        d = dict(c, idx=sel, lens=torch.tensor([600], dtype=torch.int32), mask=torch.tensor([0b10110101]))
+        out, lse = run_attend(d, ctx=torch.empty(1, 16, 512, device=DEV), workspace=(1, None))
+        flat = dict(c, idx=torch.cat([sel, torch.tensor([[600, 602, 604, 605, 607]], dtype=torch.int32)], 1))
+        check_range(flat, out, lse, [0])
+    assert _status() == 0
